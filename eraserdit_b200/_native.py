@@ -19,7 +19,7 @@ from pathlib import Path
 import torch
 
 LIBRARY_PATH = Path(__file__).resolve().parent / "liberaserdit_b200.so"
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 _c_int, _c_i64, _c_float, _vp = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
 
@@ -80,6 +80,10 @@ SIGNATURES = {
                         + [_vp, ctypes.c_size_t, _vp, _vp],
     "erd_attn_fwd_fp8_static_scratch": [_vp, _vp, _vp] + [_c_i64] * 12 + [_c_int] * 4
                                        + [_vp, _c_int, _c_float, _vp] + [_c_i64] * 4 + [_vp, _vp],
+    "erd_head_norm_rotary": [_c_int, _vp, _vp] + [_c_i64] * 6 + [_c_int] * 8
+                            + [_vp, _vp, _c_int, _c_float, _c_float, _vp, _c_float, _c_int,
+                               _c_int, _c_int, _vp, _c_int] + [_c_i64] * 4 + [_vp, _vp]
+                            + [_c_i64] * 6 + [_vp],
 }
 RESTYPES = {"erd_error_string": ctypes.c_char_p, "erd_attn_fp8_workspace_bytes": ctypes.c_size_t,
             "erd_ring_state_bytes": ctypes.c_size_t}
@@ -122,6 +126,34 @@ def check(code: int, what: str) -> None:
 
 def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+# Value type codes of the entry points that take several (ERD_BF16, ...).
+DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def call(name: str, device: torch.device, *args) -> None:
+    """Call an entry point whose last argument is the stream, on ``device``'s
+    current stream with ``device`` current, and raise on its error code."""
+    fn = getattr(load(), name)
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    if rc:
+        check(rc, name)
+
+
+def refuse_gradients(what: str, *tensors) -> None:
+    """The operators have no backward pass: an input that wants a gradient while
+    gradients are recorded is an error, not a silently detached result."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what} has no backward pass: call it under torch.no_grad() or "
+                                 "with detached inputs")
 
 
 _status: dict[int, torch.Tensor] = {}

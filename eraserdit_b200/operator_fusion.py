@@ -15,7 +15,7 @@ from typing import Any
 import torch
 
 from . import _native
-from .rotary import RopeAxisTable
+from .rotary import RopeAxisTable, RotaryPositions, head_rotary_call
 
 QK_RMSNORM_ROPE_OP = "qk_rmsnorm_rope"
 _WIDTH = 2048
@@ -159,3 +159,50 @@ def apply_fused_qk_rmsnorm_rope(query: torch.Tensor, key: torch.Tensor, query_no
     qk_norm_rope_into(query, key, _norm_weight(query_norm), _norm_weight(key_norm),
                       float(query_norm.eps), freqs, q_out, k_out)
     return q_out, k_out
+
+
+def apply_fused_qk_head_rmsnorm_rotary(query: torch.Tensor, key: torch.Tensor | None,
+                                       query_norm: Any, key_norm: Any,
+                                       rotary: RotaryPositions | None,
+                                       positions: torch.Tensor | int = 0, *,
+                                       query_out: torch.Tensor | None = None,
+                                       key_out: torch.Tensor | None = None
+                                       ) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """RMS norm of every head, then the rotation, in one pass over query
+    [B, S, H, D] and key [B, S, Hkv, D] (or None), BF16, FP16 or FP32.
+
+    ``query_norm`` / ``key_norm``: objects with ``eps`` and a ``weight`` [D] (of
+    the inputs' type or FP32; None for 1) without ``bias``, such as
+    ``torch.nn.RMSNorm(D)``.  ``rotary``: a :class:`RotaryPositions`, or None for
+    the norm alone; ``positions`` as in ``rotary.apply_rotary``.  Norm and
+    rotation are computed in FP32 and rounded once (``apply_fused_qk_rmsnorm_rope``,
+    which normalises across all heads, rounds after each step as its reference
+    does).  ``query_out`` / ``key_out`` may be the inputs themselves.
+    """
+    weights, epsilons = [], []
+    for what, x, norm in (("query", query, query_norm), ("key", key, key_norm)):
+        if x is None:
+            weights.append(None)
+            epsilons.append(1.0)
+            continue
+        weight = _norm_weight(norm)
+        if getattr(norm, "bias", None) is not None:
+            raise ValueError(f"{what}_norm must have no bias")
+        eps = getattr(norm, "eps", None)
+        if eps is None:  # torch.nn.RMSNorm's default
+            eps = torch.finfo(x.dtype).eps
+        if not float(eps) >= 0:
+            raise ValueError(f"{what}_norm needs eps >= 0")
+        if weight is not None:
+            if weight.shape != (x.shape[-1],) or not weight.is_contiguous():
+                raise ValueError(f"{what}_norm needs a contiguous weight of one head's width")
+            if weight.dtype not in (x.dtype, torch.float32) or weight.device != x.device:
+                raise ValueError(f"{what}_norm needs a weight of the inputs' type or FP32 on their "
+                                 "device")
+        weights.append(weight)
+        epsilons.append(float(eps))
+    if weights[0] is not None and weights[1] is not None and weights[0].dtype != weights[1].dtype:
+        raise ValueError("query_norm and key_norm need weights of one type")
+    return head_rotary_call("apply_fused_qk_head_rmsnorm_rotary", query, key, rotary, positions,
+                            weights[0], weights[1], True, epsilons[0], epsilons[1], False,
+                            query_out, key_out)

@@ -15,6 +15,7 @@
  *     inside a kernel that timed out (the kernel then returns early instead of
  *     hanging).  The caller reads them after synchronising.
  * BF16 tensors are passed as void* (16-bit words).
+ * Entry points that take several value types name them with the ERD_* codes.
  */
 #ifndef ERASERDIT_B200_H_
 #define ERASERDIT_B200_H_
@@ -26,7 +27,10 @@
 extern "C" {
 #endif
 
-#define ERD_ABI_VERSION 5
+#define ERD_ABI_VERSION 6
+
+/* Value types of the entry points that take a `dtype`. */
+enum { ERD_BF16 = 0, ERD_FP16 = 1, ERD_FP32 = 2 };
 
 /* ABI version probe; replaces eraserdit_mask_sta_abi()
  * (layers/attention/backends/csrc/mask_sta/core.cu:767). */
@@ -406,6 +410,40 @@ int erd_attn_fwd_fp8_static_scratch(
     const int32_t* seg_lens, int head_dim, float softmax_scale, void* out,
     int64_t o_token_stride, int64_t o_head_stride, int64_t o_batch_stride, int64_t o_seg_stride,
     int* status, void* stream);
+
+/*
+ * Rotary positions of query and key heads, optionally behind an RMS norm of
+ * each head, in one pass:
+ *   y = norm ? x * rsqrt(mean(x^2 over the head) + eps) * weight : x
+ *   (y0, y1) -> (y0 c - y1 s, y0 s + y1 c) for each of the rotary_dim / 2 pairs,
+ *   c = amplitude cos(2 pi t), s = amplitude sin(2 pi t) (s negated with
+ *   `inverse`: the transposed rotation), t = position * turns[pair], evaluated
+ *   and reduced in FP64; norm and rotation in FP32, one rounding.
+ * q [batch, tokens, q_heads, head_dim] and k [.., k_heads, ..] of `dtype`
+ * (ERD_BF16, ERD_FP16, ERD_FP32) with a contiguous head (k may be NULL with
+ * k_heads 0); q_out / k_out may be q / k themselves.  Pairs are channels
+ * (2 i, 2 i + 1) with `interleaved`, else (i, i + rotary_dim / 2); channels from
+ * rotary_dim (even, <= head_dim <= 1024) on are not turned.  Weights are
+ * [head_dim] of `dtype`, or FP32 with weight_fp32, or NULL for 1.
+ * Position of token t in batch entry b: int32 (or int64) positions[axis *
+ * pos_axis_stride + b * pos_batch_stride + t * pos_token_stride], or start + t
+ * without positions; axis 1 serves the pairs from second_axis on, axis 2 those
+ * from third_axis on (set both to rotary_dim / 2 for one axis).
+ * Heads that start on 16 bytes and whose turned part is a whole number of
+ * 16-byte chunks take 16-byte accesses; any other size or stride is read value
+ * by value.
+ */
+int erd_head_norm_rotary(
+    int dtype, const void* q, const void* k, int64_t q_token_stride, int64_t q_head_stride,
+    int64_t q_batch_stride, int64_t k_token_stride, int64_t k_head_stride, int64_t k_batch_stride,
+    int batch, int tokens, int q_heads, int k_heads, int head_dim, int rotary_dim, int interleaved,
+    int norm, const void* q_weight, const void* k_weight, int weight_fp32, float q_eps,
+    float k_eps, const double* turns, float amplitude, int inverse, int second_axis,
+    int third_axis, const void* positions, int positions_int64, int64_t pos_axis_stride,
+    int64_t pos_batch_stride, int64_t pos_token_stride, int64_t start, void* q_out, void* k_out,
+    int64_t q_out_token_stride, int64_t q_out_head_stride, int64_t q_out_batch_stride,
+    int64_t k_out_token_stride, int64_t k_out_head_stride, int64_t k_out_batch_stride,
+    void* stream);
 
 #ifdef __cplusplus
 }
