@@ -80,6 +80,8 @@ SIGNATURES = {
                         + [_vp, ctypes.c_size_t, _vp, _vp],
     "erd_attn_fwd_fp8_static_scratch": [_vp, _vp, _vp] + [_c_i64] * 12 + [_c_int] * 4
                                        + [_vp, _c_int, _c_float, _vp] + [_c_i64] * 4 + [_vp, _vp],
+    "erd_linear_act": [_c_int, _vp, _c_i64, _vp, _c_i64, _vp, _c_int, _vp, _c_int, _vp, _c_i64,
+                       _vp, _c_i64, _c_int, _c_int, _c_int, _vp, _vp],
     "erd_head_norm_rotary": [_c_int, _vp, _vp] + [_c_i64] * 6 + [_c_int] * 8
                             + [_vp, _vp, _c_int, _c_float, _c_float, _vp, _c_float, _c_int,
                                _c_int, _c_int, _vp, _c_int] + [_c_i64] * 4 + [_vp, _vp]
@@ -165,8 +167,22 @@ def status_word(device: torch.device) -> torch.Tensor:
     word = _status.get(index)
     if word is None:
         word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+        # zero before any stream's kernel looks at it
+        torch.cuda.current_stream(index).synchronize()
         _status[index] = word
     return word
+
+
+def status_pointer(device: torch.device) -> int:
+    """Address of the device's status word.  It is made by the first call on a
+    device, which can therefore not be one that a CUDA graph records."""
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    word = _status.get(index)
+    if word is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("call the operator once on this device before capturing it")
+        word = status_word(device)
+    return word.data_ptr()
 
 
 def read_status(device: torch.device, reset: bool = True) -> int:

@@ -7,6 +7,10 @@ the sm_100a tensor cores.  It serves the Q/K/V projections of
 (``models/dits/eraserdit_attention.py:248-253``; one product over the
 concatenated weights) and its output projection ``_project_output``
 (``:216-229``).  There is no fallback: an unsupported shape raises.
+
+``linear_act(x, weight, bias, activation=, gate=, residual=)`` is a product of any
+size with the rest of a block's step in its epilogue: ``residual + gate *
+act(x @ weight.T + bias)``, BF16 or FP16 (``erd_linear_act``).
 """
 
 from __future__ import annotations
@@ -112,3 +116,87 @@ def linear_bf16_scatter(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tenso
             x.shape[1], batch_stride, token_stride, _native.status_word(device).data_ptr(),
             _native.stream_handle(device))
     _native.check(rc, "erd_linear_bf16_scatter")
+
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
+
+def _row_view(what: str, t: torch.Tensor) -> tuple[int, int] | None:
+    """``_rows`` with a row stride that fits even where no row follows."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{what} needs a contiguous last dimension")
+    view = _rows(t)
+    if view is not None and view[0] <= 1:
+        return view[0], -(-t.shape[-1] // 8) * 8
+    return view
+
+
+def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
+               activation: str = "none", gate: torch.Tensor | None = None,
+               residual: torch.Tensor | None = None, out: torch.Tensor | None = None
+               ) -> torch.Tensor:
+    """``residual + gate * act(x @ weight.T + bias)`` for BF16 or FP16 CUDA tensors.
+
+    x [..., k], weight [n, k], bias [n]; ``activation``: ``"none"``, ``"relu"``,
+    ``"silu"``, ``"gelu"`` (with the normal distribution function) or
+    ``"gelu_tanh"``; ``gate`` [n], or [g, n] with g dividing the number of rows
+    (one gate per batch entry: consecutive rows / g share one); ``residual`` and
+    ``out`` [..., n], where ``out`` may be ``residual``.  Everything is added up
+    in FP32 and rounded once.  Any sizes; rows of ``x`` and ``weight`` start on 16
+    bytes (row strides, and so a contiguous k, are multiples of 8).
+    """
+    if x.dtype not in (torch.bfloat16, torch.float16) or not x.is_cuda or x.dim() < 1:
+        raise ValueError("linear_act needs a CUDA BF16 or FP16 x")
+    if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or x.shape[-1] == 0:
+        raise ValueError("weight must be [n, k] with k = x.shape[-1] > 0")
+    code = ACTIVATIONS.get(activation)
+    if code is None:
+        raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}")
+    n, k = weight.shape
+    shape = (*x.shape[:-1], n)
+    for what, t in (("weight", weight), ("bias", bias), ("gate", gate), ("residual", residual),
+                    ("out", out)):
+        if t is not None and (t.dtype != x.dtype or t.device != x.device):
+            raise ValueError(f"{what} must have x's type and device")
+    _native.refuse_gradients("linear_act", x, weight, bias, gate, residual)
+    if bias is not None and (bias.shape != (n,) or not bias.is_contiguous()):
+        raise ValueError("bias must be a contiguous [n] tensor")
+    if residual is not None and residual.shape != shape:
+        raise ValueError("residual must be [..., n]")
+    if out is None:
+        out = torch.empty(shape, device=x.device, dtype=x.dtype)
+    elif out.shape != shape or any(s == 0 and d > 1 for s, d in zip(out.stride(), out.shape)):
+        raise ValueError("out must be [..., n] and no expanded view")
+    m = out.numel() // n if n else 0
+    gate_rows = 0
+    if gate is not None:
+        if gate.dim() not in (1, 2) or gate.shape[-1] != n or not gate.is_contiguous():
+            raise ValueError("gate must be a contiguous [n] or [g, n] tensor")
+        groups = 1 if gate.dim() == 1 else gate.shape[0]
+        if m and (groups == 0 or m % groups):
+            raise ValueError("the gate's groups must divide the rows")
+        gate_rows = m // max(groups, 1)
+    if m == 0:
+        return out
+    views = [_row_view("x", x), _row_view("out", out),
+             (0, 0) if residual is None else _row_view("residual", residual)]
+    _, ldw = _row_view("weight", weight)
+    if None in views:
+        # rows that no single stride walks, e.g. prefixes [B, L, k] of wider slots:
+        # one product per leading index
+        if x.dim() < 3 or (gate is not None and gate.dim() == 2 and gate.shape[0] != x.shape[0]):
+            raise ValueError("x, residual and out must be viewable as [rows, last dim] with one "
+                             "row stride")
+        for i in range(x.shape[0]):
+            linear_act(x[i], weight, bias, activation=activation,
+                       gate=gate[i] if gate is not None and gate.dim() == 2 else gate,
+                       residual=None if residual is None else residual[i], out=out[i])
+        return out
+    (_, ldx), (_, ldy), (_, ldr) = views
+    if (x.data_ptr() | weight.data_ptr()) % 16 or ldx % 8 or ldw % 8:
+        raise ValueError("rows of x and weight must start on 16 bytes (strides multiples of 8)")
+    _native.call("erd_linear_act", x.device, _native.DTYPE_CODES[x.dtype], x.data_ptr(), ldx,
+                 weight.data_ptr(), ldw, _native.ptr(bias), code, _native.ptr(gate), gate_rows,
+                 _native.ptr(residual), ldr, out.data_ptr(), ldy, m, n, k,
+                 _native.status_pointer(x.device))
+    return out

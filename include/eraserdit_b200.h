@@ -445,6 +445,30 @@ int erd_head_norm_rotary(
     int64_t k_out_token_stride, int64_t k_out_head_stride, int64_t k_out_batch_stride,
     void* stream);
 
+/*
+ * Matrix product with its epilogue:
+ *   y = residual + gate * act(x W^T + bias),
+ * x [m, k], W [n, k], bias [n] or NULL, residual [m, n] or NULL, y [m, n] of
+ * one `dtype` (ERD_BF16 or ERD_FP16), rows apart by the ld strides (elements);
+ * gate NULL or [ceil(m / gate_rows)][n] contiguous: row i is scaled by gate row
+ * i / gate_rows.  FP32 accumulation and epilogue, one rounding; the order of
+ * the sum is fixed by m, n and k.  m, n and k are free; x, W and their row
+ * strides are 16-byte aligned (y and residual need not be: rows that start on
+ * 16 bytes are just accessed wider).  y may be residual itself.
+ */
+enum {
+  ERD_ACT_NONE = 0,
+  ERD_ACT_RELU = 1,
+  ERD_ACT_SILU = 2,
+  ERD_ACT_GELU = 3,      /* x Phi(x) */
+  ERD_ACT_GELU_TANH = 4  /* x / 2 (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) */
+};
+
+int erd_linear_act(int dtype, const void* x, int64_t ldx, const void* weight, int64_t ldw,
+                   const void* bias, int activation, const void* gate, int gate_rows,
+                   const void* residual, int64_t ld_residual, void* y, int64_t ldy, int m, int n,
+                   int k, int* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
