@@ -4,14 +4,15 @@
 // in FP32, one rounding.  Any row count, any n; rows of x and W start on 16
 // bytes (TMA), k is free.
 //
-// Two kernels, chosen by the host (pick_plan):
+// Three kernels, chosen by the host:
+//   row_kernel    up to two rows: FP32 products of W's stream, no tensor cores.
 //   pair_kernel   large products.  A persistent kernel of CTA pairs
-//                 (cta_group::2), one 256 x 256 tile a pair: each CTA stages
-//                 128 rows of x and 128 rows of W, so an instruction reads half
-//                 of W's tile from either shared memory and a CTA loads 32 KB
-//                 per 64-deep step for 128 x 256 outputs.  An accumulator is
-//                 256 TMEM columns, so two fit, and the epilogue of a tile runs
-//                 beside the products of the next.
+//                 (cta_group::2), one 256 x 256 (or 256 x 128) tile a pair: each
+//                 CTA stages 128 rows of x and half of W's tile, so an
+//                 instruction reads W from both shared memories and a CTA loads
+//                 32 KB per 64-deep step for 128 x 256 outputs.  An accumulator
+//                 is 256 TMEM columns, so two fit, and the epilogue of a tile
+//                 runs beside the products of the next.
 //   split_kernel  few tiles (short row counts, narrow outputs).  One 128 x 64
 //                 or 128 x 128 tile a CTA, the reduction split over the CTAs of
 //                 a cluster, whose FP32 partial sums are added through
@@ -45,6 +46,35 @@ __host__ __device__ constexpr uint32_t idesc(int m, int n) {
   return (1u << 4) | ((kBf16 ? 1u : 0u) << 7) | ((kBf16 ? 1u : 0u) << 10) |
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
+
+// One lane of a converged warp.  The producer and issuer loops run behind this
+// rather than behind `lane == 0`: the compiler then knows that one thread is
+// active and keeps descriptors and barrier addresses in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+
+// Place in a ring of shared-memory stages.
+struct RingPlace {
+  uint32_t s = 0, phase = 0;
+  __device__ __forceinline__ void next(uint32_t stages) {
+    if (++s == stages) {
+      s = 0;
+      phase ^= 1;
+    }
+  }
+  __device__ __forceinline__ void back(uint32_t stages) {
+    if (s == 0) {
+      s = stages;
+      phase ^= 1;
+    }
+    --s;
+  }
+};
 
 // ---------------------------------------------------------------- cluster PTX
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -160,10 +190,34 @@ __device__ __forceinline__ float times_sigmoid(float x, float z) {
 __device__ __forceinline__ float gelu_tanh(float x) {
   return times_sigmoid(x, x * fmaf(0.07135481283f, x * x, 1.5957691216f));
 }
-// gelu with the normal distribution function; erfc keeps the small values of
-// negative arguments that 1 + erf would cancel.
+// exp(z^2) erfc(z) = t P(t), t = 1 / (1 + p z), z >= 0, to 2.5e-7 of itself
+// (the form of Abramowitz and Stegun 7.1.25-26 with a P of degree 7 fitted by
+// gen_erfcx_poly.py); kErfcxP is p / sqrt(2).
+constexpr float kErfcxP = 0x1.33bb9ep-2f;
+constexpr float kErfcx0 = 0x1.eae990p-3f;
+constexpr float kErfcx1 = 0x1.ee7c9cp-3f;
+constexpr float kErfcx2 = 0x1.a0356ap-3f;
+constexpr float kErfcx3 = 0x1.f8f460p-3f;
+constexpr float kErfcx4 = -0x1.638d84p-4f;
+constexpr float kErfcx5 = 0x1.8ecc88p-2f;
+constexpr float kErfcx6 = -0x1.35bb0ap-2f;
+constexpr float kErfcx7 = 0x1.1a2760p-4f;
+// gelu with the normal distribution function, x Phi(x): Phi(-|x|) =
+// erfc(|x| / sqrt(2)) / 2 keeps its digits where 1 + erf would cancel, and
+// costs 17 instructions and 2 MUFU where erfcf made the epilogue of a 2048-deep
+// product longer than its tile's products (2.37 against 1.58 ms).
 __device__ __forceinline__ float gelu_erf(float x) {
-  return 0.5f * x * erfcf(-0.70710678118654752f * x);
+  const float t = __fdividef(1.0f, fmaf(kErfcxP, fabsf(x), 1.0f));
+  float q = fmaf(kErfcx7, t, kErfcx6);
+  q = fmaf(q, t, kErfcx5);
+  q = fmaf(q, t, kErfcx4);
+  q = fmaf(q, t, kErfcx3);
+  q = fmaf(q, t, kErfcx2);
+  q = fmaf(q, t, kErfcx1);
+  q = fmaf(q, t, kErfcx0);
+  const float below = 0.5f * q * t * ex2_approx(-0.72134752044448f * x * x);  // Phi(-|x|)
+  const float y = x * below;
+  return x > 0.f ? x - y : y;
 }
 
 template <int N>
@@ -194,7 +248,7 @@ struct Epilogue {
   long long ld_res;
   void* y;
   long long ldy;
-  int vec_res, vec_y;  // rows start on 16 bytes
+  int vec_bias, vec_gate, vec_res, vec_y;  // rows start on 16 bytes
 };
 
 // Eight values from column `col` of row `row` (what lies behind column n is 0).
@@ -229,58 +283,102 @@ constexpr int kPiece = 64;                    // columns an epilogue warp takes 
 constexpr int kStageBytes = 32 * kPiece * 2;  // 32 rows of a piece, 16-byte chunks swizzled
 constexpr int kSlabBytes = 2 * kPiece * 4;    // bias and gate of a piece as floats
 
-// One warp, 32 rows from row0 (TMEM lanes) x 64 columns from col0.  The
-// residual comes in and the result goes out through a staging block, 128 bytes
-// of a row at a time, so that a warp's access covers four whole lines instead
-// of 32 pieces of 16 bytes.
+// What an epilogue warp reads from global memory for one piece (32 rows x 64
+// columns), requested a piece ahead so that its latency lies under the products
+// or the arithmetic of the piece before.  With the loads behind the wait for
+// the accumulator a gated residual took 2.54 instead of 1.58 ms at 65280 x 8192
+// x 2048.
 template <typename T>
-__device__ __forceinline__ void epilogue_piece(const Epilogue& e, uint32_t taddr, int row0,
-                                               int col0, uint8_t* stage, float* slab, int lane) {
-  const int sub = lane >> 3, chunk = lane & 7;  // row within a group of 4, 16-byte chunk
-  if (e.residual != nullptr) {
+struct Piece {
+  int row0, col0;
+  bool inside;     // every row and column exists and rows start on 16 bytes
+  bool one_group;  // the 32 rows share a gate
+  int group;
+  float b[2], g[2];
+  uint4 res[8];
+
+  __device__ __forceinline__ void request(const Epilogue& e, int row, int col, int lane) {
+    row0 = row;
+    col0 = col;
+    const bool whole = row + 32 <= e.m && col + kPiece <= e.n;
+    inside = whole && e.vec_y && (e.residual == nullptr || e.vec_res);
+    group = 0;
+    one_group = true;
+    if (e.gate != nullptr) {
+      group = min(row + lane, e.m - 1) / e.gate_rows;
+      one_group = __all_sync(0xffffffffu, group == __shfl_sync(0xffffffffu, group, 0));
+    }
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const int rr = 4 * q + sub;
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (row0 + rr < e.m && col0 + chunk * 8 < e.n)
-        v = load8<T>(e.residual, e.ld_res, e.vec_res, row0 + rr, col0 + chunk * 8, e.n);
-      *reinterpret_cast<uint4*>(stage + rr * 128 + ((chunk ^ (rr & 7)) * 16)) = v;
+    for (int i = 0; i < 2; ++i) {
+      const int c = col + lane + 32 * i;
+      b[i] = 0.f;
+      g[i] = 1.f;
+      if (c < e.n) {
+        if (e.bias != nullptr) b[i] = to_float(static_cast<const T*>(e.bias)[c]);
+        if (e.gate != nullptr && one_group)
+          g[i] = to_float(static_cast<const T*>(e.gate)[static_cast<long long>(group) * e.n + c]);
+      }
+    }
+    if (e.residual != nullptr) {
+      const int r = row + (lane >> 3), c = col + (lane & 7) * 8;
+      if (inside) {
+        const T* p = static_cast<const T*>(e.residual) + r * e.ld_res + c;
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          res[q] = *reinterpret_cast<const uint4*>(p + 4 * q * e.ld_res);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          res[q] = make_uint4(0u, 0u, 0u, 0u);
+          if (r + 4 * q < e.m && c < e.n)
+            res[q] = load8<T>(e.residual, e.ld_res, e.vec_res, r + 4 * q, c, e.n);
+        }
+      }
     }
   }
-  const int row = row0 + lane;
-  int group = 0;
-  bool one_group = true;
-  if (e.gate != nullptr) {
-    group = min(row, e.m - 1) / e.gate_rows;
-    one_group = __all_sync(0xffffffffu, group == __shfl_sync(0xffffffffu, group, 0));
-  }
+
+  // First half: the requested values move to shared memory, which frees the
+  // registers for the next request.
+  __device__ __forceinline__ void park(const Epilogue& e, uint8_t* stage, float* slab, int lane) {
+    const int sub = lane >> 3, chunk = lane & 7;  // row within a group of 4, 16-byte chunk
+    if (e.residual != nullptr) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int c = lane + 32 * i;
-    float b = 0.f, g = 1.f;
-    if (col0 + c < e.n) {
-      if (e.bias != nullptr) b = to_float(static_cast<const T*>(e.bias)[col0 + c]);
-      if (e.gate != nullptr && one_group)
-        g = to_float(
-            static_cast<const T*>(e.gate)[static_cast<long long>(group) * e.n + col0 + c]);
+      for (int q = 0; q < 8; ++q) {
+        const int rr = 4 * q + sub;
+        *reinterpret_cast<uint4*>(stage + rr * 128 + ((chunk ^ (rr & 7)) * 16)) = res[q];
+      }
     }
-    slab[c] = b;
-    slab[kPiece + c] = g;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      slab[lane + 32 * i] = b[i];
+      slab[kPiece + lane + 32 * i] = g[i];
+    }
+    __syncwarp();
   }
-  __syncwarp();
-  uint32_t r[kPiece];
-  tmem_ld_wait_64(taddr, r);
+};
+
+// One piece: a lane owns a row of it, adds up its 64 columns from TMEM and the
+// parked values, and leaves the result in the staging block, from where the
+// warp stores 128 bytes of a row at a time (four whole lines an instruction
+// instead of 32 pieces of 16 bytes).
+template <typename T>
+__device__ __forceinline__ void finish_piece(const Epilogue& e, uint32_t taddr, int row0, int col0,
+                                             bool inside, bool one_group, int group,
+                                             uint8_t* stage, const float* slab, int lane) {
+  const int sub = lane >> 3, chunk = lane & 7;
   uint8_t* own = stage + lane * 128;
-#pragma unroll
+#pragma unroll 1
   for (int h = 0; h < 2; ++h) {  // 32 columns at a time
+    uint32_t r[32];
+    tmem_ld_wait_32(taddr + h * 32, r);
     float v[32];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float4 b = reinterpret_cast<const float4*>(slab)[h * 8 + i];
-      v[4 * i] = __uint_as_float(r[h * 32 + 4 * i]) + b.x;
-      v[4 * i + 1] = __uint_as_float(r[h * 32 + 4 * i + 1]) + b.y;
-      v[4 * i + 2] = __uint_as_float(r[h * 32 + 4 * i + 2]) + b.z;
-      v[4 * i + 3] = __uint_as_float(r[h * 32 + 4 * i + 3]) + b.w;
+      v[4 * i] = __uint_as_float(r[4 * i]) + b.x;
+      v[4 * i + 1] = __uint_as_float(r[4 * i + 1]) + b.y;
+      v[4 * i + 2] = __uint_as_float(r[4 * i + 2]) + b.z;
+      v[4 * i + 3] = __uint_as_float(r[4 * i + 3]) + b.w;
     }
     activate(v, e.act);
     if (e.gate != nullptr) {
@@ -294,10 +392,10 @@ __device__ __forceinline__ void epilogue_piece(const Epilogue& e, uint32_t taddr
           v[4 * i + 3] *= g.w;
         }
       } else {  // two groups meet within these 32 rows
-        const T* g = static_cast<const T*>(e.gate) + static_cast<long long>(group) * e.n;
+        const T* g = static_cast<const T*>(e.gate) + static_cast<long long>(group) * e.n + col0;
 #pragma unroll
         for (int i = 0; i < 32; ++i)
-          if (col0 + h * 32 + i < e.n) v[i] *= to_float(g[col0 + h * 32 + i]);
+          if (col0 + h * 32 + i < e.n) v[i] *= to_float(g[h * 32 + i]);
       }
     }
 #pragma unroll
@@ -318,40 +416,56 @@ __device__ __forceinline__ void epilogue_piece(const Epilogue& e, uint32_t taddr
     }
   }
   __syncwarp();
+  const int r = row0 + sub, c = col0 + chunk * 8;
+  if (inside) {
+    T* p = static_cast<T*>(e.y) + r * e.ldy + c;
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    const int rr = 4 * q + sub;
-    if (row0 + rr < e.m && col0 + chunk * 8 < e.n)
-      store8<T>(e.y, e.ldy, e.vec_y, row0 + rr, col0 + chunk * 8, e.n,
-                *reinterpret_cast<const uint4*>(stage + rr * 128 + ((chunk ^ (rr & 7)) * 16)));
+    for (int q = 0; q < 8; ++q)
+      *reinterpret_cast<uint4*>(p + 4 * q * e.ldy) = *reinterpret_cast<const uint4*>(
+          stage + (4 * q + sub) * 128 + ((chunk ^ ((4 * q + sub) & 7)) * 16));
+  } else {
+#pragma unroll 1
+    for (int q = 0; q < 8; ++q) {
+      const int rr = 4 * q + sub;
+      if (row0 + rr < e.m && c < e.n)
+        store8<T>(e.y, e.ldy, e.vec_y, row0 + rr, c, e.n,
+                  *reinterpret_cast<const uint4*>(stage + rr * 128 + ((chunk ^ (rr & 7)) * 16)));
+    }
   }
   __syncwarp();
 }
 
 // ---------------------------------------------------------------- pair kernel
-constexpr int kPairStages = 5;
-constexpr int kPairOperandBytes = 128 * kRowBytes;  // 16 KB of x and of W per CTA and stage
 constexpr int kPairEpilogueWarps = 8;
 constexpr int kPairThreads = 32 * (2 + kPairEpilogueWarps);
-constexpr int kPairTile = 256;  // rows and columns of a pair's tile
+constexpr int kPairRows = 256;                      // rows of a pair's tile
+constexpr int kPairABytes = 128 * kRowBytes;        // x of one CTA and stage
+constexpr int kPairMaxStages = 7;
 
 struct __align__(8) PairBarriers {
-  uint64_t full[kPairStages];   // the leader's: bytes of both CTAs
-  uint64_t empty[kPairStages];  // each CTA's own
-  uint64_t acc_full[2];         // each CTA's own
-  uint64_t acc_empty[2];        // the leader's: every epilogue warp of both CTAs
+  uint64_t full[kPairMaxStages];   // the leader's: bytes of both CTAs
+  uint64_t empty[kPairMaxStages];  // each CTA's own
+  uint64_t acc_full[2];            // each CTA's own
+  uint64_t acc_empty[2];           // the leader's: every epilogue warp of both CTAs
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
 };
 
-constexpr int kPairSmemA = 0;
-constexpr int kPairSmemB = kPairSmemA + kPairStages * kPairOperandBytes;
-constexpr int kPairSmemStage = kPairSmemB + kPairStages * kPairOperandBytes;
-constexpr int kPairSmemSlab = kPairSmemStage + kPairEpilogueWarps * kStageBytes;
-constexpr int kPairSmemBar = kPairSmemSlab + kPairEpilogueWarps * kSlabBytes;
-constexpr int kPairSmemLaunch = kPairSmemBar + 1024 + 1024;  // + base alignment
-static_assert(kPairSmemLaunch <= 227 * 1024, "shared memory budget");
+// Tiles of 256 columns, or of 128 where those end in a nearly empty wave.
+template <int BN>
+struct PairTile {
+  static constexpr int kBBytes = BN / 2 * kRowBytes;  // W of one CTA and stage
+  static constexpr int kStages = BN == 256 ? 5 : 7;
+  static constexpr int kPieces = BN / 2 / 64;         // of an epilogue warp
+  static constexpr int kSmemA = 0;
+  static constexpr int kSmemB = kSmemA + kStages * kPairABytes;
+  static constexpr int kSmemStage = kSmemB + kStages * kBBytes;
+  static constexpr int kSmemSlab = kSmemStage + kPairEpilogueWarps * kStageBytes;
+  static constexpr int kSmemBar = kSmemSlab + kPairEpilogueWarps * kSlabBytes;
+  static constexpr int kSmemLaunch = kSmemBar + 1024 + 1024;  // + base alignment
+  static_assert(kSmemLaunch <= 227 * 1024 && kStages <= kPairMaxStages, "shared memory budget");
+};
 
 struct PairParams {
   Epilogue e;
@@ -359,25 +473,37 @@ struct PairParams {
   int* status;
 };
 
-template <typename T, bool kBf16>
+// Tiles in the order the pairs take them: bands of kBand tile rows, column by
+// column within a band, so that the tiles in flight form a block that reads
+// few distinct rows of x and of W.
+constexpr int kBand = 8;
+__device__ __forceinline__ void tile_place(const PairParams& p, int tile, int& tm, int& tn) {
+  const int band = tile / (kBand * p.tiles_n);
+  const int rows = min(kBand, p.tiles_m - band * kBand);
+  const int r = tile - band * kBand * p.tiles_n;
+  tn = r / rows;
+  tm = band * kBand + r - tn * rows;
+}
+
+template <typename T, bool kBf16, int BN>
 __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
                 const __grid_constant__ CUtensorMap tmap_b, const PairParams p) {
+  using P = PairTile<BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  PairBarriers* bars = reinterpret_cast<PairBarriers*>(smem + kPairSmemBar);
-  const uint32_t sA = smem_u32(smem + kPairSmemA);
-  const uint32_t sB = smem_u32(smem + kPairSmemB);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  PairBarriers* bars = reinterpret_cast<PairBarriers*>(smem + P::kSmemBar);
+  const uint32_t sA = smem_u32(smem + P::kSmemA);
+  const uint32_t sB = smem_u32(smem + P::kSmemB);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int tiles = p.tiles_m * p.tiles_n;
-  const int ksteps = (p.k + kBK - 1) / kBK;
   volatile int* abort = &bars->abort;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kPairStages; ++s) {
+    for (int s = 0; s < P::kStages; ++s) {
       mbar_init(smem_u32(&bars->full[s]), 1);
       mbar_init(smem_u32(&bars->empty[s]), 1);
     }
@@ -390,7 +516,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc_pair(smem_u32(&bars->tmem_base), 512);
+    tmem_alloc_pair(smem_u32(&bars->tmem_base), 2 * BN);
     tmem_relinquish_pair();
   }
   tc_fence_before();
@@ -400,44 +526,53 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
-    if (lane == 0) {
+    if (elect_one()) {
       tma_prefetch_desc(&tmap_a);
       tma_prefetch_desc(&tmap_b);
-      uint32_t it = 0;
+      RingPlace at;
+      uint32_t issued = 0;
       bool ok = true;
+      const uint32_t full0 = smem_u32(&bars->full[0]), empty0 = smem_u32(&bars->empty[0]);
+      const uint32_t leader0 = map_rank(full0, 0);
       for (int tile = pair; ok && tile < tiles; tile += pairs) {
-        const int m0 = (tile / p.tiles_n) * kPairTile + static_cast<int>(rank) * 128;
-        const int n0 = (tile % p.tiles_n) * kPairTile + static_cast<int>(rank) * 128;
-        for (int kk = 0; kk < ksteps; ++kk, ++it) {
-          const uint32_t s = it % kPairStages;
-          const uint32_t ph = (it / kPairStages) & 1;
-          if (!mbar_wait(smem_u32(&bars->empty[s]), ph ^ 1, abort, p.status,
+        int tm, tn;
+        tile_place(p, tile, tm, tn);
+        const int m0 = tm * kPairRows + static_cast<int>(rank) * 128;
+        const int n0 = tn * BN + static_cast<int>(rank) * (BN / 2);
+        for (int k0 = 0; k0 < p.k; k0 += kBK) {
+          if (!mbar_wait(empty0 + 8 * at.s, at.phase ^ 1, abort, p.status,
                          kStatusTimeoutProducer)) {
             ok = false;
             break;
           }
-          const uint32_t full = smem_u32(&bars->full[s]);
           // The leader announces the bytes of both CTAs.  The other CTA's may
           // land first: the phase cannot end before the leader's arrival.
-          if (rank == 0) mbar_arrive_expect_tx(full, 4 * kPairOperandBytes);
-          const uint32_t bar = map_rank(full, 0);
-          tma_load_2d_pair(sA + s * kPairOperandBytes, &tmap_a, bar, kk * kBK, m0);
-          tma_load_2d_pair(sB + s * kPairOperandBytes, &tmap_b, bar, kk * kBK, n0);
+          if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * at.s, 2 * (kPairABytes + P::kBBytes));
+          const uint32_t bar = leader0 + 8 * at.s;
+          tma_load_2d_pair(sA + at.s * kPairABytes, &tmap_a, bar, k0, m0);
+          tma_load_2d_pair(sB + at.s * P::kBBytes, &tmap_b, bar, k0, n0);
+          at.next(P::kStages);
+          ++issued;
         }
       }
       if (*abort && rank == 0) {
         // Let the loads that may be in flight land before exiting.
-        for (int d = 0; d < kPairStages && it > 0; ++d) {
-          --it;
-          mbar_wait_drain(smem_u32(&bars->full[it % kPairStages]), (it / kPairStages) & 1);
+        for (uint32_t d = 0; d < P::kStages && d < issued; ++d) {
+          at.back(P::kStages);
+          mbar_wait_drain(full0 + 8 * at.s, at.phase);
         }
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------- MMA issuer (the leader)
-    if (lane == 0 && rank == 0) {
-      constexpr uint32_t id = idesc<kBf16>(256, 256);
-      uint32_t it = 0, count = 0;
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t id = idesc<kBf16>(256, BN);
+      // Descriptors of stage 0; a stage or 32 bytes of K further is an addition
+      // to the address field (16-byte units).
+      const uint64_t da0 = sdesc_sw128(sA, 16, 1024), db0 = sdesc_sw128(sB, 16, 1024);
+      const uint32_t full0 = smem_u32(&bars->full[0]), empty0 = smem_u32(&bars->empty[0]);
+      RingPlace at;
+      uint32_t count = 0;
       bool ok = true;
       for (int tile = pair; ok && tile < tiles; tile += pairs, ++count) {
         const uint32_t buf = count & 1;
@@ -447,21 +582,23 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
           break;
         }
         tc_fence_after();
-        const uint32_t d = tmem + buf * 256;
-        for (int kk = 0; kk < ksteps; ++kk, ++it) {
-          const uint32_t s = it % kPairStages;
-          const uint32_t ph = (it / kPairStages) & 1;
-          if (!mbar_wait(smem_u32(&bars->full[s]), ph, abort, p.status, kStatusTimeoutMma)) {
+        const uint32_t d = tmem + buf * BN;
+        uint32_t acc = 0;
+        for (int k0 = 0; k0 < p.k; k0 += kBK) {
+          if (!mbar_wait(full0 + 8 * at.s, at.phase, abort, p.status, kStatusTimeoutMma)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a = sA + s * kPairOperandBytes, b = sB + s * kPairOperandBytes;
+          const uint64_t da = da0 + at.s * (kPairABytes / 16);
+          const uint64_t db = db0 + at.s * (P::kBBytes / 16);
 #pragma unroll
-          for (int k4 = 0; k4 < 4; ++k4)
-            mma_pair_ss(d, sdesc_sw128(a + k4 * 32, 16, 1024), sdesc_sw128(b + k4 * 32, 16, 1024),
-                        id, (kk > 0 || k4 > 0) ? 1u : 0u);
-          mma_commit_pair(smem_u32(&bars->empty[s]));
+          for (int k4 = 0; k4 < 4; ++k4) {
+            mma_pair_ss(d, da + 2 * k4, db + 2 * k4, id, acc);
+            acc = 1;
+          }
+          mma_commit_pair(empty0 + 8 * at.s);
+          at.next(P::kStages);
         }
         if (!ok) break;
         mma_commit_pair(smem_u32(&bars->acc_full[buf]));
@@ -473,8 +610,21 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   } else {
     // ------------------------------------------------------------ epilogue
     const int w = warp - 2, quad = warp & 3, half = w >> 2;
-    uint8_t* stage = smem + kPairSmemStage + w * kStageBytes;
-    float* slab = reinterpret_cast<float*>(smem + kPairSmemSlab + w * kSlabBytes);
+    uint8_t* stage = smem + P::kSmemStage + w * kStageBytes;
+    float* slab = reinterpret_cast<float*>(smem + P::kSmemSlab + w * kSlabBytes);
+    // This warp's corner of a tile; pieces without rows or columns are skipped.
+    auto corner = [&](int tile, int& row0, int& col0) {
+      int tm, tn;
+      tile_place(p, tile, tm, tn);
+      row0 = tm * kPairRows + static_cast<int>(rank) * 128 + quad * 32;
+      col0 = tn * BN + half * (BN / 2);
+    };
+    Piece<T> piece;
+    int row0, col0;
+    if (pair < tiles) {
+      corner(pair, row0, col0);
+      if (row0 < p.e.m && col0 < p.e.n) piece.request(p.e, row0, col0, lane);
+    }
     uint32_t count = 0;
     for (int tile = pair; tile < tiles; tile += pairs, ++count) {
       const uint32_t buf = count & 1;
@@ -482,15 +632,25 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
                                              abort, p.status, kStatusTimeoutEpilogue)))
         break;
       tc_fence_after();
-      const int row0 = (tile / p.tiles_n) * kPairTile + static_cast<int>(rank) * 128 + quad * 32;
-      const int col0 = (tile % p.tiles_n) * kPairTile + half * 128;
       const uint32_t taddr =
-          tmem + (static_cast<uint32_t>(quad * 32) << 16) + buf * 256 + half * 128;
-      if (row0 < p.e.m) {
+          tmem + (static_cast<uint32_t>(quad * 32) << 16) + buf * BN + half * (BN / 2);
 #pragma unroll 1
-        for (int c = 0; c < 2; ++c)
-          if (col0 + c * kPiece < p.e.n)
-            epilogue_piece<T>(p.e, taddr + c * kPiece, row0, col0 + c * kPiece, stage, slab, lane);
+      for (int c = 0; c < P::kPieces; ++c) {
+        const bool any = row0 < p.e.m && col0 + c * kPiece < p.e.n;
+        const int row = row0, col = col0 + c * kPiece;
+        const bool inside = piece.inside, one_group = piece.one_group;
+        const int group = piece.group;
+        if (any) piece.park(p.e, stage, slab, lane);
+        // the next piece, of this tile or the next
+        const bool last = c == P::kPieces - 1;
+        if (last && tile + pairs < tiles) corner(tile + pairs, row0, col0);
+        if (!last || tile + pairs < tiles) {
+          const int next = col0 + (last ? 0 : kPiece);
+          if (row0 < p.e.m && next < p.e.n) piece.request(p.e, row0, next, lane);
+        }
+        if (any)
+          finish_piece<T>(p.e, taddr + c * kPiece, row, col, inside, one_group, group, stage, slab,
+                          lane);
       }
       tc_fence_before();
       __syncwarp();
@@ -502,14 +662,17 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc_pair(tmem, 512);
+    tmem_dealloc_pair(tmem, 2 * BN);
   }
 }
 
 // --------------------------------------------------------------- split kernel
 constexpr int kSplitEpilogueWarps = 4;
 constexpr int kSplitThreads = 32 * (2 + kSplitEpilogueWarps);
-constexpr int kSplitMaxStages = 12;
+constexpr int kSplitMaxStages = 20;
+// Clusters of eight leave multiprocessors of a group idle (15 fit at a time
+// with one CTA each), so their CTAs came in two waves.
+constexpr int kMaxSplits = 4;
 
 struct __align__(8) SplitBarriers {
   uint64_t full[kSplitMaxStages];
@@ -525,6 +688,7 @@ struct SplitParams {
   int a_rows;   // rows of the x box (a multiple of 8, at most 128)
   int stages;   // ring depth that fits the shared memory of this launch
   int splits;   // CTAs of a cluster: parts of the reduction
+  int direct;   // one part whose warps finish their rows from TMEM
   int tail;     // offset of the staging blocks and barriers
   int* status;
 };
@@ -542,6 +706,19 @@ struct SplitSmem {
       kSplitEpilogueWarps * (kStageBytes + kSlabBytes) + 1024;  // staging, slabs, barriers
 };
 
+// Bias, gate and residual of eight columns of one row.
+template <typename T>
+struct Side {
+  uint4 bias, gate, res;
+  __device__ __forceinline__ void request(const Epilogue& e, int row, int col) {
+    bias = gate = res = make_uint4(0u, 0u, 0u, 0u);
+    if (e.bias != nullptr) bias = load8<T>(e.bias, 0, e.vec_bias, 0, col, e.n);
+    if (e.gate != nullptr)
+      gate = load8<T>(e.gate, e.n, e.vec_gate, row / e.gate_rows, col, e.n);
+    if (e.residual != nullptr) res = load8<T>(e.residual, e.ld_res, e.vec_res, row, col, e.n);
+  }
+};
+
 // 16-byte chunk `c4` of row `r` of the partial sums, swizzled so that the 32
 // rows a warp writes at a time do not meet in the same banks.
 template <int BN>
@@ -550,7 +727,7 @@ __device__ __forceinline__ int partial_offset(int r, int c4) {
 }
 
 template <typename T, bool kBf16, int BN>
-__global__ void __launch_bounds__(kSplitThreads)
+__global__ void __launch_bounds__(kSplitThreads, 1)
     split_kernel(const __grid_constant__ CUtensorMap tmap_a,
                  const __grid_constant__ CUtensorMap tmap_b, const SplitParams p) {
   using S = SplitSmem<BN>;
@@ -563,7 +740,7 @@ __global__ void __launch_bounds__(kSplitThreads)
       tail + kSplitEpilogueWarps * (kStageBytes + kSlabBytes));
   const uint32_t sA = smem_u32(smem);
   const uint32_t sB = sA + p.stages * a_bytes;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int split = blockIdx.x % p.splits;  // also the rank in the cluster
   const int tile = blockIdx.x / p.splits;
   const int m0 = (tile / p.tiles_n) * 128, n0 = (tile % p.tiles_n) * BN;
@@ -590,51 +767,73 @@ __global__ void __launch_bounds__(kSplitThreads)
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
 
+  // Unless the accumulator is finished in place: the eight-column chunks of the
+  // tile that this CTA finishes; what a thread's first one needs is requested now.
+  const int chunks = min(128, p.e.m - m0) * (BN / 8);
+  const int share_lo = static_cast<int>(static_cast<long long>(chunks) * split / p.splits);
+  const int share_hi = static_cast<int>(static_cast<long long>(chunks) * (split + 1) / p.splits);
+  Side<T> side;
+  if (!p.direct) {
+    const int i = share_lo + static_cast<int>(threadIdx.x);
+    if (i < share_hi && n0 + i % (BN / 8) * 8 < p.e.n)
+      side.request(p.e, m0 + i / (BN / 8), n0 + i % (BN / 8) * 8);
+  }
+
   bool have = false;  // this warp's rows of the accumulator may be read
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t tx = static_cast<uint32_t>(p.a_rows * kRowBytes + S::kBBytes);
-      int it = 0;
-      for (int kk = k_lo; kk < k_hi; ++kk, ++it) {
-        const int s = it % p.stages;
-        const uint32_t ph = (it / p.stages) & 1;
-        if (!mbar_wait(smem_u32(&bars->empty[s]), ph ^ 1, abort, p.status,
-                       kStatusTimeoutProducer))
+      const uint32_t full0 = smem_u32(&bars->full[0]), empty0 = smem_u32(&bars->empty[0]);
+      const uint32_t stages = static_cast<uint32_t>(p.stages);
+      RingPlace at;
+      uint32_t issued = 0;
+      for (int kk = k_lo; kk < k_hi; ++kk) {
+        if (!mbar_wait(empty0 + 8 * at.s, at.phase ^ 1, abort, p.status, kStatusTimeoutProducer))
           break;
-        const uint32_t full = smem_u32(&bars->full[s]);
+        const uint32_t full = full0 + 8 * at.s;
         mbar_arrive_expect_tx(full, tx);
-        tma_load_2d(sB + s * S::kBBytes, &tmap_b, full, kk * kBK, n0);
-        tma_load_2d(sA + s * a_bytes, &tmap_a, full, kk * kBK, m0);
+        tma_load_2d(sB + at.s * S::kBBytes, &tmap_b, full, kk * kBK, n0);
+        tma_load_2d(sA + at.s * a_bytes, &tmap_a, full, kk * kBK, m0);
+        at.next(stages);
+        ++issued;
       }
       if (*abort) {
-        for (int d = 0; d < p.stages && it > 0; ++d) {
-          --it;
-          mbar_wait_drain(smem_u32(&bars->full[it % p.stages]), (it / p.stages) & 1);
+        for (uint32_t d = 0; d < stages && d < issued; ++d) {
+          at.back(stages);
+          mbar_wait_drain(full0 + 8 * at.s, at.phase);
         }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t id = idesc<kBf16>(128, BN);
-      for (int kk = k_lo, it = 0; kk < k_hi; ++kk, ++it) {
-        const int s = it % p.stages;
-        const uint32_t ph = (it / p.stages) & 1;
-        if (!mbar_wait(smem_u32(&bars->full[s]), ph, abort, p.status, kStatusTimeoutMma)) break;
+      const uint64_t da0 = sdesc_sw128(sA, 16, 1024), db0 = sdesc_sw128(sB, 16, 1024);
+      const uint32_t full0 = smem_u32(&bars->full[0]), empty0 = smem_u32(&bars->empty[0]);
+      const uint32_t stages = static_cast<uint32_t>(p.stages);
+      RingPlace at;
+      uint32_t acc = 0;
+      for (int kk = k_lo; kk < k_hi; ++kk) {
+        if (!mbar_wait(full0 + 8 * at.s, at.phase, abort, p.status, kStatusTimeoutMma)) break;
         tc_fence_after();
-        const uint32_t a = sA + s * a_bytes, b = sB + s * S::kBBytes;
+        const uint64_t da = da0 + at.s * static_cast<uint32_t>(a_bytes / 16);
+        const uint64_t db = db0 + at.s * (S::kBBytes / 16);
         // Rows of the product beyond the x box read whatever the shared memory
         // behind it holds; their accumulator lanes are never read.
 #pragma unroll
         for (int k4 = 0; k4 < 4; ++k4) {
-          mma_bf16_ss(tmem, sdesc_sw128(a + k4 * 32, 16, 1024), sdesc_sw128(b + k4 * 32, 16, 1024),
-                      id, (it > 0 || k4 > 0) ? 1u : 0u);
+          mma_bf16_ss(tmem, da + 2 * k4, db + 2 * k4, id, acc);
+          acc = 1;
         }
-        mma_commit(smem_u32(&bars->empty[s]));
+        mma_commit(empty0 + 8 * at.s);
+        at.next(stages);
       }
       mma_commit(smem_u32(&bars->acc_full));
       mbar_wait_drain(smem_u32(&bars->acc_full), 0);
     }
   } else {
+    Piece<T> piece;
+    const int first_row = m0 + (warp & 3) * 32;
+    if (p.direct && first_row < p.e.m) piece.request(p.e, first_row, n0, lane);
     have = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->acc_full), 0, abort, p.status,
                                              kStatusTimeoutEpilogue));
     // A reduction that was cut short has set the flag before it committed.
@@ -644,14 +843,21 @@ __global__ void __launch_bounds__(kSplitThreads)
     const int row0 = m0 + quad * 32;
     const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     if (have && row0 < p.e.m) {
-      if (p.splits == 1) {
+      if (p.direct) {
         uint8_t* stage = tail + (warp - 2) * kStageBytes;
         float* slab = reinterpret_cast<float*>(tail + kSplitEpilogueWarps * kStageBytes +
                                                (warp - 2) * kSlabBytes);
 #pragma unroll 1
-        for (int c = 0; c < BN; c += kPiece)
-          if (n0 + c < p.e.n)
-            epilogue_piece<T>(p.e, taddr + c, row0, n0 + c, stage, slab, lane);
+        for (int c = 0; c < BN; c += kPiece) {
+          if (n0 + c >= p.e.n) break;
+          const bool inside = piece.inside, one_group = piece.one_group;
+          const int group = piece.group;
+          piece.park(p.e, stage, slab, lane);
+          if (c + kPiece < BN && n0 + c + kPiece < p.e.n)
+            piece.request(p.e, row0, n0 + c + kPiece, lane);
+          finish_piece<T>(p.e, taddr + c, row0, n0 + c, inside, one_group, group, stage, slab,
+                          lane);
+        }
       } else {
         // The ring is free: every load has been consumed by a finished product.
         const int r = quad * 32 + lane;
@@ -670,54 +876,59 @@ __global__ void __launch_bounds__(kSplitThreads)
     }
   }
   tc_fence_before();
-  if (p.splits == 1) {
+  if (p.direct) {
     __syncthreads();
   } else {
     cluster_sync();
     // Each CTA adds and finishes its share of the tile, eight columns a thread.
     // A split that gave up has set the status word; its partial sums are stale
     // and the tile's values are then as undefined as those of any timed-out call.
-    const int rows = min(128, p.e.m - m0);
-    const int total = rows * (BN / 8);
-    const int lo = static_cast<int>(static_cast<long long>(total) * split / p.splits);
-    const int hi = static_cast<int>(static_cast<long long>(total) * (split + 1) / p.splits);
     const uint32_t base = smem_u32(smem);
-    for (int i = lo + static_cast<int>(threadIdx.x); i < hi; i += kSplitThreads) {
+    for (int i = share_lo + static_cast<int>(threadIdx.x); i < share_hi; i += kSplitThreads) {
       const int r = i / (BN / 8), c8 = i % (BN / 8);
       const int row = m0 + r, col = n0 + c8 * 8;
       if (col >= p.e.n) continue;
+      // All requests first: one round trip over the cluster, not one per part.
+      float4 a[kMaxSplits], b[kMaxSplits];
+#pragma unroll
+      for (int s = 0; s < kMaxSplits; ++s) {
+        if (s < p.splits) {
+          const uint32_t peer = map_rank(base, static_cast<uint32_t>(s));
+          a[s] = ld_cluster(peer + partial_offset<BN>(r, c8 * 2));
+          b[s] = ld_cluster(peer + partial_offset<BN>(r, c8 * 2 + 1));
+        }
+      }
+      if (i >= share_lo + kSplitThreads) side.request(p.e, row, col);
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = 0.f;
-      for (int s = 0; s < p.splits; ++s) {
-        const uint32_t peer = map_rank(base, static_cast<uint32_t>(s));
-        const float4 a = ld_cluster(peer + partial_offset<BN>(r, c8 * 2));
-        const float4 b = ld_cluster(peer + partial_offset<BN>(r, c8 * 2 + 1));
-        v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
-        v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
-      }
-      if (p.e.bias != nullptr) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (col + j < p.e.n) v[j] += to_float(static_cast<const T*>(p.e.bias)[col + j]);
+      for (int s = 0; s < kMaxSplits; ++s) {
+        if (s < p.splits) {
+          v[0] += a[s].x, v[1] += a[s].y, v[2] += a[s].z, v[3] += a[s].w;
+          v[4] += b[s].x, v[5] += b[s].y, v[6] += b[s].z, v[7] += b[s].w;
+        }
+      }
+      const uint32_t bias[4] = {side.bias.x, side.bias.y, side.bias.z, side.bias.w};
+      const uint32_t gate[4] = {side.gate.x, side.gate.y, side.gate.z, side.gate.w};
+      const uint32_t res[4] = {side.res.x, side.res.y, side.res.z, side.res.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = unpack2<T>(bias[j]);
+        v[2 * j] += f.x;
+        v[2 * j + 1] += f.y;
       }
       activate(v, p.e.act);
-      if (p.e.gate != nullptr) {
-        const T* g = static_cast<const T*>(p.e.gate) +
-                     static_cast<long long>(row / p.e.gate_rows) * p.e.n + col;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (col + j < p.e.n) v[j] *= to_float(g[j]);
-      }
-      if (p.e.residual != nullptr) {
-        const uint4 w = load8<T>(p.e.residual, p.e.ld_res, p.e.vec_res, row, col, p.e.n);
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = unpack2<T>(ww[j]);
-          v[2 * j] += f.x;
-          v[2 * j + 1] += f.y;
+      for (int j = 0; j < 4; ++j) {
+        if (p.e.gate != nullptr) {
+          const float2 g = unpack2<T>(gate[j]);
+          v[2 * j] *= g.x;
+          v[2 * j + 1] *= g.y;
         }
+        const float2 f = unpack2<T>(res[j]);
+        v[2 * j] += f.x;
+        v[2 * j + 1] += f.y;
       }
       store8<T>(p.e.y, p.e.ldy, p.e.vec_y, row, col, p.e.n,
                 make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]),
@@ -732,39 +943,205 @@ __global__ void __launch_bounds__(kSplitThreads)
   }
 }
 
+// ----------------------------------------------------------------- row kernel
+// A few rows (at most 2) are a stream over W: a warp takes four columns (rows
+// of W), its lanes 16 bytes of each at a time, and multiplies them with every
+// row of x in FP32.  No barrier, TMEM or cluster set-up stands before the first
+// load.  The reduction may be shared by several warps of the block (their sums
+// are added in warp order).
+constexpr int kRowWarps = 8;
+constexpr int kRowCols = 4;
+constexpr int kRowMax = 2;
+
+template <typename T, int M>
+__global__ void __launch_bounds__(32 * kRowWarps)
+    row_kernel(const Epilogue e, const T* __restrict__ x, long long ldx, const T* __restrict__ w,
+               long long ldw, int k, int share) {
+  constexpr int V = M * kRowCols;  // sums of a warp
+  __shared__ float sums[kRowWarps][V];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = warp % share;
+  const int col0 =
+      static_cast<int>(blockIdx.x * (kRowWarps / share) + warp / share) * kRowCols;
+  const T* wr[kRowCols];
+  const T* xr[M];
+#pragma unroll
+  for (int r = 0; r < kRowCols; ++r) wr[r] = w + min(col0 + r, e.n - 1) * ldw;
+#pragma unroll
+  for (int i = 0; i < M; ++i) xr[i] = x + min(i, e.m - 1) * ldx;
+  float acc[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] = 0.f;
+
+  auto add = [&](const uint4 (&wv)[kRowCols], const uint4 (&xv)[M]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float2 wf[kRowCols];
+#pragma unroll
+      for (int r = 0; r < kRowCols; ++r)
+        wf[r] = unpack2<T>(q == 0 ? wv[r].x : q == 1 ? wv[r].y : q == 2 ? wv[r].z : wv[r].w);
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        const float2 xf =
+            unpack2<T>(q == 0 ? xv[i].x : q == 1 ? xv[i].y : q == 2 ? xv[i].z : xv[i].w);
+#pragma unroll
+        for (int r = 0; r < kRowCols; ++r)
+          acc[i * kRowCols + r] =
+              fmaf(xf.y, wf[r].y, fmaf(xf.x, wf[r].x, acc[i * kRowCols + r]));
+      }
+    }
+  };
+  const int chunks = k / 8, step = 32 * share;
+  int c = part * 32 + lane;
+  constexpr int U = 4;  // chunks requested at a time
+#pragma unroll 1
+  for (; c + (U - 1) * step < chunks; c += U * step) {
+    uint4 wv[U][kRowCols], xv[U][M];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int r = 0; r < kRowCols; ++r)
+        wv[u][r] = *reinterpret_cast<const uint4*>(wr[r] + (c + u * step) * 8LL);
+#pragma unroll
+      for (int i = 0; i < M; ++i)
+        xv[u][i] = *reinterpret_cast<const uint4*>(xr[i] + (c + u * step) * 8LL);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) add(wv[u], xv[u]);
+  }
+#pragma unroll 1
+  for (; c < chunks; c += step) {
+    uint4 wv[kRowCols], xv[M];
+#pragma unroll
+    for (int r = 0; r < kRowCols; ++r) wv[r] = *reinterpret_cast<const uint4*>(wr[r] + c * 8LL);
+#pragma unroll
+    for (int i = 0; i < M; ++i) xv[i] = *reinterpret_cast<const uint4*>(xr[i] + c * 8LL);
+    add(wv, xv);
+  }
+  if (part == 0 && lane < k - chunks * 8) {  // what lies behind k may not be read
+    const int kk = chunks * 8 + lane;
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+      for (int r = 0; r < kRowCols; ++r)
+        acc[i * kRowCols + r] =
+            fmaf(to_float(xr[i][kk]), to_float(wr[r][kk]), acc[i * kRowCols + r]);
+  }
+  // Sums over the lanes: halve the values a lane is responsible for while there
+  // are several, then add what is left; value i ends in the lanes whose top
+  // log2(V) bits are i.
+  int left = V, mine = 0;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    if (left > 1) {
+      left /= 2;
+      const bool hi = (lane & d) != 0;
+      mine += hi ? left : 0;
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        if (i < left) {
+          const float keep = hi ? acc[i + left] : acc[i];
+          const float give = hi ? acc[i] : acc[i + left];
+          acc[i] = keep + __shfl_xor_sync(0xffffffffu, give, d);
+        }
+      }
+    } else {
+      acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], d);
+    }
+  }
+  constexpr int kDup = 32 / V;  // lanes that hold the same value
+  if (share > 1) {
+    if (lane % kDup == 0) sums[warp][mine] = acc[0];
+    __syncthreads();
+    if (part != 0) return;
+    acc[0] = 0.f;
+    for (int s = 0; s < share; ++s) acc[0] += sums[warp + s][mine];
+  }
+  const int row = mine / kRowCols, col = col0 + mine % kRowCols;
+  if (lane % kDup != 0 || row >= e.m || col >= e.n) return;
+  float v[1] = {acc[0]};
+  if (e.bias != nullptr) v[0] += to_float(static_cast<const T*>(e.bias)[col]);
+  activate(v, e.act);
+  if (e.gate != nullptr)
+    v[0] *= to_float(static_cast<const T*>(e.gate)[static_cast<long long>(row / e.gate_rows) * e.n +
+                                                   col]);
+  if (e.residual != nullptr) v[0] += to_float(static_cast<const T*>(e.residual)[row * e.ld_res + col]);
+  const uint32_t packed = pack2<T>(v[0], 0.f);
+  static_cast<uint16_t*>(e.y)[row * e.ldy + col] = static_cast<uint16_t>(packed);
+}
+
 // ------------------------------------------------------------------ host side
 struct Plan {
   bool pair;
   int bn, splits, a_rows;
 };
 
-// Which kernel, and how a small product is cut.
+// Which kernel for more than kRowMax rows, and how a small product is cut: the
+// least estimated time, in clocks, of
+//   the pair kernel: 512 (256 columns) or 400 a 64-deep step and tile, whole waves
+//   of sms / 2 tiles;
+//   the split kernel with 64 or 128 columns and 1, 2 or 4 parts, one wave of CTAs
+//   (its steps wait for L2, and parts add a round trip through the cluster).
 Plan pick_plan(int m, int n, int k, int sms) {
-  Plan pl = {};
-  const long long tiles_pair = static_cast<long long>((m + 255) / 256) * ((n + 255) / 256);
-  if (tiles_pair * 2 >= sms) {
-    pl.pair = true;
-    return pl;
+  const long long ksteps = (k + kBK - 1) / kBK;
+  auto waves = [](long long tiles, long long at_once) { return (tiles + at_once - 1) / at_once; };
+  Plan best = {};
+  long long least = -1;
+  auto offer = [&](bool pair, int bn, int splits, long long cost) {
+    if (least >= 0 && cost >= least) return;
+    least = cost;
+    best.pair = pair;
+    best.bn = bn;
+    best.splits = splits;
+  };
+  for (int bn = 256; bn >= 128; bn -= 128) {
+    const long long tiles = ((m + 255LL) / 256) * ((n + bn - 1LL) / bn);
+    offer(true, bn, 1, waves(tiles, sms / 2) * ksteps * (bn == 256 ? 512 : 400) + 9000);
   }
-  const int ksteps = (k + kBK - 1) / kBK;
-  const long long tm = (m + 127) / 128;
-  const long long t128 = tm * ((n + 127) / 128), t64 = tm * ((n + 63) / 64);
-  pl.bn = t128 >= sms ? 128 : 64;
-  const long long tiles = pl.bn == 128 ? t128 : t64;
-  pl.splits = 1;
-  while (pl.splits < 8 && tiles * pl.splits * 2 <= 2LL * sms && ksteps / (pl.splits * 2) >= 4)
-    pl.splits *= 2;
-  pl.a_rows = m >= 128 ? 128 : (m + 7) / 8 * 8;
-  return pl;
+  for (int bn = 64; bn <= 128; bn += 64) {
+    const long long tiles = ((m + 127LL) / 128) * ((n + bn - 1LL) / bn);
+    for (int splits = 1; splits <= kMaxSplits; splits *= 2) {
+      if (splits > 1 && (ksteps < 4 * splits || tiles * splits > sms)) break;
+      const long long steps = (ksteps + splits - 1) / splits;
+      offer(false, bn, splits,
+            waves(tiles * splits, sms) * (steps * (bn == 64 ? 270 : 300) + 3000) + 3000 +
+                (splits > 1 ? 2500 : 0));
+    }
+  }
+  best.a_rows = m >= 128 ? 128 : (m + 7) / 8 * 8;
+  return best;
+}
+
+template <typename T, bool kBf16, int BN>
+int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, PairParams p, int sms,
+                cudaStream_t st) {
+  using P = PairTile<BN>;
+  const long long tm = (p.e.m + 255LL) / 256, tn = (p.e.n + BN - 1LL) / BN;
+  if (tm * tn > (1LL << 30)) return kErrTooLarge;
+  p.tiles_m = static_cast<int>(tm);
+  p.tiles_n = static_cast<int>(tn);
+  cudaError_t e = cudaFuncSetAttribute(pair_kernel<T, kBf16, BN>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, P::kSmemLaunch);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const long long pairs = tm * tn < sms / 2 ? tm * tn : sms / 2;
+  pair_kernel<T, kBf16, BN>
+      <<<static_cast<unsigned>(2 * pairs), kPairThreads, P::kSmemLaunch, st>>>(ta, tb, p);
+  return static_cast<int>(cudaGetLastError());
 }
 
 template <typename T, bool kBf16, int BN>
 int launch_split(const CUtensorMap& ta, const CUtensorMap& tb, SplitParams p, const Plan& pl,
                  cudaStream_t st) {
   using S = SplitSmem<BN>;
+  // Few rows or several parts: all threads finish eight-column chunks of the sums
+  // in shared memory (few rows would leave a whole piece to one or two warps,
+  // some 3500 clocks).
+  p.direct = pl.splits == 1 && p.e.m > 64;
   const int ksteps = (p.k + kBK - 1) / kBK;
   const int per_split = (ksteps + pl.splits - 1) / pl.splits;
-  const int budget = 112 * 1024 - S::kTail - 1024;  // two CTAs on a multiprocessor
+  // One CTA a multiprocessor with as deep a ring as fits: three stages (two CTAs
+  // a multiprocessor) left 0.47 us of load latency in every 64-deep step.
+  const int budget = 227 * 1024 - S::kTail - 1024;
   p.stages = budget / S::ring(pl.a_rows, 1);
   if (p.stages > kSplitMaxStages) p.stages = kSplitMaxStages;
   if (p.stages > per_split) p.stages = per_split;
@@ -773,7 +1150,7 @@ int launch_split(const CUtensorMap& ta, const CUtensorMap& tb, SplitParams p, co
   p.tail = S::ring(pl.a_rows, p.stages);
   const int reach = (p.stages - 1) * S::a_bytes(pl.a_rows) + 128 * kRowBytes;
   if (p.tail < reach) p.tail = reach;
-  if (pl.splits > 1 && p.tail < 128 * BN * 4) p.tail = 128 * BN * 4;
+  if (!p.direct && p.tail < 128 * BN * 4) p.tail = 128 * BN * 4;
   const int bytes = p.tail + S::kTail + 1024;  // + base alignment
   cudaError_t e = cudaFuncSetAttribute(split_kernel<T, kBf16, BN>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
@@ -812,22 +1189,32 @@ int run(const Epilogue& e, const void* x, int64_t ldx, const void* w, int64_t ld
   cudaError_t err = cudaGetDevice(&dev);
   if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (err != cudaSuccess) return static_cast<int>(err);
-  Plan pl = pick_plan(e.m, e.n, k, sms);
+  if (e.m <= kRowMax) {
+    // Enough warps to fill the device, each with two chunks a lane at least.
+    const int groups = (e.n + kRowCols - 1) / kRowCols;
+    int share = 1;
+    while (share < kRowWarps && static_cast<long long>(groups) * share < 16LL * sms &&
+           k >= 32 * 8 * 4 * share)
+      share *= 2;
+    const unsigned blocks =
+        static_cast<unsigned>((groups + kRowWarps / share - 1) / (kRowWarps / share));
+    const T* xt = static_cast<const T*>(x);
+    const T* wt = static_cast<const T*>(w);
+    if (e.m == 1)
+      row_kernel<T, 1><<<blocks, 32 * kRowWarps, 0, st>>>(e, xt, ldx, wt, ldw, k, share);
+    else
+      row_kernel<T, 2><<<blocks, 32 * kRowWarps, 0, st>>>(e, xt, ldx, wt, ldw, k, share);
+    return static_cast<int>(cudaGetLastError());
+  }
+  const Plan pl = pick_plan(e.m, e.n, k, sms);
   CUtensorMap ta, tb;
   if (pl.pair) {
-    const long long tm = (e.m + 255) / 256, tn = (e.n + 255) / 256;
-    if (tm * tn > (1LL << 30)) return kErrTooLarge;
     if (operand_map(&ta, kBf16, x, e.m, k, ldx, 128) ||
-        operand_map(&tb, kBf16, w, e.n, k, ldw, 128))
+        operand_map(&tb, kBf16, w, e.n, k, ldw, pl.bn / 2))
       return kErrTensorMap;
-    PairParams p = {e, k, static_cast<int>(tm), static_cast<int>(tn), status};
-    err = cudaFuncSetAttribute(pair_kernel<T, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               kPairSmemLaunch);
-    if (err != cudaSuccess) return static_cast<int>(err);
-    const long long pairs = tm * tn < sms / 2 ? tm * tn : sms / 2;
-    pair_kernel<T, kBf16>
-        <<<static_cast<unsigned>(2 * pairs), kPairThreads, kPairSmemLaunch, st>>>(ta, tb, p);
-    return static_cast<int>(cudaGetLastError());
+    const PairParams p = {e, k, 0, 0, status};
+    return pl.bn == 256 ? launch_pair<T, kBf16, 256>(ta, tb, p, sms, st)
+                        : launch_pair<T, kBf16, 128>(ta, tb, p, sms, st);
   }
   if (operand_map(&ta, kBf16, x, e.m, k, ldx, pl.a_rows) ||
       operand_map(&tb, kBf16, w, e.n, k, ldw, pl.bn))
@@ -874,6 +1261,8 @@ extern "C" int erd_linear_act(int dtype, const void* x, int64_t ldx, const void*
   e.ld_res = ld_residual;
   e.y = y;
   e.ldy = ldy;
+  e.vec_bias = aligned16(bias);
+  e.vec_gate = aligned16(gate) && (n & 7) == 0;
   e.vec_res = aligned16(residual) && (ld_residual & 7) == 0;
   e.vec_y = aligned16(y) && (ldy & 7) == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
