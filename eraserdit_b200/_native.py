@@ -80,6 +80,12 @@ SIGNATURES = {
                         + [_vp, ctypes.c_size_t, _vp, _vp],
     "erd_attn_fwd_fp8_static_scratch": [_vp, _vp, _vp] + [_c_i64] * 12 + [_c_int] * 4
                                        + [_vp, _c_int, _c_float, _vp] + [_c_i64] * 4 + [_vp, _vp],
+    "erd_block_topk_workspace_bytes": [_c_int] * 8,
+    "erd_block_topk_attn": [_c_int, _vp, _vp, _vp] + [_c_i64] * 9 + [_c_int] * 6
+                           + [_vp, _vp, _c_int, _c_int, _c_int, _c_float, _vp] + [_c_i64] * 3
+                           + [_vp, _vp, ctypes.c_size_t, _vp, _vp],
+    "erd_block_key_means": [_c_int, _vp, _c_i64, _c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int,
+                            _vp, _vp, _vp],
     "erd_linear_act": [_c_int, _vp, _c_i64, _vp, _c_i64, _vp, _c_int, _vp, _c_int, _vp, _c_i64,
                        _vp, _c_i64, _c_int, _c_int, _c_int, _vp, _vp],
     "erd_head_norm_rotary": [_c_int, _vp, _vp] + [_c_i64] * 6 + [_c_int] * 8
@@ -88,7 +94,8 @@ SIGNATURES = {
                             + [_c_i64] * 6 + [_vp],
 }
 RESTYPES = {"erd_error_string": ctypes.c_char_p, "erd_attn_fp8_workspace_bytes": ctypes.c_size_t,
-            "erd_ring_state_bytes": ctypes.c_size_t}
+            "erd_ring_state_bytes": ctypes.c_size_t,
+            "erd_block_topk_workspace_bytes": ctypes.c_size_t}
 
 _lib = None
 _lock = threading.Lock()

@@ -1,0 +1,1182 @@
+// Attention over key blocks that a cheap score selects, head_dim 64, BF16 or
+// FP16 on sm_100a:
+//   score(I, J) = (sum_{i in I} q_i) . mean_{j in J, j < length} k_j     (FP64)
+//   each query block I keeps its `topk` highest-scoring key blocks (ties: the
+//   lowest index), and its queries attend the valid keys of those blocks.
+// A query block is 128 queries (one tile of the tensor cores) or one query.
+//
+// The scores are sums in 64 bits so that the choice does not depend on the
+// order of summation: sums of 64 or 128 16-bit values are exact or nearly so,
+// and two blocks change places only where their scores agree to 1e-15.
+//
+// Steps (all on the caller's stream):
+//   pool_kernel     one pass over k (and, for blocks of 128, q): block sums.
+//                   Bound by memory; a caller that keeps the key means next to
+//                   its keys (key_pool) skips it for single queries.
+//   score_kernel    blocks of 128: scores = sums times means, FP64 tiles.
+//   select_kernel   blocks of 128: one warp a row finds the topk-th key by
+//                   bisection over the bits of the scores.
+//   row_select_kernel   single queries: scores and choice in one CTA a row.
+//   tile_attn_kernel    blocks of 128: tcgen05 attention over the chosen blocks.
+//   row_attn_kernel     single queries: a stream over the chosen blocks, split
+//                   over a cluster when there are few rows.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <cstdint>
+#include <math_constants.h>
+
+#include "../../include/eraserdit_b200.h"
+#include "host_common.h"
+#include "sm100_ptx.cuh"
+#include "tmem_io.cuh"
+
+namespace erd {
+namespace btk {
+
+constexpr int kDim = 64;       // head_dim
+constexpr int kTile = 128;     // queries of a tile and keys of a step
+constexpr int kHalf = 64;      // keys that are loaded (and chosen) together at least
+
+// ------------------------------------------------------------ small helpers
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  return pack_bf16x2(lo, hi);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 p = unpack2<T>(w[i]);
+    f[2 * i] = p.x;
+    f[2 * i + 1] = p.y;
+  }
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+
+struct Strides {
+  long long token, head, batch;
+};
+
+// Valid keys of a batch entry.
+__device__ __forceinline__ int key_length(const int* lengths, int b, int kv_len) {
+  return lengths == nullptr ? kv_len : min(max(__ldg(lengths + b), 0), kv_len);
+}
+
+// ---------------------------------------------------------------- block sums
+struct PoolParams {
+  const void* x;
+  Strides st;
+  int heads, len, block, blocks;
+  const int* lengths;  // keys only; null: all
+  int mean;            // divide by the number of summed tokens
+  double* out;         // [batch][heads][blocks][64]
+};
+
+// One warp sums one block of four heads: a lane eight channels, one 16-byte
+// load a token.
+template <typename T>
+__device__ __forceinline__ void pool_block(const PoolParams& p, long long item, int lane) {
+  const int hg = (p.heads + 3) / 4;
+  const int h = static_cast<int>(item % hg) * 4 + lane / 8;
+  const long long bn = item / hg;
+  const int n = static_cast<int>(bn % p.blocks), b = static_cast<int>(bn / p.blocks);
+  if (h >= p.heads) return;
+  const int len = key_length(p.lengths, b, p.len);
+  const int t0 = n * p.block, t1 = min(t0 + p.block, len);
+  const T* src =
+      static_cast<const T*>(p.x) + b * p.st.batch + h * p.st.head + (lane & 7) * 8;
+  double sum[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum[i] = 0.0;
+  constexpr int U = 8;
+  int t = t0;
+  for (; t + U <= t1; t += U) {
+    uint4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const uint4*>(src + (t + u) * p.st.token);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[8];
+      unpack8<T>(v[u], f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] += static_cast<double>(f[i]);
+    }
+  }
+  for (; t < t1; ++t) {
+    float f[8];
+    unpack8<T>(*reinterpret_cast<const uint4*>(src + t * p.st.token), f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] += static_cast<double>(f[i]);
+  }
+  if (p.mean && t1 > t0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] /= static_cast<double>(t1 - t0);
+  }
+  double2* dst = reinterpret_cast<double2*>(
+      p.out + ((static_cast<long long>(b) * p.heads + h) * p.blocks + n) * kDim + (lane & 7) * 8);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) dst[i] = make_double2(sum[2 * i], sum[2 * i + 1]);
+}
+
+constexpr int kPoolWarps = 4;
+template <typename T>
+__global__ void __launch_bounds__(32 * kPoolWarps)
+    pool_kernel(const PoolParams a, const PoolParams b, long long items_a, long long items) {
+  const long long item = static_cast<long long>(blockIdx.x) * kPoolWarps + (threadIdx.x >> 5);
+  if (item >= items) return;
+  if (item < items_a)
+    pool_block<T>(a, item, threadIdx.x & 31);
+  else
+    pool_block<T>(b, item - items_a, threadIdx.x & 31);
+}
+
+// ------------------------------------------------------------------- scores
+// scores[b][h][g][n] = q_sum[b][h][g] . k_mean[b][h / per][n], 64 x 64 a CTA,
+// 4 x 4 a thread.  0.5 G N d FP64 products; a small part of the attention.
+constexpr int kScoreTile = 64;
+constexpr int kScoreSmem = 2 * kDim * kScoreTile * 8;
+__global__ void __launch_bounds__(256)
+    score_kernel(const double* q_sum, const double* k_mean, double* scores, int heads, int per,
+                 int groups, int blocks) {
+  extern __shared__ double tiles[];  // [64 d][64 groups], [64 d][64 blocks]
+  double* sq = tiles;
+  double* sk = tiles + kDim * kScoreTile;
+  const int n0 = blockIdx.x * kScoreTile, g0 = blockIdx.y * kScoreTile;
+  const int bh = blockIdx.z;
+  const int b = bh / heads, h = bh - b * heads;
+  const long long kv = static_cast<long long>(b) * (heads / per) + h / per;
+  // 4 threads a row, 16 doubles each; a warp's stores fall on 8 rows of 4 columns
+  const int r = threadIdx.x / 4, c = threadIdx.x % 4 * 16;
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) {
+    double2 a = make_double2(0.0, 0.0), k = make_double2(0.0, 0.0);
+    if (g0 + r < groups)
+      a = *reinterpret_cast<const double2*>(
+          q_sum + (static_cast<long long>(bh) * groups + g0 + r) * kDim + c + i);
+    if (n0 + r < blocks)
+      k = *reinterpret_cast<const double2*>(k_mean + (kv * blocks + n0 + r) * kDim + c + i);
+    sq[(c + i) * kScoreTile + r] = a.x;
+    sq[(c + i + 1) * kScoreTile + r] = a.y;
+    sk[(c + i) * kScoreTile + r] = k.x;
+    sk[(c + i + 1) * kScoreTile + r] = k.y;
+  }
+  __syncthreads();
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  double acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.0;
+#pragma unroll 4
+  for (int d = 0; d < kDim; ++d) {
+    const double2* qa = reinterpret_cast<const double2*>(sq + d * kScoreTile + ty * 4);
+    const double2* ka = reinterpret_cast<const double2*>(sk + d * kScoreTile + tx * 4);
+    const double2 q01 = qa[0], q23 = qa[1], k01 = ka[0], k23 = ka[1];
+    const double qv[4] = {q01.x, q01.y, q23.x, q23.y}, kv4[4] = {k01.x, k01.y, k23.x, k23.y};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = fma(qv[i], kv4[j], acc[i][j]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int g = g0 + ty * 4 + i;
+    if (g >= groups) continue;
+    double* dst = scores + (static_cast<long long>(bh) * groups + g) * blocks;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = n0 + tx * 4 + j;
+      if (n < blocks) dst[n] = acc[i][j];
+    }
+  }
+}
+
+// ---------------------------------------------------------------- selection
+// Order-preserving key of a score: greater score, greater key; -0 is 0, NaN is
+// below every number.
+__device__ __forceinline__ unsigned long long score_key(double s) {
+  if (s != s) return 0ull;
+  const unsigned long long u =
+      static_cast<unsigned long long>(__double_as_longlong(s + 0.0));
+  return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
+}
+
+// One warp writes the indices of the `take` greatest of n keys (ties: lowest
+// index) in ascending order, then -1 up to topk.  `key(i)` gives key i; with
+// kPer > 0 (n <= 32 kPer) their upper words stay in registers.  Bisection over
+// the bits of the upper words, which ends as soon as a threshold splits off
+// exactly `take` keys (after some twenty steps for scores that differ), and
+// over the lower words of those that tie there only if they do.
+template <int kPer, typename Key>
+__device__ __forceinline__ void select_topk(Key key, int n, int take, int topk, int* out,
+                                            int lane) {
+  uint32_t hi[kPer > 0 ? kPer : 1];
+  const int rounds = (n + 31) / 32;
+  if (kPer > 0) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int i = j * 32 + lane;
+      hi[j] = i < n ? static_cast<uint32_t>(key(i) >> 32) : 0u;
+    }
+  }
+  // number of keys whose upper word is at least t (t > 0: absent ones are 0)
+  auto at_least = [&](uint32_t t) {
+    int c = 0;
+    if (kPer > 0) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) c += hi[j] >= t;
+    } else {
+      for (int j = 0; j < rounds; ++j) {
+        const int i = j * 32 + lane;
+        c += i < n && static_cast<uint32_t>(key(i) >> 32) >= t;
+      }
+    }
+    return __reduce_add_sync(0xffffffffu, c);
+  };
+  // Greatest t with at_least(t) >= take (take <= n, so t = 0 always holds).
+  uint32_t t = 0;
+  bool exact = take >= n;  // everything is taken
+  if (!exact) {
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t up = t | (1u << bit);
+      const int c = at_least(up);
+      if (c >= take) {
+        t = up;
+        if (c == take) {
+          exact = true;
+          break;
+        }
+      }
+    }
+  }
+  // Keys above t are taken, those at t as far as `ties` allows by their lower
+  // words.
+  uint32_t low = 0;
+  int ties = 0;  // keys equal to (t, low) that are taken
+  if (!exact) {
+    const int above = t == 0xffffffffu ? 0 : at_least(t + 1);
+    const int want = take - above;
+    auto low_at_least = [&](uint32_t v) {
+      int c = 0;
+      for (int j = 0; j < rounds; ++j) {
+        const int i = j * 32 + lane;
+        if (i < n) {
+          const unsigned long long k = key(i);
+          c += static_cast<uint32_t>(k >> 32) == t && static_cast<uint32_t>(k) >= v;
+        }
+      }
+      return __reduce_add_sync(0xffffffffu, c);
+    };
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t up = low | (1u << bit);
+      if (low_at_least(up) >= want) low = up;
+    }
+    ties = want - (low == 0xffffffffu ? 0 : low_at_least(low + 1));
+  }
+  int count = 0, tied = 0;
+  const unsigned long long bound = (static_cast<unsigned long long>(t) << 32) | low;
+  for (int j = 0; j < rounds; ++j) {
+    const int i = j * 32 + lane;
+    bool yes = false, tie = false;
+    if (i < n) {
+      const unsigned long long k = key(i);
+      if (take >= n)
+        yes = true;
+      else if (exact)
+        yes = static_cast<uint32_t>(k >> 32) >= t;
+      else {
+        yes = k > bound;
+        tie = k == bound;
+      }
+    }
+    const uint32_t tie_mask = __ballot_sync(0xffffffffu, tie);
+    const uint32_t before = (1u << lane) - 1;
+    if (tie && tied + __popc(tie_mask & before) < ties) yes = true;
+    tied += __popc(tie_mask);
+    const uint32_t mask = __ballot_sync(0xffffffffu, yes);
+    if (yes) out[count + __popc(mask & before)] = i;
+    count += __popc(mask);
+  }
+  for (int i = take + lane; i < topk; i += 32) out[i] = -1;
+}
+
+constexpr int kSelectWarps = 4;
+template <int kPer>
+__global__ void __launch_bounds__(32 * kSelectWarps)
+    select_kernel(const double* scores, int* selection, const int* lengths, long long rows,
+                  long long rows_per_batch, int blocks, int kv_len, int key_block, int topk) {
+  const long long row = static_cast<long long>(blockIdx.x) * kSelectWarps + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int len = key_length(lengths, static_cast<int>(row / rows_per_batch), kv_len);
+  const int n = (len + key_block - 1) / key_block;
+  const double* s = scores + row * blocks;
+  select_topk<kPer>([&](int i) { return score_key(s[i]); }, n, min(topk, n), topk,
+                    selection + row * topk, threadIdx.x & 31);
+}
+
+// Single queries: one CTA scores every block of a row (8 lanes a block, eight
+// channels each), and its first warp selects.
+struct RowSelectParams {
+  const void* q;
+  Strides q_st;
+  const double* k_mean;
+  const int* lengths;
+  int heads, per, q_len, kv_len, key_block, blocks, topk;
+  int* selection;
+};
+
+constexpr int kRowSelectWarps = 8;
+template <typename T>
+__global__ void __launch_bounds__(32 * kRowSelectWarps) row_select_kernel(const RowSelectParams p) {
+  extern __shared__ unsigned long long keys[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long row = blockIdx.x;  // (batch, head, query)
+  const int qi = static_cast<int>(row % p.q_len);
+  const int bh = static_cast<int>(row / p.q_len);
+  const int b = bh / p.heads, h = bh - b * p.heads;
+  const int len = key_length(p.lengths, b, p.kv_len);
+  const int n = (len + p.key_block - 1) / p.key_block;
+  const int take = min(p.topk, n);
+  int* out = p.selection + row * p.topk;
+  if (take < n) {
+    const T* q = static_cast<const T*>(p.q) + b * p.q_st.batch + h * p.q_st.head +
+                 qi * p.q_st.token + (lane & 7) * 8;
+    float f[8];
+    unpack8<T>(*reinterpret_cast<const uint4*>(q), f);
+    double qd[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) qd[i] = static_cast<double>(f[i]);
+    const double* mean =
+        p.k_mean +
+        (static_cast<long long>(b) * (p.heads / p.per) + h / p.per) * p.blocks * kDim +
+        (lane & 7) * 8;
+    constexpr int U = 4;  // blocks of a lane group requested together
+    for (int i0 = warp * 4; i0 < n; i0 += kRowSelectWarps * 4 * U) {
+      double2 v[U][4];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * kRowSelectWarps * 4 + lane / 8;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          v[u][j] = i < n ? *reinterpret_cast<const double2*>(mean + i * static_cast<long long>(kDim) + 2 * j)
+                          : make_double2(0.0, 0.0);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * kRowSelectWarps * 4 + lane / 8;
+        double s = 0.0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s = fma(qd[2 * j], v[u][j].x, s);
+          s = fma(qd[2 * j + 1], v[u][j].y, s);
+        }
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        if ((lane & 7) == 0 && i < n) keys[i] = score_key(s);
+      }
+    }
+  }
+  __syncthreads();
+  if (warp != 0) return;
+  auto key = [&](int i) { return keys[i]; };
+  if (n <= 32 * 16)
+    select_topk<16>(key, n, take, p.topk, out, lane);
+  else
+    select_topk<0>(key, n, take, p.topk, out, lane);
+}
+
+// -------------------------------------------------- attention of 128-row tiles
+// One CTA a query tile (two CTAs a multiprocessor, so one's softmax runs beside
+// the other's products): warps 0-3 softmax, one thread a row; warp 4 TMA
+// producer; warp 5 MMA issuer.  A step is 128 keys: two 64-key pieces, which
+// need not be neighbours (the two halves of a key block of 128, or two chosen
+// blocks of 64).  TMEM: S 128 columns, O 64, P 64.
+constexpr int kTileThreads = 192;
+constexpr int kKStages = 3, kVStages = 2;
+constexpr int kTileBytes = kTile * kDim * 2;  // 16 KB
+constexpr float kRescale = 8.0f;  // log2 units the running maximum may lag behind
+
+struct __align__(8) TileBarriers {
+  uint64_t q_full;
+  uint64_t k_full[kKStages], k_empty[kKStages];
+  uint64_t v_full[kVStages], v_empty[kVStages];
+  uint64_t s_full, p_full, o_done, drain;
+  uint32_t tmem_base;
+  int abort;
+};
+constexpr int kTileSmemK = kTileBytes;
+constexpr int kTileSmemV = kTileSmemK + kKStages * kTileBytes;
+constexpr int kTileSmemBar = kTileSmemV + kVStages * kTileBytes;
+constexpr int kTileSmemLaunch = kTileSmemBar + 512 + 1024;  // + base alignment
+static_assert(2 * (kTileSmemLaunch + 1024) <= 228 * 1024, "two CTAs a multiprocessor");
+static_assert(sizeof(TileBarriers) <= 512, "barrier block");
+
+struct TileParams {
+  int q_len, kv_len, per;  // per: query heads of a key head
+  int key_block, topk;
+  const int* lengths;
+  const int* selection;  // [batch][heads][tiles][topk], ascending, -1 behind
+  float scale_log2;
+  void* out;
+  Strides o_st;
+  int* status;
+};
+
+// First key of 64-key piece `i` of a tile's list (kv_len where there is none,
+// which TMA reads as zeros).
+__device__ __forceinline__ int piece_key(const TileParams& p, const int* list, int i, int pieces) {
+  if (i >= pieces) return p.kv_len;
+  const int shift = p.key_block >> 7;  // pieces of a block: 1 << shift
+  return __ldg(list + (i >> shift)) * p.key_block + (i & shift) * kHalf;
+}
+
+// kind::f16 instruction descriptor with BF16 (format 1) or FP16 (format 0)
+// operands, FP32 accumulation; b_mn_major: B's rows are the reduction (V).
+template <bool kBf16>
+__host__ __device__ constexpr uint32_t idesc(int m, int n, bool b_mn_major) {
+  return (1u << 4) | ((kBf16 ? 1u : 0u) << 7) | ((kBf16 ? 1u : 0u) << 10) |
+         ((b_mn_major ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+template <typename T, bool kBf16>
+__global__ void __launch_bounds__(kTileThreads, 2)
+    tile_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
+                     const __grid_constant__ CUtensorMap tmap_k,
+                     const __grid_constant__ CUtensorMap tmap_v, const TileParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  TileBarriers* bars = reinterpret_cast<TileBarriers*>(smem + kTileSmemBar);
+  const uint32_t sQ = smem_u32(smem), sK = sQ + kTileSmemK, sV = sQ + kTileSmemV;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  const int tile = blockIdx.x, head = blockIdx.y, batch = blockIdx.z;
+  const int len = key_length(p.lengths, batch, p.kv_len);
+  const int kept = min(p.topk, (len + p.key_block - 1) / p.key_block);
+  const int pieces = kept << (p.key_block >> 7);
+  const int steps = (pieces + 1) / 2;
+  const int* list =
+      p.selection +
+      ((static_cast<long long>(batch) * gridDim.y + head) * gridDim.x + tile) * p.topk;
+  const int row = threadIdx.x & 127;
+  const int tok = tile * kTile + row;
+  T* dst = static_cast<T*>(p.out) + batch * p.o_st.batch + head * p.o_st.head +
+           tok * p.o_st.token;
+  if (steps == 0) {  // no valid key: zeros
+    if (threadIdx.x < kTile && tok < p.q_len) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    return;
+  }
+  volatile int* abort = &bars->abort;
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&bars->q_full), 1);
+    for (int s = 0; s < kKStages; ++s) {
+      mbar_init(smem_u32(&bars->k_full[s]), 1);
+      mbar_init(smem_u32(&bars->k_empty[s]), 1);
+    }
+    for (int s = 0; s < kVStages; ++s) {
+      mbar_init(smem_u32(&bars->v_full[s]), 1);
+      mbar_init(smem_u32(&bars->v_empty[s]), 1);
+    }
+    mbar_init(smem_u32(&bars->s_full), 1);
+    mbar_init(smem_u32(&bars->p_full), kTile);
+    mbar_init(smem_u32(&bars->o_done), 1);
+    mbar_init(smem_u32(&bars->drain), 1);
+    bars->abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 4) {
+    tmem_alloc(smem_u32(&bars->tmem_base), 256);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+
+  if (warp == 4) {
+    // ------------------------------------------------------------ producer
+    if (elect_one()) {
+      tma_prefetch_desc(&tmap_q);
+      tma_prefetch_desc(&tmap_k);
+      tma_prefetch_desc(&tmap_v);
+      const int kv_head = head / p.per;
+      const uint32_t q_bar = smem_u32(&bars->q_full);
+      mbar_arrive_expect_tx(q_bar, kTileBytes);
+      tma_load_5d(sQ, &tmap_q, q_bar, 0, tile * kTile, head, batch, 0);
+      int j = 0;
+      for (; j < steps; ++j) {
+        const int a = piece_key(p, list, 2 * j, pieces), b = piece_key(p, list, 2 * j + 1, pieces);
+        const int ks = j % kKStages, vs = j % kVStages;
+        if (!mbar_wait(smem_u32(&bars->k_empty[ks]), ((j / kKStages) & 1) ^ 1, abort, p.status,
+                       kStatusTimeoutProducer))
+          break;
+        const uint32_t kb = smem_u32(&bars->k_full[ks]), kd = sK + ks * kTileBytes;
+        mbar_arrive_expect_tx(kb, kTileBytes);
+        tma_load_5d(kd, &tmap_k, kb, 0, a, kv_head, batch, 0);
+        tma_load_5d(kd + kTileBytes / 2, &tmap_k, kb, 0, b, kv_head, batch, 0);
+        if (!mbar_wait(smem_u32(&bars->v_empty[vs]), ((j / kVStages) & 1) ^ 1, abort, p.status,
+                       kStatusTimeoutProducer))
+          break;
+        const uint32_t vb = smem_u32(&bars->v_full[vs]), vd = sV + vs * kTileBytes;
+        mbar_arrive_expect_tx(vb, kTileBytes);
+        tma_load_5d(vd, &tmap_v, vb, 0, a, kv_head, batch, 0);
+        tma_load_5d(vd + kTileBytes / 2, &tmap_v, vb, 0, b, kv_head, batch, 0);
+      }
+      if (*abort) {
+        // Let every load this thread may have started land before the CTA exits.
+        mbar_wait_drain(q_bar, 0);
+        for (int d = max(0, j - kKStages); d <= j && d < steps; ++d) {
+          mbar_wait_drain(smem_u32(&bars->k_full[d % kKStages]), (d / kKStages) & 1);
+          mbar_wait_drain(smem_u32(&bars->v_full[d % kVStages]), (d / kVStages) & 1);
+        }
+      }
+    }
+  } else if (warp == 5) {
+    // ---------------------------------------------------------- MMA issuer
+    if (elect_one()) {
+      constexpr uint32_t id_qk = idesc<kBf16>(kTile, kTile, false);
+      constexpr uint32_t id_pv = idesc<kBf16>(kTile, kDim, true);
+      const uint32_t tS = tmem, tO = tmem + 128, tP = tmem + 192;
+      const uint64_t dq = sdesc_sw128(sQ, 16, 1024);
+      const uint64_t dk0 = sdesc_sw128(sK, 16, 1024), dv0 = sdesc_sw128(sV, 1024, 1024);
+      uint32_t ks = 0, kph = 0, vs = 0, vph = 0;  // next stages to be read
+      auto issue_qk = [&]() {
+        const uint64_t dk = dk0 + ks * (kTileBytes / 16);
+#pragma unroll
+        for (int k = 0; k < kDim / 16; ++k)
+          mma_bf16_ss(tS, dq + 2 * k, dk + 2 * k, id_qk, k > 0);
+        mma_commit(smem_u32(&bars->s_full));
+        mma_commit(smem_u32(&bars->k_empty[ks]));
+        if (++ks == kKStages) ks = 0, kph ^= 1;
+      };
+      bool ok = mbar_wait(smem_u32(&bars->q_full), 0, abort, p.status, kStatusTimeoutMma) &&
+                mbar_wait(smem_u32(&bars->k_full[0]), 0, abort, p.status, kStatusTimeoutMma);
+      if (ok) {
+        tc_fence_after();
+        issue_qk();
+      }
+      for (int j = 0; ok && j < steps; ++j) {
+        const bool more = j + 1 < steps;
+        if (more &&
+            !mbar_wait(smem_u32(&bars->k_full[ks]), kph, abort, p.status, kStatusTimeoutMma))
+          break;
+        if (!mbar_wait(smem_u32(&bars->v_full[vs]), vph, abort, p.status, kStatusTimeoutMma))
+          break;
+        if (!mbar_wait(smem_u32(&bars->p_full), j & 1, abort, p.status, kStatusTimeoutMma)) break;
+        tc_fence_after();
+        if (more) issue_qk();
+        const uint64_t dv = dv0 + vs * (kTileBytes / 16);
+#pragma unroll
+        for (int k = 0; k < kTile / 16; ++k)
+          mma_bf16_ts(tO, tP + k * 8, dv + k * (2048 / 16), id_pv, (j > 0 || k > 0) ? 1u : 0u);
+        mma_commit(smem_u32(&bars->o_done));
+        mma_commit(smem_u32(&bars->v_empty[vs]));
+        if (++vs == kVStages) vs = 0, vph ^= 1;
+      }
+      // Every product completes before TMEM is released.
+      mma_commit(smem_u32(&bars->drain));
+      mbar_wait_drain(smem_u32(&bars->drain), 0);
+    }
+  } else {
+    // ------------------------------------------------------------- softmax
+    const uint32_t lane_off = static_cast<uint32_t>(warp * 32) << 16;
+    const uint32_t tS = tmem + lane_off, tO = tmem + 128 + lane_off, tP = tmem + 192 + lane_off;
+    const float c = p.scale_log2;
+    float m_run = -CUDART_INF_F, l_run = 0.f;  // running maximum (log2 domain) and sum
+    bool ok = true;
+    for (int j = 0; j < steps; ++j) {
+      // Valid keys of the step's two pieces (read before the wait).
+      const int key_a = piece_key(p, list, 2 * j, pieces);
+      const int key_b = piece_key(p, list, 2 * j + 1, pieces);
+      const int na = min(max(len - key_a, 0), kHalf), nb = min(max(len - key_b, 0), kHalf);
+      const bool whole = na == kHalf && nb == kHalf;
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->s_full), j & 1, abort, p.status,
+                                             kStatusTimeoutSoftmax))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      float mx0 = -CUDART_INF_F, mx1 = -CUDART_INF_F, mx2 = -CUDART_INF_F, mx3 = -CUDART_INF_F;
+      {
+        uint32_t sr[128];
+        tmem_ld_wait_128(tS, sr);
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < kTile; ++i)
+            if (i < kHalf ? i >= na : i - kHalf >= nb) sr[i] = __float_as_uint(-CUDART_INF_F);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          mx0 = fmax3(mx0, __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
+          mx1 = fmax3(mx1, __uint_as_float(sr[32 + i]), __uint_as_float(sr[33 + i]));
+          mx2 = fmax3(mx2, __uint_as_float(sr[64 + i]), __uint_as_float(sr[65 + i]));
+          mx3 = fmax3(mx3, __uint_as_float(sr[96 + i]), __uint_as_float(sr[97 + i]));
+        }
+      }
+      const float m_tile = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * c;
+      float m_new = m_run;
+      bool rescale = false;
+      if (m_tile > m_run + kRescale) {
+        m_new = m_tile;
+        rescale = j > 0;
+      }
+      if (j > 0) {  // P and O are free once the previous product has completed
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->o_done), (j - 1) & 1, abort,
+                                               p.status, kStatusTimeoutSoftmax))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+      }
+      if (__any_sync(0xffffffffu, rescale)) {
+        const float alpha = rescale ? ex2_approx(m_run - m_new) : 1.0f;
+        l_run *= alpha;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t o[32];
+          tmem_ld_wait_32(tO + h * 32, o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          tmem_st32(tO + h * 32, o);
+        }
+      }
+      m_run = m_new;
+      // A row that has met only -inf so far weighs those keys 0.
+      const float neg_m = m_new == -CUDART_INF_F ? 0.f : -m_new;
+      float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t pk[32], sr[64];
+        tmem_ld_wait_64(tS + h * 64, sr);
+        if (!whole) {
+          const int n = h ? nb : na;
+#pragma unroll
+          for (int i = 0; i < kHalf; ++i)
+            if (i >= n) sr[i] = __float_as_uint(-CUDART_INF_F);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          float x0, x1;
+          fma2(x0, x1, __uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1]), c, c, neg_m,
+               neg_m);
+          const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+          add2(sum0, sum1, sum0, sum1, p0, p1);
+          pk[i] = pack2<T>(p0, p1);
+        }
+        tmem_st32(tP + h * 32, pk);
+      }
+      l_run += sum0 + sum1;
+      // Rows of V behind the sequence's end may hold anything (0 * NaN is NaN):
+      // they are cleared before the product reads them.
+      if (!whole && len < p.kv_len) {
+        const int vs = j % kVStages;
+        if (!__all_sync(0xffffffffu,
+                        mbar_wait(smem_u32(&bars->v_full[vs]), (j / kVStages) & 1, abort, p.status,
+                                  kStatusTimeoutSoftmax))) {
+          ok = false;
+          break;
+        }
+        if ((row & (kHalf - 1)) >= (row < kHalf ? na : nb)) {
+          uint4* v = reinterpret_cast<uint4*>(smem + kTileSmemV + vs * kTileBytes + row * 128);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(smem_u32(&bars->p_full));
+    }
+    if (ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->o_done), (steps - 1) & 1, abort,
+                                                p.status, kStatusTimeoutEpilogue))) {
+      tc_fence_after();
+      uint32_t o[64];
+      tmem_ld_wait_64(tO, o);
+      if (tok < p.q_len) {
+        const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            w[k] = pack2<T>(__uint_as_float(o[8 * i + 2 * k]) * inv,
+                            __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
+          reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 256);
+  }
+}
+
+// ------------------------------------------------- attention of single queries
+// Eight lanes share a key (16 bytes each of its K and V rows); a lane group
+// takes eight neighbouring keys at a time, with its own running maximum and
+// sum, and the groups, warps and CTAs of a row are merged at the end, in a
+// fixed order.  Bound by the chosen blocks' bytes: 16 loads of 16 bytes a lane
+// are in flight.
+constexpr int kRowWarps = 8;
+constexpr int kRowKeys = 8;
+constexpr int kMaxSplits = 8;
+
+struct RowParams {
+  const void *q, *k, *v;
+  Strides q_st, k_st, v_st, o_st;
+  void* out;
+  const int* lengths;
+  const int* selection;
+  int heads, per, q_len, kv_len, key_block, topk, splits;
+  float scale_log2;
+};
+
+__device__ __forceinline__ float ld_cluster_f32(const float* p, uint32_t rank) {
+  uint32_t at;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+
+// Weight that a part with maximum m has under the common maximum `top`.
+__device__ __forceinline__ float part_weight(float m, float top) {
+  return m == -CUDART_INF_F ? 0.f : ex2_approx(m - top);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kRowWarps, 2) row_attn_kernel(const RowParams p) {
+  __shared__ float part_m[kRowWarps], part_l[kRowWarps], part_o[kRowWarps][kDim];
+  __shared__ float cta[kDim + 2];  // this CTA's O, maximum, sum
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = static_cast<int>(blockIdx.x % p.splits);  // also the rank in the cluster
+  const long long row = blockIdx.x / p.splits;                // (batch, head, query)
+  const int qi = static_cast<int>(row % p.q_len);
+  const int bh = static_cast<int>(row / p.q_len);
+  const int b = bh / p.heads, h = bh - b * p.heads;
+  const int len = key_length(p.lengths, b, p.kv_len);
+  const int kept = min(p.topk, (len + p.key_block - 1) / p.key_block);
+  const int shift = p.key_block >> 7;
+  const int pieces = kept << shift;
+  const int lo = static_cast<int>(static_cast<long long>(pieces) * split / p.splits);
+  const int hi = static_cast<int>(static_cast<long long>(pieces) * (split + 1) / p.splits);
+  const int* list = p.selection + row * p.topk;
+  const int group = lane >> 3, c8 = (lane & 7) * 8;
+  float q[8];
+  {
+    const T* src = static_cast<const T*>(p.q) + b * p.q_st.batch + h * p.q_st.head +
+                   qi * p.q_st.token + c8;
+    unpack8<T>(*reinterpret_cast<const uint4*>(src), q);
+  }
+  const T* kp = static_cast<const T*>(p.k) + b * p.k_st.batch + h / p.per * p.k_st.head + c8;
+  const T* vp = static_cast<const T*>(p.v) + b * p.v_st.batch + h / p.per * p.v_st.head + c8;
+  float m = -CUDART_INF_F, l = 0.f, o[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = 0.f;
+  // units of 32 keys: half a 64-key piece, eight keys a lane group
+  for (int u = 2 * lo + warp; u < 2 * hi; u += kRowWarps) {
+    const int first = __ldg(list + ((u >> 1) >> shift)) * p.key_block +
+                      ((u >> 1) & shift) * kHalf + (u & 1) * 32 + group * kRowKeys;
+    uint4 kv[kRowKeys], vv[kRowKeys];
+#pragma unroll
+    for (int i = 0; i < kRowKeys; ++i) {
+      kv[i] = vv[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (first + i < len) kv[i] = *reinterpret_cast<const uint4*>(kp + (first + i) * p.k_st.token);
+    }
+#pragma unroll
+    for (int i = 0; i < kRowKeys; ++i)
+      if (first + i < len) vv[i] = *reinterpret_cast<const uint4*>(vp + (first + i) * p.v_st.token);
+    float s[kRowKeys], top = m;
+#pragma unroll
+    for (int i = 0; i < kRowKeys; ++i) {
+      float f[8], d = 0.f;
+      unpack8<T>(kv[i], f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d = fmaf(q[j], f[j], d);
+#pragma unroll
+      for (int x = 1; x < 8; x <<= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
+      s[i] = first + i < len ? d * p.scale_log2 : -CUDART_INF_F;
+      top = fmaxf(top, s[i]);
+    }
+    const float zero = top == -CUDART_INF_F ? 0.f : top;
+    const float alpha = ex2_approx(m - zero);
+    l *= alpha;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] *= alpha;
+#pragma unroll
+    for (int i = 0; i < kRowKeys; ++i) {
+      const float w = ex2_approx(s[i] - zero);
+      l += w;
+      float f[8];
+      unpack8<T>(vv[i], f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = fmaf(w, f[j], o[j]);
+    }
+    m = top;
+  }
+  // the four lane groups of the warp
+#pragma unroll
+  for (int x = 8; x < 32; x <<= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, x), top = fmaxf(m, m2);
+    const float mine = part_weight(m, top), theirs = part_weight(m2, top);
+    l = l * mine + __shfl_xor_sync(0xffffffffu, l, x) * theirs;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      o[j] = o[j] * mine + __shfl_xor_sync(0xffffffffu, o[j], x) * theirs;
+    m = top;
+  }
+  if (lane < 8) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) part_o[warp][c8 + j] = o[j];
+    if (lane == 0) {
+      part_m[warp] = m;
+      part_l[warp] = l;
+    }
+  }
+  __syncthreads();
+  const int d = threadIdx.x;
+  float om = 0.f, lm = 0.f, top = -CUDART_INF_F;
+  if (d < kDim) {
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, part_m[w]);
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) {
+      const float weight = part_weight(part_m[w], top);
+      om += part_o[w][d] * weight;
+      lm += part_l[w] * weight;
+    }
+  }
+  if (p.splits > 1) {
+    if (d < kDim) cta[d] = om;
+    if (d == 0) {
+      cta[kDim] = top;
+      cta[kDim + 1] = lm;
+    }
+    cluster_sync();
+    if (split == 0 && d < kDim) {
+      float ms[kMaxSplits], ls[kMaxSplits], os[kMaxSplits];
+#pragma unroll
+      for (int s = 0; s < kMaxSplits; ++s) {
+        if (s < p.splits) {
+          ms[s] = ld_cluster_f32(&cta[kDim], s);
+          ls[s] = ld_cluster_f32(&cta[kDim + 1], s);
+          os[s] = ld_cluster_f32(&cta[d], s);
+        }
+      }
+      top = -CUDART_INF_F;
+      om = lm = 0.f;
+#pragma unroll
+      for (int s = 0; s < kMaxSplits; ++s)
+        if (s < p.splits) top = fmaxf(top, ms[s]);
+#pragma unroll
+      for (int s = 0; s < kMaxSplits; ++s) {
+        if (s < p.splits) {
+          const float weight = part_weight(ms[s], top);
+          om += os[s] * weight;
+          lm += ls[s] * weight;
+        }
+      }
+    }
+    cluster_sync();  // the others' sums have been read
+  }
+  if (split == 0 && d < kDim) {
+    const float y = lm == 0.f ? 0.f : om / lm;
+    uint16_t* dst = static_cast<uint16_t*>(p.out) + b * p.o_st.batch + h * p.o_st.head +
+                    qi * p.o_st.token + d;
+    *dst = static_cast<uint16_t>(pack2<T>(y, 0.f));
+  }
+}
+
+// ---------------------------------------------------------------- host side
+struct Sizes {
+  long long blocks, groups;
+  size_t pool, q_sum, scores, total;
+};
+
+Sizes workspace_sizes(long long batch, long long q_heads, long long kv_heads, long long q_len,
+                      long long kv_len, int query_block, int key_block, bool has_pool) {
+  Sizes s = {};
+  s.blocks = (kv_len + key_block - 1) / key_block;
+  s.groups = (q_len + query_block - 1) / query_block;
+  s.pool = has_pool ? 0 : static_cast<size_t>(batch * kv_heads * s.blocks * kDim) * 8;
+  if (query_block == kTile) {
+    s.q_sum = static_cast<size_t>(batch * q_heads * s.groups * kDim) * 8;
+    s.scores = static_cast<size_t>(batch * q_heads * s.groups * s.blocks) * 8;
+  }
+  s.total = s.pool + s.q_sum + s.scores;
+  return s;
+}
+
+bool strides_ok(const Strides& s) { return ((s.token | s.head | s.batch) & 7) == 0; }
+
+int operand_map(CUtensorMap* map, bool bf16, const void* base, int len, int heads, int batch,
+                const Strides& st, int rows) {
+  const uint64_t dims[5] = {static_cast<uint64_t>(kDim), static_cast<uint64_t>(len),
+                            static_cast<uint64_t>(heads), static_cast<uint64_t>(batch), 1};
+  // a dimension of one still needs a valid stride
+  auto stride = [](long long s, uint64_t n) -> uint64_t {
+    return n > 1 ? static_cast<uint64_t>(s) * 2 : 16;
+  };
+  const uint64_t strides[4] = {stride(st.token, dims[1]), stride(st.head, dims[2]),
+                               stride(st.batch, dims[3]), 16};
+  const uint32_t box[5] = {kDim, static_cast<uint32_t>(rows), 1, 1, 1};
+  return encode_tensor_map(
+      map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
+      const_cast<void*>(base), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+long long pool_items(const PoolParams& p, int batch) {
+  return static_cast<long long>(batch) * p.blocks * ((p.heads + 3) / 4);
+}
+
+template <typename T>
+int launch_pool(const PoolParams* a, const PoolParams* b, int batch, cudaStream_t st) {
+  const long long items_a = a == nullptr ? 0 : pool_items(*a, batch);
+  const long long items = items_a + (b == nullptr ? 0 : pool_items(*b, batch));
+  const long long ctas = (items + kPoolWarps - 1) / kPoolWarps;
+  if (ctas > 0x7fffffffLL) return kErrTooLarge;
+  const PoolParams none = {};
+  pool_kernel<T><<<static_cast<unsigned>(ctas), 32 * kPoolWarps, 0, st>>>(
+      a == nullptr ? none : *a, b == nullptr ? none : *b, items_a, items);
+  return static_cast<int>(cudaGetLastError());
+}
+
+struct Call {
+  const void *q, *k, *v;
+  Strides q_st, k_st, v_st, o_st;
+  int batch, q_heads, kv_heads, q_len, kv_len;
+  const int* lengths;
+  const double* pool;
+  int topk, query_block, key_block;
+  float scale;
+  void* out;
+  int* selection;
+  char* workspace;
+  int* status;
+};
+
+template <typename T, bool kBf16>
+int run(const Call& c, cudaStream_t st) {
+  const Sizes sz = workspace_sizes(c.batch, c.q_heads, c.kv_heads, c.q_len, c.kv_len,
+                                   c.query_block, c.key_block, c.pool != nullptr);
+  const bool tiles = c.query_block == kTile;
+  const int blocks = static_cast<int>(sz.blocks), groups = static_cast<int>(sz.groups);
+  double* own_pool = reinterpret_cast<double*>(c.workspace);
+  double* q_sum = reinterpret_cast<double*>(c.workspace + sz.pool);
+  double* scores = reinterpret_cast<double*>(c.workspace + sz.pool + sz.q_sum);
+  const double* pool = c.pool != nullptr ? c.pool : own_pool;
+  const int per = c.q_heads / c.kv_heads;
+  const float scale_log2 = c.scale * 1.4426950408889634f;
+
+  const PoolParams kp = {c.k, c.k_st, c.kv_heads, c.kv_len, c.key_block, blocks, c.lengths, 1,
+                         own_pool};
+  const PoolParams qp = {c.q, c.q_st, c.q_heads, c.q_len, kTile, groups, nullptr, 0, q_sum};
+  if (c.pool == nullptr || tiles) {
+    if (int rc = launch_pool<T>(c.pool == nullptr ? &kp : nullptr, tiles ? &qp : nullptr, c.batch,
+                                st))
+      return rc;
+  }
+  if (tiles) {
+    cudaError_t e = cudaFuncSetAttribute(
+        score_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kScoreSmem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    const dim3 grid((blocks + kScoreTile - 1) / kScoreTile, (groups + kScoreTile - 1) / kScoreTile,
+                    static_cast<unsigned>(c.batch * c.q_heads));
+    score_kernel<<<grid, 256, kScoreSmem, st>>>(q_sum, pool, scores, c.q_heads, per, groups,
+                                                blocks);
+    if ((e = cudaGetLastError()) != cudaSuccess) return static_cast<int>(e);
+    const long long per_batch = static_cast<long long>(c.q_heads) * groups;
+    const long long rows = c.batch * per_batch;
+    const unsigned ctas = static_cast<unsigned>((rows + kSelectWarps - 1) / kSelectWarps);
+    auto select = blocks <= 32 * 8 ? select_kernel<8>
+                  : blocks <= 32 * 16 ? select_kernel<16>
+                  : blocks <= 32 * 32 ? select_kernel<32> : select_kernel<0>;
+    select<<<ctas, 32 * kSelectWarps, 0, st>>>(scores, c.selection, c.lengths, rows, per_batch,
+                                               blocks, c.kv_len, c.key_block, c.topk);
+    if ((e = cudaGetLastError()) != cudaSuccess) return static_cast<int>(e);
+    CUtensorMap tq, tk, tv;
+    if (operand_map(&tq, kBf16, c.q, c.q_len, c.q_heads, c.batch, c.q_st, kTile) ||
+        operand_map(&tk, kBf16, c.k, c.kv_len, c.kv_heads, c.batch, c.k_st, kHalf) ||
+        operand_map(&tv, kBf16, c.v, c.kv_len, c.kv_heads, c.batch, c.v_st, kHalf))
+      return kErrTensorMap;
+    e = cudaFuncSetAttribute(tile_attn_kernel<T, kBf16>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmemLaunch);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    const TileParams p = {c.q_len, c.kv_len, per, c.key_block, c.topk, c.lengths, c.selection,
+                          scale_log2, c.out, c.o_st, c.status};
+    tile_attn_kernel<T, kBf16>
+        <<<dim3(groups, c.q_heads, c.batch), kTileThreads, kTileSmemLaunch, st>>>(tq, tk, tv, p);
+    return static_cast<int>(cudaGetLastError());
+  }
+
+  const long long rows = static_cast<long long>(c.batch) * c.q_heads * c.q_len;
+  const int key_bytes = blocks * 8;
+  cudaError_t e;
+  if (key_bytes > 48 * 1024) {
+    e = cudaFuncSetAttribute(row_select_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             key_bytes);
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  const RowSelectParams sp = {c.q, c.q_st, pool, c.lengths, c.q_heads, per, c.q_len, c.kv_len,
+                              c.key_block, blocks, c.topk, c.selection};
+  row_select_kernel<T>
+      <<<static_cast<unsigned>(rows), 32 * kRowSelectWarps, key_bytes, st>>>(sp);
+  if ((e = cudaGetLastError()) != cudaSuccess) return static_cast<int>(e);
+  RowParams p = {c.q, c.k, c.v, c.q_st, c.k_st, c.v_st, c.o_st, c.out, c.lengths, c.selection,
+                 c.q_heads, per, c.q_len, c.kv_len, c.key_block, c.topk, 1, scale_log2};
+  // Parts of a row: as many CTAs as two a multiprocessor hold, each with four
+  // 64-key pieces at least.
+  const long long most = static_cast<long long>(c.topk < blocks ? c.topk : blocks)
+                         << (c.key_block >> 7);
+  while (p.splits < kMaxSplits && rows * p.splits * 2 <= 2 * 148 * 2 && most / (p.splits * 2) >= 4)
+    p.splits *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * p.splits));
+  cfg.blockDim = dim3(32 * kRowWarps);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(p.splits);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, row_attn_kernel<T>, p));
+}
+
+}  // namespace btk
+}  // namespace erd
+
+using namespace erd;
+
+extern "C" size_t erd_block_topk_workspace_bytes(int batch, int q_heads, int kv_heads, int q_len,
+                                                 int kv_len, int query_block, int key_block,
+                                                 int has_pool) {
+  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || q_len <= 0 || kv_len <= 0 ||
+      (query_block != 1 && query_block != btk::kTile) || (key_block != 64 && key_block != 128))
+    return 0;
+  return btk::workspace_sizes(batch, q_heads, kv_heads, q_len, kv_len, query_block, key_block,
+                              has_pool != 0)
+      .total;
+}
+
+extern "C" int erd_block_key_means(int dtype, const void* k, int64_t k_token_stride,
+                                   int64_t k_head_stride, int64_t k_batch_stride, int batch,
+                                   int kv_heads, int kv_len, int key_block,
+                                   const int32_t* key_lengths, double* means, void* stream) {
+  if (k == nullptr || means == nullptr) return kErrNullPointer;
+  if ((dtype != ERD_BF16 && dtype != ERD_FP16) || batch <= 0 || kv_heads <= 0 || kv_len <= 0 ||
+      (key_block != 64 && key_block != 128))
+    return kErrBadShape;
+  const btk::Strides st = {k_token_stride, k_head_stride, k_batch_stride};
+  if (!aligned16(k) || !aligned16(means) || !btk::strides_ok(st) ||
+      (reinterpret_cast<uintptr_t>(key_lengths) & 3) != 0)
+    return kErrMisaligned;
+  if (int rc = check_device_sm100()) return rc;
+  const btk::PoolParams p = {k, st, kv_heads, kv_len, key_block,
+                             static_cast<int>((kv_len + static_cast<long long>(key_block) - 1) / key_block),
+                             key_lengths, 1, means};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == ERD_BF16 ? btk::launch_pool<__nv_bfloat16>(&p, nullptr, batch, s)
+                           : btk::launch_pool<__half>(&p, nullptr, batch, s);
+}
+
+extern "C" int erd_block_topk_attn(
+    int dtype, const void* q, const void* k, const void* v, int64_t q_token_stride,
+    int64_t q_head_stride, int64_t q_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
+    int64_t k_batch_stride, int64_t v_token_stride, int64_t v_head_stride, int64_t v_batch_stride,
+    int batch, int q_heads, int kv_heads, int q_len, int kv_len, int head_dim,
+    const int32_t* key_lengths, const double* key_means, int topk, int query_block, int key_block,
+    float softmax_scale, void* out, int64_t o_token_stride, int64_t o_head_stride,
+    int64_t o_batch_stride, int32_t* selection, void* workspace, size_t workspace_bytes,
+    int* status, void* stream) {
+  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || selection == nullptr)
+    return kErrNullPointer;
+  if ((dtype != ERD_BF16 && dtype != ERD_FP16) || head_dim != btk::kDim || batch <= 0 ||
+      q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || q_len <= 0 || kv_len <= 0 ||
+      topk <= 0 || (query_block != 1 && query_block != btk::kTile) ||
+      (key_block != 64 && key_block != 128) ||
+      !(softmax_scale > 0.f && softmax_scale <= 3.0e38f))
+    return kErrBadShape;
+  if (batch > 65535 || q_heads > 65535 || static_cast<long long>(batch) * q_heads > 65535 ||
+      kv_len > 0x7fff0000 || q_len > 0x7fff0000)
+    return kErrTooLarge;
+  const btk::Sizes sz =
+      btk::workspace_sizes(batch, q_heads, kv_heads, q_len, kv_len, query_block, key_block,
+                           key_means != nullptr);
+  const long long rows = static_cast<long long>(batch) * q_heads * sz.groups;
+  if (rows > (1LL << 27) || (query_block == 1 && sz.blocks * 8 > 227 * 1024) ||
+      (sz.groups + 63) / 64 > 65535)
+    return kErrTooLarge;
+  if (sz.total > 0 && workspace == nullptr) return kErrNullPointer;
+  if (workspace_bytes < sz.total) return kErrBadShape;
+  btk::Call c = {};
+  c.q = q;
+  c.k = k;
+  c.v = v;
+  c.q_st = {q_token_stride, q_head_stride, q_batch_stride};
+  c.k_st = {k_token_stride, k_head_stride, k_batch_stride};
+  c.v_st = {v_token_stride, v_head_stride, v_batch_stride};
+  c.o_st = {o_token_stride, o_head_stride, o_batch_stride};
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) ||
+      !aligned16(workspace) || !aligned16(key_means) || !btk::strides_ok(c.q_st) ||
+      !btk::strides_ok(c.k_st) || !btk::strides_ok(c.v_st) || !btk::strides_ok(c.o_st) ||
+      ((reinterpret_cast<uintptr_t>(key_lengths) | reinterpret_cast<uintptr_t>(selection)) & 3) != 0)
+    return kErrMisaligned;
+  if (int rc = check_device_sm100()) return rc;
+  c.batch = batch;
+  c.q_heads = q_heads;
+  c.kv_heads = kv_heads;
+  c.q_len = q_len;
+  c.kv_len = kv_len;
+  c.lengths = key_lengths;
+  c.pool = key_means;
+  c.topk = topk;
+  c.query_block = query_block;
+  c.key_block = key_block;
+  c.scale = softmax_scale;
+  c.out = out;
+  c.selection = selection;
+  c.workspace = static_cast<char*>(workspace);
+  c.status = status;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == ERD_BF16 ? btk::run<__nv_bfloat16, true>(c, st) : btk::run<__half, false>(c, st);
+}

@@ -19,7 +19,7 @@ REPO = PACKAGE.parent
 LIBRARY = PACKAGE / "liberaserdit_b200.so"
 SOURCES = ["host_common.cu", "prologue.cu", "attention_bf16.cu", "attention_fp8.cu",
            "attention_fp8_static.cu", "tokens.cu", "peer.cu", "quant.cu", "linear.cu",
-           "head_rotary.cu", "linear_act.cu"]
+           "head_rotary.cu", "linear_act.cu", "block_topk.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -469,6 +469,51 @@ int erd_linear_act(int dtype, const void* x, int64_t ldx, const void* weight, in
                    const void* residual, int64_t ld_residual, void* y, int64_t ldy, int m, int n,
                    int k, int* status, void* stream);
 
+/*
+ * Attention over key blocks that a cheap score selects, head_dim 64.
+ * A query block is `query_block` (128 or 1) consecutive queries, a key block
+ * `key_block` (64 or 128) consecutive keys.  For query block I and key block J
+ * of one head, score = (sum of I's queries) . (mean of J's keys below the
+ * sequence's length), in FP64; each query block of each head keeps its `topk`
+ * highest-scoring blocks with a valid key (all, if there are fewer; ties: the
+ * lowest index; NaN ranks last), and its queries attend the valid keys of those:
+ * out = softmax(q . k * softmax_scale) v, 0 where there is none
+ * (softmax_scale positive and finite: masked keys are -inf times it).
+ * q / out [batch, q_len, q_heads, 64], k / v [batch, kv_len, kv_heads, 64] of
+ * `dtype` (ERD_BF16 or ERD_FP16), element strides, 16-byte aligned; query head h
+ * reads key head h / (q_heads / kv_heads).  key_lengths: device int32 [batch]
+ * (clamped to [0, kv_len]; keys behind are not read into any result, whatever
+ * they hold) or NULL.  key_means: the block means of k as erd_block_key_means
+ * writes them, or NULL to compute them in this call.  selection: int32 [batch]
+ * [q_heads][ceil(q_len / query_block)][topk], receives the chosen blocks in
+ * ascending order, then -1.  `workspace` (16-byte aligned) holds at least
+ * erd_block_topk_workspace_bytes(...) bytes.  batch * q_heads is at most 65535;
+ * query_block 1 takes at most 29056 key blocks.
+ */
+size_t erd_block_topk_workspace_bytes(int batch, int q_heads, int kv_heads, int q_len, int kv_len,
+                                      int query_block, int key_block, int has_pool);
+
+int erd_block_topk_attn(int dtype, const void* q, const void* k, const void* v,
+                        int64_t q_token_stride, int64_t q_head_stride, int64_t q_batch_stride,
+                        int64_t k_token_stride, int64_t k_head_stride, int64_t k_batch_stride,
+                        int64_t v_token_stride, int64_t v_head_stride, int64_t v_batch_stride,
+                        int batch, int q_heads, int kv_heads, int q_len, int kv_len, int head_dim,
+                        const int32_t* key_lengths, const double* key_means, int topk,
+                        int query_block, int key_block, float softmax_scale, void* out,
+                        int64_t o_token_stride, int64_t o_head_stride, int64_t o_batch_stride,
+                        int32_t* selection, void* workspace, size_t workspace_bytes, int* status,
+                        void* stream);
+
+/*
+ * Means of every block of key_block keys over its valid keys, in FP64:
+ * means [batch][kv_heads][ceil(kv_len / key_block)][64] (0 for a block without a
+ * valid key).  A caller that keeps keys keeps these next to them and recomputes
+ * only the blocks it appends to (a view of k from a block's first key on).
+ */
+int erd_block_key_means(int dtype, const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                        int64_t k_batch_stride, int batch, int kv_heads, int kv_len, int key_block,
+                        const int32_t* key_lengths, double* means, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
