@@ -27,15 +27,16 @@ KEY_BLOCKS = (64, 128)
 
 def _strides(what: str, t: torch.Tensor) -> tuple[int, int, int]:
     """(token, head, batch) strides of a BSHD tensor, 0 for a dimension of one."""
-    shape, strides = t.shape, t.stride()
-    if strides[3] != 1:
+    batch, token, head, channel = t.stride()
+    nb, nt, nh, _ = t.shape
+    if channel != 1:
         raise ValueError(f"{what} must have a contiguous head_dim")
-    out = tuple(strides[i] if shape[i] > 1 else 0 for i in (1, 2, 0))
-    if t.data_ptr() % 16 or any(s % 8 for s in out):
+    batch, token, head = batch if nb > 1 else 0, token if nt > 1 else 0, head if nh > 1 else 0
+    if t.data_ptr() % 16 or (batch | token | head) % 8:
         raise ValueError(f"{what} needs 16-byte aligned rows (strides multiple of 8 elements)")
-    if any(s == 0 and shape[i] > 1 for s, i in zip(out, (1, 2, 0))):
+    if (nb > 1 and not batch) or (nt > 1 and not token) or (nh > 1 and not head):
         raise ValueError(f"{what} must not be an expanded view (shared key heads are given once)")
-    return out
+    return token, head, batch
 
 
 def _check_tensor(what: str, t: torch.Tensor) -> None:
@@ -117,12 +118,14 @@ def block_topk_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Te
     if not 0.0 < softmax_scale < float("inf"):
         raise ValueError("softmax_scale must be positive and finite")
     _check_lengths(key_lengths, key)
-    _native.refuse_gradients("block_topk_attention", query, key, value)
+    if torch.is_grad_enabled():
+        _native.refuse_gradients("block_topk_attention", query, key, value)
     if key_pool is not None:
         _check_means(key_pool, key, key_block)
+    device, dtype = query.device, query.dtype
     groups = -(-q_len // query_block)
     if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+        out = query.new_empty(query.shape)
     elif out.shape != query.shape or out.dtype != query.dtype or out.device != query.device:
         raise ValueError("out must have the query's shape, type and device")
     selection = torch.empty(batch, heads, groups, topk, dtype=torch.int32, device=query.device)
@@ -136,13 +139,13 @@ def block_topk_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Te
             # from torch's allocator, call by call: it follows streams and captures
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
         _native.call(
-            "erd_block_topk_attn", query.device, _native.DTYPE_CODES[query.dtype],
+            "erd_block_topk_attn", device, _native.DTYPE_CODES[dtype],
             query.data_ptr(), key.data_ptr(), value.data_ptr(), *_strides("query", query),
             *_strides("key", key), *_strides("value", value), batch, heads, kv_heads, q_len,
             kv_len, HEAD_DIM, _native.ptr(key_lengths), _native.ptr(key_pool), topk, query_block,
             key_block, float(softmax_scale), out.data_ptr(), *_strides("out", out),
             selection.data_ptr(), _native.ptr(workspace), nbytes,
-            _native.status_pointer(query.device))
+            _native.status_pointer(device))
     elif batch and q_len:  # no keys at all
         out.zero_()
         selection.fill_(-1)

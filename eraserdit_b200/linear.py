@@ -121,14 +121,31 @@ def linear_bf16_scatter(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tenso
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
 
-def _row_view(what: str, t: torch.Tensor) -> tuple[int, int] | None:
-    """``_rows`` with a row stride that fits even where no row follows."""
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+_LINEAR_TYPES = (torch.bfloat16, torch.float16)
+
+
+def _row_stride(what: str, t: torch.Tensor) -> int | None:
+    """Stride of ``t``'s rows, one that fits where no row follows, or None when its
+    leading dimensions do not form one strided row axis."""
+    last = t.shape[-1]
+    if t.is_contiguous():
+        return last if t.dim() > 1 and t.numel() > last else -(-last // 8) * 8
+    if last > 1 and t.stride(-1) != 1:
         raise ValueError(f"{what} needs a contiguous last dimension")
-    view = _rows(t)
-    if view is not None and view[0] <= 1:
-        return view[0], -(-t.shape[-1] // 8) * 8
-    return view
+    if t.numel() == last:
+        return -(-last // 8) * 8
+    if t.dim() == 2:
+        return t.stride(0)
+    # the stride of the last dimension that has several entries, met by all others
+    stride = expect = None
+    for size, step in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size > 1:
+            if stride is None:
+                stride = expect = step
+            if step != expect:
+                return None
+            expect *= size
+    return stride
 
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -145,29 +162,32 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     in FP32 and rounded once.  Any sizes; rows of ``x`` and ``weight`` start on 16
     bytes (row strides, and so a contiguous k, are multiples of 8).
     """
-    if x.dtype not in (torch.bfloat16, torch.float16) or not x.is_cuda or x.dim() < 1:
+    dtype, device = x.dtype, x.device
+    if dtype not in _LINEAR_TYPES or device.type != "cuda" or x.dim() < 1:
         raise ValueError("linear_act needs a CUDA BF16 or FP16 x")
-    if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or x.shape[-1] == 0:
+    shape = x.shape
+    if weight.dim() != 2 or weight.shape[1] != shape[-1] or shape[-1] == 0:
         raise ValueError("weight must be [n, k] with k = x.shape[-1] > 0")
     code = ACTIVATIONS.get(activation)
     if code is None:
         raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}")
     n, k = weight.shape
-    shape = (*x.shape[:-1], n)
+    shape = shape[:-1] + (n,)
     for what, t in (("weight", weight), ("bias", bias), ("gate", gate), ("residual", residual),
                     ("out", out)):
-        if t is not None and (t.dtype != x.dtype or t.device != x.device):
+        if t is not None and (t.dtype != dtype or t.device != device):
             raise ValueError(f"{what} must have x's type and device")
-    _native.refuse_gradients("linear_act", x, weight, bias, gate, residual)
+    if torch.is_grad_enabled():
+        _native.refuse_gradients("linear_act", x, weight, bias, gate, residual)
     if bias is not None and (bias.shape != (n,) or not bias.is_contiguous()):
         raise ValueError("bias must be a contiguous [n] tensor")
     if residual is not None and residual.shape != shape:
         raise ValueError("residual must be [..., n]")
     if out is None:
-        out = torch.empty(shape, device=x.device, dtype=x.dtype)
+        out = x.new_empty(shape)
     elif out.shape != shape or any(s == 0 and d > 1 for s, d in zip(out.stride(), out.shape)):
         raise ValueError("out must be [..., n] and no expanded view")
-    m = out.numel() // n if n else 0
+    m = x.numel() // k
     gate_rows = 0
     if gate is not None:
         if gate.dim() not in (1, 2) or gate.shape[-1] != n or not gate.is_contiguous():
@@ -176,12 +196,11 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
         if m and (groups == 0 or m % groups):
             raise ValueError("the gate's groups must divide the rows")
         gate_rows = m // max(groups, 1)
-    if m == 0:
+    if m == 0 or n == 0:
         return out
-    views = [_row_view("x", x), _row_view("out", out),
-             (0, 0) if residual is None else _row_view("residual", residual)]
-    _, ldw = _row_view("weight", weight)
-    if None in views:
+    ldx, ldy, ldw = _row_stride("x", x), _row_stride("out", out), _row_stride("weight", weight)
+    ldr = 0 if residual is None else _row_stride("residual", residual)
+    if ldx is None or ldy is None or ldr is None:
         # rows that no single stride walks, e.g. prefixes [B, L, k] of wider slots:
         # one product per leading index
         if x.dim() < 3 or (gate is not None and gate.dim() == 2 and gate.shape[0] != x.shape[0]):
@@ -192,11 +211,12 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
                        gate=gate[i] if gate is not None and gate.dim() == 2 else gate,
                        residual=None if residual is None else residual[i], out=out[i])
         return out
-    (_, ldx), (_, ldy), (_, ldr) = views
-    if (x.data_ptr() | weight.data_ptr()) % 16 or ldx % 8 or ldw % 8:
+    xp, wp = x.data_ptr(), weight.data_ptr()
+    if (xp | wp) % 16 or (ldx | ldw) % 8:
         raise ValueError("rows of x and weight must start on 16 bytes (strides multiples of 8)")
-    _native.call("erd_linear_act", x.device, _native.DTYPE_CODES[x.dtype], x.data_ptr(), ldx,
-                 weight.data_ptr(), ldw, _native.ptr(bias), code, _native.ptr(gate), gate_rows,
-                 _native.ptr(residual), ldr, out.data_ptr(), ldy, m, n, k,
-                 _native.status_pointer(x.device))
+    _native.call("erd_linear_act", device, _native.DTYPE_CODES[dtype], xp, ldx, wp, ldw,
+                 None if bias is None else bias.data_ptr(), code,
+                 None if gate is None else gate.data_ptr(), gate_rows,
+                 None if residual is None else residual.data_ptr(), ldr, out.data_ptr(), ldy, m, n,
+                 k, _native.status_pointer(device))
     return out

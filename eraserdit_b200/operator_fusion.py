@@ -161,6 +161,26 @@ def apply_fused_qk_rmsnorm_rope(query: torch.Tensor, key: torch.Tensor, query_no
     return q_out, k_out
 
 
+def _head_norm(what: str, x: torch.Tensor, norm: Any) -> tuple[torch.Tensor | None, float]:
+    """Weight and eps of a norm over one head of ``x``."""
+    weight = getattr(norm, "weight", None)
+    if getattr(norm, "bias", None) is not None:
+        raise ValueError(f"{what}_norm must have no bias")
+    eps = getattr(norm, "eps", None)
+    if eps is None:  # torch.nn.RMSNorm's default
+        eps = torch.finfo(x.dtype).eps
+    eps = float(eps)
+    if not eps >= 0:
+        raise ValueError(f"{what}_norm needs eps >= 0")
+    if weight is not None:
+        if weight.shape != x.shape[-1:] or not weight.is_contiguous():
+            raise ValueError(f"{what}_norm needs a contiguous weight of one head's width")
+        if weight.dtype not in (x.dtype, torch.float32) or weight.device != x.device:
+            raise ValueError(f"{what}_norm needs a weight of the inputs' type or FP32 on their "
+                             "device")
+    return weight, eps
+
+
 def apply_fused_qk_head_rmsnorm_rotary(query: torch.Tensor, key: torch.Tensor | None,
                                        query_norm: Any, key_norm: Any,
                                        rotary: RotaryPositions | None,
@@ -179,30 +199,9 @@ def apply_fused_qk_head_rmsnorm_rotary(query: torch.Tensor, key: torch.Tensor | 
     which normalises across all heads, rounds after each step as its reference
     does).  ``query_out`` / ``key_out`` may be the inputs themselves.
     """
-    weights, epsilons = [], []
-    for what, x, norm in (("query", query, query_norm), ("key", key, key_norm)):
-        if x is None:
-            weights.append(None)
-            epsilons.append(1.0)
-            continue
-        weight = _norm_weight(norm)
-        if getattr(norm, "bias", None) is not None:
-            raise ValueError(f"{what}_norm must have no bias")
-        eps = getattr(norm, "eps", None)
-        if eps is None:  # torch.nn.RMSNorm's default
-            eps = torch.finfo(x.dtype).eps
-        if not float(eps) >= 0:
-            raise ValueError(f"{what}_norm needs eps >= 0")
-        if weight is not None:
-            if weight.shape != (x.shape[-1],) or not weight.is_contiguous():
-                raise ValueError(f"{what}_norm needs a contiguous weight of one head's width")
-            if weight.dtype not in (x.dtype, torch.float32) or weight.device != x.device:
-                raise ValueError(f"{what}_norm needs a weight of the inputs' type or FP32 on their "
-                                 "device")
-        weights.append(weight)
-        epsilons.append(float(eps))
-    if weights[0] is not None and weights[1] is not None and weights[0].dtype != weights[1].dtype:
+    q_weight, q_eps = _head_norm("query", query, query_norm)
+    k_weight, k_eps = (None, 1.0) if key is None else _head_norm("key", key, key_norm)
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         raise ValueError("query_norm and key_norm need weights of one type")
     return head_rotary_call("apply_fused_qk_head_rmsnorm_rotary", query, key, rotary, positions,
-                            weights[0], weights[1], True, epsilons[0], epsilons[1], False,
-                            query_out, key_out)
+                            q_weight, k_weight, True, q_eps, k_eps, False, query_out, key_out)

@@ -251,7 +251,7 @@ def _positions_args(rotary: RotaryPositions, positions, batch: int, tokens: int)
         raise ValueError("positions must be an int or an int32 / int64 tensor")
     if positions.device != rotary.device:
         raise ValueError("positions and the rotary frequencies are on different devices")
-    shape, strides, axis = tuple(positions.shape), positions.stride(), 0
+    shape, strides, axis = positions.shape, positions.stride(), 0
     if rotary.axes > 1:
         if len(shape) < 2 or shape[0] != rotary.axes:
             raise ValueError(f"positions must be [{rotary.axes}, S] or [{rotary.axes}, B, S]")
@@ -262,37 +262,47 @@ def _positions_args(rotary: RotaryPositions, positions, batch: int, tokens: int)
         per_batch, per_token = (strides[0] if shape[0] == batch else 0), strides[1]
     else:
         raise ValueError(f"positions must cover [{tokens}] or [{batch}, {tokens}] tokens")
-    return (positions.data_ptr(), int(positions.dtype == torch.int64), axis, per_batch, per_token, 0)
+    return positions.data_ptr(), positions.dtype == torch.int64, axis, per_batch, per_token, 0
 
 
-def _check_heads(what: str, x: torch.Tensor, like: torch.Tensor | None = None) -> None:
+def _check_heads(what: str, x: torch.Tensor, like: torch.Tensor | None = None) -> tuple:
+    """The checks of a [B, S, H, D] operand; its (token, head, batch) strides."""
     if x.dim() != 4 or not x.is_cuda or x.dtype not in _native.DTYPE_CODES:
         raise ValueError(f"{what} must be a CUDA BF16, FP16 or FP32 [B, S, H, D] tensor")
-    if x.stride(3) != 1 and x.shape[3] > 1:
+    batch, token, head, channel = x.stride()
+    if channel != 1 and x.shape[3] > 1:
         raise ValueError(f"{what} must have a contiguous head_dim")
     if like is not None and (x.dtype != like.dtype or x.device != like.device
                              or x.shape[:2] != like.shape[:2] or x.shape[3] != like.shape[3]):
         raise ValueError(f"{what} must match the query's type, device, tokens and head_dim")
+    return token, head, batch
 
 
-def _check_out(what: str, out: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+def _check_out(what: str, out: torch.Tensor, x: torch.Tensor) -> tuple:
     if out.shape != x.shape:
         raise ValueError(f"{what} must have its input's shape")
-    _check_heads(what, out, x)
     if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
         raise ValueError(f"{what} must not be an expanded view")
-    return out
+    return _check_heads(what, out, x)
+
+
+def _new_out(x: torch.Tensor) -> tuple[torch.Tensor, tuple]:
+    """An empty contiguous tensor of x's shape and its (token, head, batch) strides."""
+    _, tokens, heads, dim = x.shape
+    return x.new_empty(x.shape), (heads * dim, dim, tokens * heads * dim)
 
 
 def head_rotary_call(what: str, query, key, rotary, positions, q_weight, k_weight, norm: bool,
                      q_eps: float, k_eps: float, inverse: bool, query_out, key_out) -> tuple:
     """Checks and launch shared by the rotation with and without the norm."""
-    _check_heads("query", query)
-    if key is not None:
-        _check_heads("key", key, query)
-    _native.refuse_gradients(what, query, key, q_weight, k_weight)
+    q_strides, k_strides = _check_heads("query", query), (0, 0, 0)
     batch, tokens, heads, dim = query.shape
-    kv_heads = 0 if key is None else key.shape[2]
+    kv_heads, k_out, k_ptr, ko_ptr, ko_strides = 0, None, None, None, (0, 0, 0)
+    if key is not None:
+        k_strides = _check_heads("key", key, query)
+        kv_heads, k_ptr = key.shape[2], key.data_ptr()
+    if torch.is_grad_enabled():
+        _native.refuse_gradients(what, query, key, q_weight, k_weight)
     if rotary is not None:
         if not isinstance(rotary, RotaryPositions):
             raise ValueError("rotary must be a RotaryPositions")
@@ -301,36 +311,38 @@ def head_rotary_call(what: str, query, key, rotary, positions, q_weight, k_weigh
         if rotary.device != query.device:
             raise ValueError("rotary lives on another device than the query")
         where = _positions_args(rotary, positions, batch, tokens)
-        turn = (rotary.turns.data_ptr(), rotary.amplitude, int(inverse), rotary.second_axis,
+        turn = (rotary.turns.data_ptr(), rotary.amplitude, inverse, rotary.second_axis,
                 rotary.third_axis)
-        rotary_dim, interleaved = rotary.rotary_dim, int(rotary.layout == "interleaved")
+        rotary_dim, interleaved = rotary.rotary_dim, rotary.layout == "interleaved"
     else:
         where, turn = (None, 0, 0, 0, 0, 0), (None, 1.0, 0, 0, 0)
         rotary_dim = interleaved = 0
-    q_out = torch.empty(query.shape, dtype=query.dtype, device=query.device) \
-        if query_out is None else _check_out("query_out", query_out, query)
-    k_out = None
+    if query_out is None:
+        q_out, qo_strides = _new_out(query)
+    else:
+        q_out, qo_strides = query_out, _check_out("query_out", query_out, query)
     if key is not None:
-        k_out = torch.empty(key.shape, dtype=key.dtype, device=key.device) \
-            if key_out is None else _check_out("key_out", key_out, key)
+        if key_out is None:
+            k_out, ko_strides = _new_out(key)
+        else:
+            k_out, ko_strides = key_out, _check_out("key_out", key_out, key)
+        ko_ptr = k_out.data_ptr()
     elif key_out is not None:
         raise ValueError("key_out needs a key")
     if batch * tokens * (heads + kv_heads) * dim == 0:
         return q_out, k_out
     if heads == 0:
         raise ValueError("the query needs at least one head")
-    strides = lambda t: (0, 0, 0) if t is None else (t.stride(1), t.stride(2), t.stride(0))
     weight = q_weight if q_weight is not None else k_weight
+    device = query.device
     _native.call(
-        "erd_head_norm_rotary", query.device, _native.DTYPE_CODES[query.dtype], query.data_ptr(),
-        _native.ptr(key), *strides(query), *strides(key), batch, tokens, heads, kv_heads, dim,
-        rotary_dim, interleaved, int(norm), _native.ptr(q_weight), _native.ptr(k_weight),
-        int(weight is not None and weight.dtype == torch.float32), q_eps, k_eps, *turn, *where,
-        q_out.data_ptr(), _native.ptr(k_out), *strides(q_out), *strides(k_out))
-    if rotary is not None:
-        stream = torch.cuda.current_stream(query.device)
-        if stream.cuda_stream != rotary._stream:
-            rotary.turns.record_stream(stream)
+        "erd_head_norm_rotary", device, _native.DTYPE_CODES[query.dtype], query.data_ptr(), k_ptr,
+        *q_strides, *k_strides, batch, tokens, heads, kv_heads, dim, rotary_dim, interleaved, norm,
+        _native.ptr(q_weight), _native.ptr(k_weight),
+        weight is not None and weight.dtype == torch.float32, q_eps, k_eps, *turn, *where,
+        q_out.data_ptr(), ko_ptr, *qo_strides, *ko_strides)
+    if rotary is not None and _native.raw_stream(device.index) != rotary._stream:
+        rotary.turns.record_stream(torch.cuda.current_stream(device))
     return q_out, k_out
 
 
