@@ -413,27 +413,32 @@ __global__ void __launch_bounds__(32 * kRowSelectWarps) row_select_kernel(const 
 }
 
 // -------------------------------------------------- attention of 128-row tiles
-// One CTA a query tile (two CTAs a multiprocessor, so one's softmax runs beside
-// the other's products): warps 0-3 softmax, one thread a row; warp 4 TMA
-// producer; warp 5 MMA issuer.  A step is 128 keys: two 64-key pieces, which
-// need not be neighbours (the two halves of a key block of 128, or two chosen
-// blocks of 64).  TMEM: S 128 columns, O 64, P 64.
+// One CTA a query tile, two CTAs a multiprocessor: warps 0-3 softmax, one thread
+// a row; warp 4 TMA producer; warp 5 MMA issuer.  A step is one 64-key piece of
+// a chosen block.  TMEM: three score buffers of 64 columns and O (64).  P is
+// written over the scores it came from, so a buffer goes S -> P -> free, and the
+// issuer keeps two products S ahead of the softmax: the chain P ready -> QK ->
+// S ready (some 830 clocks with one buffer of 128 keys) and the wait for the
+// previous P V leave the softmax's path.
 constexpr int kTileThreads = 192;
-constexpr int kKStages = 3, kVStages = 2;
-constexpr int kTileBytes = kTile * kDim * 2;  // 16 KB
+constexpr int kBufs = 3;                     // score buffers
+constexpr int kKStages = 5, kVStages = 5;    // 64-key pieces of K and of V
+constexpr int kTileBytes = kTile * kDim * 2;   // Q, 16 KB
+constexpr int kPieceBytes = kHalf * kDim * 2;  // 8 KB
 constexpr float kRescale = 8.0f;  // log2 units the running maximum may lag behind
 
 struct __align__(8) TileBarriers {
   uint64_t q_full;
   uint64_t k_full[kKStages], k_empty[kKStages];
   uint64_t v_full[kVStages], v_empty[kVStages];
-  uint64_t s_full, p_full, o_done, drain;
+  uint64_t s_full[kBufs], p_full[kBufs];
+  uint64_t o_done[2], drain;  // P V of even and of odd steps
   uint32_t tmem_base;
   int abort;
 };
 constexpr int kTileSmemK = kTileBytes;
-constexpr int kTileSmemV = kTileSmemK + kKStages * kTileBytes;
-constexpr int kTileSmemBar = kTileSmemV + kVStages * kTileBytes;
+constexpr int kTileSmemV = kTileSmemK + kKStages * kPieceBytes;
+constexpr int kTileSmemBar = kTileSmemV + kVStages * kPieceBytes;
 constexpr int kTileSmemLaunch = kTileSmemBar + 512 + 1024;  // + base alignment
 static_assert(2 * (kTileSmemLaunch + 1024) <= 228 * 1024, "two CTAs a multiprocessor");
 static_assert(sizeof(TileBarriers) <= 512, "barrier block");
@@ -449,10 +454,8 @@ struct TileParams {
   int* status;
 };
 
-// First key of 64-key piece `i` of a tile's list (kv_len where there is none,
-// which TMA reads as zeros).
-__device__ __forceinline__ int piece_key(const TileParams& p, const int* list, int i, int pieces) {
-  if (i >= pieces) return p.kv_len;
+// First key of 64-key piece `i` of a tile's list.
+__device__ __forceinline__ int piece_key(const TileParams& p, const int* list, int i) {
   const int shift = p.key_block >> 7;  // pieces of a block: 1 << shift
   return __ldg(list + (i >> shift)) * p.key_block + (i & shift) * kHalf;
 }
@@ -480,8 +483,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   const int tile = blockIdx.x, head = blockIdx.y, batch = blockIdx.z;
   const int len = key_length(p.lengths, batch, p.kv_len);
   const int kept = min(p.topk, (len + p.key_block - 1) / p.key_block);
-  const int pieces = kept << (p.key_block >> 7);
-  const int steps = (pieces + 1) / 2;
+  const int steps = kept << (p.key_block >> 7);  // 64-key pieces
   const int* list =
       p.selection +
       ((static_cast<long long>(batch) * gridDim.y + head) * gridDim.x + tile) * p.topk;
@@ -507,9 +509,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       mbar_init(smem_u32(&bars->v_full[s]), 1);
       mbar_init(smem_u32(&bars->v_empty[s]), 1);
     }
-    mbar_init(smem_u32(&bars->s_full), 1);
-    mbar_init(smem_u32(&bars->p_full), kTile);
-    mbar_init(smem_u32(&bars->o_done), 1);
+    for (int i = 0; i < kBufs; ++i) {
+      mbar_init(smem_u32(&bars->s_full[i]), 1);
+      mbar_init(smem_u32(&bars->p_full[i]), kTile);
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&bars->o_done[i]), 1);
     mbar_init(smem_u32(&bars->drain), 1);
     bars->abort = 0;
     fence_mbar_init();
@@ -534,23 +538,23 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       mbar_arrive_expect_tx(q_bar, kTileBytes);
       tma_load_5d(sQ, &tmap_q, q_bar, 0, tile * kTile, head, batch, 0);
       int j = 0;
+      uint32_t ks = 0, kph = 0, vs = 0, vph = 0;
       for (; j < steps; ++j) {
-        const int a = piece_key(p, list, 2 * j, pieces), b = piece_key(p, list, 2 * j + 1, pieces);
-        const int ks = j % kKStages, vs = j % kVStages;
-        if (!mbar_wait(smem_u32(&bars->k_empty[ks]), ((j / kKStages) & 1) ^ 1, abort, p.status,
+        const int key = piece_key(p, list, j);
+        if (!mbar_wait(smem_u32(&bars->k_empty[ks]), kph ^ 1, abort, p.status,
                        kStatusTimeoutProducer))
           break;
-        const uint32_t kb = smem_u32(&bars->k_full[ks]), kd = sK + ks * kTileBytes;
-        mbar_arrive_expect_tx(kb, kTileBytes);
-        tma_load_5d(kd, &tmap_k, kb, 0, a, kv_head, batch, 0);
-        tma_load_5d(kd + kTileBytes / 2, &tmap_k, kb, 0, b, kv_head, batch, 0);
-        if (!mbar_wait(smem_u32(&bars->v_empty[vs]), ((j / kVStages) & 1) ^ 1, abort, p.status,
+        const uint32_t kb = smem_u32(&bars->k_full[ks]);
+        mbar_arrive_expect_tx(kb, kPieceBytes);
+        tma_load_5d(sK + ks * kPieceBytes, &tmap_k, kb, 0, key, kv_head, batch, 0);
+        if (++ks == kKStages) ks = 0, kph ^= 1;
+        if (!mbar_wait(smem_u32(&bars->v_empty[vs]), vph ^ 1, abort, p.status,
                        kStatusTimeoutProducer))
           break;
-        const uint32_t vb = smem_u32(&bars->v_full[vs]), vd = sV + vs * kTileBytes;
-        mbar_arrive_expect_tx(vb, kTileBytes);
-        tma_load_5d(vd, &tmap_v, vb, 0, a, kv_head, batch, 0);
-        tma_load_5d(vd + kTileBytes / 2, &tmap_v, vb, 0, b, kv_head, batch, 0);
+        const uint32_t vb = smem_u32(&bars->v_full[vs]);
+        mbar_arrive_expect_tx(vb, kPieceBytes);
+        tma_load_5d(sV + vs * kPieceBytes, &tmap_v, vb, 0, key, kv_head, batch, 0);
+        if (++vs == kVStages) vs = 0, vph ^= 1;
       }
       if (*abort) {
         // Let every load this thread may have started land before the CTA exits.
@@ -564,44 +568,48 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   } else if (warp == 5) {
     // ---------------------------------------------------------- MMA issuer
     if (elect_one()) {
-      constexpr uint32_t id_qk = idesc<kBf16>(kTile, kTile, false);
+      constexpr uint32_t id_qk = idesc<kBf16>(kTile, kHalf, false);
       constexpr uint32_t id_pv = idesc<kBf16>(kTile, kDim, true);
-      const uint32_t tS = tmem, tO = tmem + 128, tP = tmem + 192;
+      const uint32_t tO = tmem + kBufs * kHalf;
       const uint64_t dq = sdesc_sw128(sQ, 16, 1024);
       const uint64_t dk0 = sdesc_sw128(sK, 16, 1024), dv0 = sdesc_sw128(sV, 1024, 1024);
       uint32_t ks = 0, kph = 0, vs = 0, vph = 0;  // next stages to be read
+      uint32_t qb = 0;                            // next score buffer to be written
+      // S of the next piece.  Its buffer's P was read by a product issued before:
+      // products execute in the order of their issue.
       auto issue_qk = [&]() {
-        const uint64_t dk = dk0 + ks * (kTileBytes / 16);
+        if (!mbar_wait(smem_u32(&bars->k_full[ks]), kph, abort, p.status, kStatusTimeoutMma))
+          return false;
+        tc_fence_after();
+        const uint64_t dk = dk0 + ks * (kPieceBytes / 16);
 #pragma unroll
         for (int k = 0; k < kDim / 16; ++k)
-          mma_bf16_ss(tS, dq + 2 * k, dk + 2 * k, id_qk, k > 0);
-        mma_commit(smem_u32(&bars->s_full));
+          mma_bf16_ss(tmem + qb * kHalf, dq + 2 * k, dk + 2 * k, id_qk, k > 0);
+        mma_commit(smem_u32(&bars->s_full[qb]));
         mma_commit(smem_u32(&bars->k_empty[ks]));
         if (++ks == kKStages) ks = 0, kph ^= 1;
+        if (++qb == kBufs) qb = 0;
+        return true;
       };
-      bool ok = mbar_wait(smem_u32(&bars->q_full), 0, abort, p.status, kStatusTimeoutMma) &&
-                mbar_wait(smem_u32(&bars->k_full[0]), 0, abort, p.status, kStatusTimeoutMma);
-      if (ok) {
-        tc_fence_after();
-        issue_qk();
-      }
+      bool ok = mbar_wait(smem_u32(&bars->q_full), 0, abort, p.status, kStatusTimeoutMma);
+      for (int j = 0; ok && j < kBufs && j < steps; ++j) ok = issue_qk();
+      uint32_t pb = 0, pph = 0;
       for (int j = 0; ok && j < steps; ++j) {
-        const bool more = j + 1 < steps;
-        if (more &&
-            !mbar_wait(smem_u32(&bars->k_full[ks]), kph, abort, p.status, kStatusTimeoutMma))
-          break;
         if (!mbar_wait(smem_u32(&bars->v_full[vs]), vph, abort, p.status, kStatusTimeoutMma))
           break;
-        if (!mbar_wait(smem_u32(&bars->p_full), j & 1, abort, p.status, kStatusTimeoutMma)) break;
+        if (!mbar_wait(smem_u32(&bars->p_full[pb]), pph, abort, p.status, kStatusTimeoutMma))
+          break;
         tc_fence_after();
-        if (more) issue_qk();
-        const uint64_t dv = dv0 + vs * (kTileBytes / 16);
+        const uint64_t dv = dv0 + vs * (kPieceBytes / 16);
 #pragma unroll
-        for (int k = 0; k < kTile / 16; ++k)
-          mma_bf16_ts(tO, tP + k * 8, dv + k * (2048 / 16), id_pv, (j > 0 || k > 0) ? 1u : 0u);
-        mma_commit(smem_u32(&bars->o_done));
+        for (int k = 0; k < kHalf / 16; ++k)
+          mma_bf16_ts(tO, tmem + pb * kHalf + k * 8, dv + k * (2048 / 16), id_pv,
+                      (j > 0 || k > 0) ? 1u : 0u);
+        mma_commit(smem_u32(&bars->o_done[j & 1]));
         mma_commit(smem_u32(&bars->v_empty[vs]));
         if (++vs == kVStages) vs = 0, vph ^= 1;
+        if (++pb == kBufs) pb = 0, pph ^= 1;
+        if (j + kBufs < steps) ok = issue_qk();
       }
       // Every product completes before TMEM is released.
       mma_commit(smem_u32(&bars->drain));
@@ -610,38 +618,40 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   } else {
     // ------------------------------------------------------------- softmax
     const uint32_t lane_off = static_cast<uint32_t>(warp * 32) << 16;
-    const uint32_t tS = tmem + lane_off, tO = tmem + 128 + lane_off, tP = tmem + 192 + lane_off;
+    const uint32_t tO = tmem + kBufs * kHalf + lane_off;
     const float c = p.scale_log2;
     float m_run = -CUDART_INF_F, l_run = 0.f;  // running maximum (log2 domain) and sum
     bool ok = true;
+    uint32_t buf = 0, sph = 0;
+    // Whole-warp wait for P V of step j (called for every j, in order: the next
+    // phase of that barrier needs a P that this warp has not handed over yet).
+    auto pv_done = [&](int j) {
+      return __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->o_done[j & 1]), (j >> 1) & 1, abort,
+                                               p.status, kStatusTimeoutSoftmax));
+    };
     for (int j = 0; j < steps; ++j) {
-      // Valid keys of the step's two pieces (read before the wait).
-      const int key_a = piece_key(p, list, 2 * j, pieces);
-      const int key_b = piece_key(p, list, 2 * j + 1, pieces);
-      const int na = min(max(len - key_a, 0), kHalf), nb = min(max(len - key_b, 0), kHalf);
-      const bool whole = na == kHalf && nb == kHalf;
-      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->s_full), j & 1, abort, p.status,
+      const int n = min(len - piece_key(p, list, j), kHalf);  // valid keys of the piece
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->s_full[buf]), sph, abort, p.status,
                                              kStatusTimeoutSoftmax))) {
         ok = false;
         break;
       }
       tc_fence_after();
+      const uint32_t tS = tmem + buf * kHalf + lane_off;
+      uint32_t sr[kHalf];
+      tmem_ld_wait_64(tS, sr);
+      if (n < kHalf) {
+#pragma unroll
+        for (int i = 0; i < kHalf; ++i)
+          if (i >= n) sr[i] = __float_as_uint(-CUDART_INF_F);
+      }
       float mx0 = -CUDART_INF_F, mx1 = -CUDART_INF_F, mx2 = -CUDART_INF_F, mx3 = -CUDART_INF_F;
-      {
-        uint32_t sr[128];
-        tmem_ld_wait_128(tS, sr);
-        if (!whole) {
 #pragma unroll
-          for (int i = 0; i < kTile; ++i)
-            if (i < kHalf ? i >= na : i - kHalf >= nb) sr[i] = __float_as_uint(-CUDART_INF_F);
-        }
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          mx0 = fmax3(mx0, __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
-          mx1 = fmax3(mx1, __uint_as_float(sr[32 + i]), __uint_as_float(sr[33 + i]));
-          mx2 = fmax3(mx2, __uint_as_float(sr[64 + i]), __uint_as_float(sr[65 + i]));
-          mx3 = fmax3(mx3, __uint_as_float(sr[96 + i]), __uint_as_float(sr[97 + i]));
-        }
+      for (int i = 0; i < 16; i += 2) {
+        mx0 = fmax3(mx0, __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
+        mx1 = fmax3(mx1, __uint_as_float(sr[16 + i]), __uint_as_float(sr[17 + i]));
+        mx2 = fmax3(mx2, __uint_as_float(sr[32 + i]), __uint_as_float(sr[33 + i]));
+        mx3 = fmax3(mx3, __uint_as_float(sr[48 + i]), __uint_as_float(sr[49 + i]));
       }
       const float m_tile = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * c;
       float m_new = m_run;
@@ -650,15 +660,17 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         m_new = m_tile;
         rescale = j > 0;
       }
-      if (j > 0) {  // P and O are free once the previous product has completed
-        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->o_done), (j - 1) & 1, abort,
-                                               p.status, kStatusTimeoutSoftmax))) {
+      // Followed at a distance of two steps, so that no phase is missed.
+      if (j > 1 && !pv_done(j - 2)) {
+        ok = false;
+        break;
+      }
+      if (__any_sync(0xffffffffu, rescale)) {
+        if (!pv_done(j - 1)) {  // O holds every product so far
           ok = false;
           break;
         }
         tc_fence_after();
-      }
-      if (__any_sync(0xffffffffu, rescale)) {
         const float alpha = rescale ? ex2_approx(m_run - m_new) : 1.0f;
         l_run *= alpha;
 #pragma unroll
@@ -674,31 +686,21 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       // A row that has met only -inf so far weighs those keys 0.
       const float neg_m = m_new == -CUDART_INF_F ? 0.f : -m_new;
       float sum0 = 0.f, sum1 = 0.f;
+      uint32_t pk[32];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t pk[32], sr[64];
-        tmem_ld_wait_64(tS + h * 64, sr);
-        if (!whole) {
-          const int n = h ? nb : na;
-#pragma unroll
-          for (int i = 0; i < kHalf; ++i)
-            if (i >= n) sr[i] = __float_as_uint(-CUDART_INF_F);
-        }
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float x0, x1;
-          fma2(x0, x1, __uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1]), c, c, neg_m,
-               neg_m);
-          const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-          add2(sum0, sum1, sum0, sum1, p0, p1);
-          pk[i] = pack2<T>(p0, p1);
-        }
-        tmem_st32(tP + h * 32, pk);
+      for (int i = 0; i < 32; ++i) {
+        float x0, x1;
+        fma2(x0, x1, __uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1]), c, c, neg_m,
+             neg_m);
+        const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+        add2(sum0, sum1, sum0, sum1, p0, p1);
+        pk[i] = pack2<T>(p0, p1);
       }
+      tmem_st32(tS, pk);
       l_run += sum0 + sum1;
       // Rows of V behind the sequence's end may hold anything (0 * NaN is NaN):
       // they are cleared before the product reads them.
-      if (!whole && len < p.kv_len) {
+      if (n < kHalf && len < p.kv_len) {
         const int vs = j % kVStages;
         if (!__all_sync(0xffffffffu,
                         mbar_wait(smem_u32(&bars->v_full[vs]), (j / kVStages) & 1, abort, p.status,
@@ -706,8 +708,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
           ok = false;
           break;
         }
-        if ((row & (kHalf - 1)) >= (row < kHalf ? na : nb)) {
-          uint4* v = reinterpret_cast<uint4*>(smem + kTileSmemV + vs * kTileBytes + row * 128);
+        if (row < kHalf && row >= n) {
+          uint4* v = reinterpret_cast<uint4*>(smem + kTileSmemV + vs * kPieceBytes + row * 128);
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
         }
@@ -715,10 +717,10 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       }
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(smem_u32(&bars->p_full));
+      mbar_arrive(smem_u32(&bars->p_full[buf]));
+      if (++buf == kBufs) buf = 0, sph ^= 1;
     }
-    if (ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->o_done), (steps - 1) & 1, abort,
-                                                p.status, kStatusTimeoutEpilogue))) {
+    if (ok && (steps < 2 || pv_done(steps - 2)) && pv_done(steps - 1)) {
       tc_fence_after();
       uint32_t o[64];
       tmem_ld_wait_64(tO, o);
