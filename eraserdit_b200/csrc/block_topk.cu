@@ -413,35 +413,38 @@ __global__ void __launch_bounds__(32 * kRowSelectWarps) row_select_kernel(const 
 }
 
 // -------------------------------------------------- attention of 128-row tiles
-// One CTA a query tile, two CTAs a multiprocessor: warps 0-3 softmax, one thread
-// a row; warp 4 TMA producer; warp 5 MMA issuer.  A step is one 64-key piece of
-// a chosen block.  TMEM: three score buffers of 64 columns and O (64).  P is
-// written over the scores it came from, so a buffer goes S -> P -> free, and the
-// issuer keeps two products S ahead of the softmax: the chain P ready -> QK ->
-// S ready (some 830 clocks with one buffer of 128 keys) and the wait for the
-// previous P V leave the softmax's path.
-constexpr int kTileThreads = 192;
-constexpr int kBufs = 3;                     // score buffers
-constexpr int kKStages = 5, kVStages = 5;    // 64-key pieces of K and of V
+// One CTA a query tile, four CTAs a multiprocessor.  A step is one 64-key piece
+// of a chosen block.  Warps 0-3 softmax, one thread a row; one thread of warp 4
+// loads (TMA) and issues the products.  TMEM: scores 64 columns, O 64; P is
+// written over the scores it came from.
+//
+// A CTA's steps are a chain (S ready -> softmax -> P V and the next Q K -> S
+// ready) of which the exponentials (8192 a step, 16 a clock and multiprocessor)
+// are 512 clocks at least.  Four chains keep that unit and the tensor cores
+// busy where two (with their buffers doubled instead) reached 65 % and 32 %:
+// 1.59 ms at 32640 tokens x 32 heads, 64 of 510 blocks.
+//
+// The chain also orders everything else.  When every row's P of step j has
+// arrived, S(j) had been ready, so Q K(j) and P V(j - 1) had completed: their
+// stages of K and V are free without further barriers, and O may be rescaled.
+constexpr int kTileThreads = 160;
+constexpr int kStages = 2;                     // 64-key pieces of K and of V
 constexpr int kTileBytes = kTile * kDim * 2;   // Q, 16 KB
 constexpr int kPieceBytes = kHalf * kDim * 2;  // 8 KB
 constexpr float kRescale = 8.0f;  // log2 units the running maximum may lag behind
 
 struct __align__(8) TileBarriers {
-  uint64_t q_full;
-  uint64_t k_full[kKStages], k_empty[kKStages];
-  uint64_t v_full[kVStages], v_empty[kVStages];
-  uint64_t s_full[kBufs], p_full[kBufs];
-  uint64_t o_done[2], drain;  // P V of even and of odd steps
+  uint64_t q_full, k_full[kStages], v_full[kStages];
+  uint64_t s_full, p_full, o_done;
   uint32_t tmem_base;
   int abort;
 };
 constexpr int kTileSmemK = kTileBytes;
-constexpr int kTileSmemV = kTileSmemK + kKStages * kPieceBytes;
-constexpr int kTileSmemBar = kTileSmemV + kVStages * kPieceBytes;
-constexpr int kTileSmemLaunch = kTileSmemBar + 512 + 1024;  // + base alignment
-static_assert(2 * (kTileSmemLaunch + 1024) <= 228 * 1024, "two CTAs a multiprocessor");
-static_assert(sizeof(TileBarriers) <= 512, "barrier block");
+constexpr int kTileSmemV = kTileSmemK + kStages * kPieceBytes;
+constexpr int kTileSmemBar = kTileSmemV + kStages * kPieceBytes;
+constexpr int kTileSmemLaunch = kTileSmemBar + 256 + 1024;  // + base alignment
+static_assert(4 * (kTileSmemLaunch + 1024) <= 228 * 1024, "four CTAs a multiprocessor");
+static_assert(sizeof(TileBarriers) <= 256, "barrier block");
 
 struct TileParams {
   int q_len, kv_len, per;  // per: query heads of a key head
@@ -453,6 +456,96 @@ struct TileParams {
   Strides o_st;
   int* status;
 };
+
+// Maximum of three, NaN if one is.
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Loads 16 TMEM columns of this thread's lane and waits for them.
+__device__ __forceinline__ void tmem_ld_wait_16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// 2^x for a pair of x <= kRescale on the FMA pipe: exp2_poly2 (a cubic, 7.5e-5 of
+// the value, against BF16's 2^-9), and for FP16 weights (2^-12) the same split
+// with the quartic that minimises the relative error on [0, 1) (2.7e-6,
+// minimax_exp2(4) of gen_exp2_poly.py).  Below 2^-126 both give 2^-126.
+template <typename T>
+__device__ __forceinline__ void exp2_fma(float x0, float x1, float& y0, float& y1) {
+  exp2_poly2(x0, x1, y0, y1);
+}
+template <>
+__device__ __forceinline__ void exp2_fma<__half>(float x0, float x1, float& y0, float& y1) {
+  constexpr float c0 = 0x1.00002cp+0f, c1 = 0x1.62d164p-1f, c2 = 0x1.ee79bep-3f,
+                  c3 = 0x1.aa12a4p-5f, c4 = 0x1.bb7f6ep-7f;
+  x0 = fmaxf(x0, -126.0f);
+  x1 = fmaxf(x1, -126.0f);
+  float t0, t1, j0, j1, f0, f1, p0, p1;
+  add2_rm(t0, t1, x0, x1, kRoundMagic, kRoundMagic);  // t = magic + floor(x)
+  sub2(j0, j1, t0, t1, kRoundMagic, kRoundMagic);     // floor(x), exact
+  sub2(f0, f1, x0, x1, j0, j1);                       // f in [0, 1), exact
+  fma2(p0, p1, c4, c4, f0, f1, c3, c3);
+  fma2(p0, p1, p0, p1, f0, f1, c2, c2);
+  fma2(p0, p1, p0, p1, f0, f1, c1, c1);
+  fma2(p0, p1, p0, p1, f0, f1, c0, c0);
+  y0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+  y1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+}
+
+// Of every four pairs of a row's weights one takes the FMA pipe and three MUFU,
+// whose work four chains are bound by first: 32640 tokens x 16 heads took 805 us
+// with none, 756 with one in eight, 727 with two, 773 with three.
+constexpr int kFmaEvery = 4;
+
+// Weights of one row's 64 scores, of which the first n count: P = 2^(S c - m) as
+// 16-bit pairs, their FP32 sum, and the maximum of S c.  What is masked or -inf
+// weighs 2^-126 in an FMA pair and 0 in the others (V's masked rows are zeros,
+// and a row that has met only -inf, m = -inf, is cleared at the end).  A score
+// that is NaN or +inf makes the sum NaN, as it makes the softmax.
+template <typename T>
+__device__ __forceinline__ void weigh(uint32_t tS, float c, float m, int n, uint32_t (&pk)[32],
+                                      float& sum, float& m_tile) {
+  uint32_t sr[kHalf];
+  tmem_ld_wait_64(tS, sr);
+  if (n < kHalf) {
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i)
+      if (i >= n) sr[i] = __float_as_uint(-CUDART_INF_F);
+  }
+  const float neg_m = m == -CUDART_INF_F ? 0.f : -m;
+  float sum0 = 0.f, sum1 = 0.f, mx0 = -CUDART_INF_F, mx1 = -CUDART_INF_F;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const float s0 = __uint_as_float(sr[2 * i]), s1 = __uint_as_float(sr[2 * i + 1]);
+    float x0, x1, p0, p1;
+    fma2(x0, x1, s0, s1, c, c, neg_m, neg_m);
+    if (i & 1)
+      mx1 = fmax3_nan(mx1, s0, s1);
+    else
+      mx0 = fmax3_nan(mx0, s0, s1);
+    if (i % kFmaEvery == 0) {
+      exp2_fma<T>(x0, x1, p0, p1);
+    } else {
+      p0 = ex2_approx(x0);
+      p1 = ex2_approx(x1);
+    }
+    add2(sum0, sum1, sum0, sum1, p0, p1);
+    pk[i] = pack2<T>(p0, p1);
+  }
+  m_tile = fmax3_nan(mx0, mx1, mx1) * c;
+  sum = m_tile < CUDART_INF_F ? sum0 + sum1 : CUDART_NAN_F;
+}
 
 // First key of 64-key piece `i` of a tile's list.
 __device__ __forceinline__ int piece_key(const TileParams& p, const int* list, int i) {
@@ -470,7 +563,7 @@ __host__ __device__ constexpr uint32_t idesc(int m, int n, bool b_mn_major) {
 }
 
 template <typename T, bool kBf16>
-__global__ void __launch_bounds__(kTileThreads, 2)
+__global__ void __launch_bounds__(kTileThreads, 4)
     tile_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
                      const __grid_constant__ CUtensorMap tmap_k,
                      const __grid_constant__ CUtensorMap tmap_v, const TileParams p) {
@@ -488,38 +581,36 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       p.selection +
       ((static_cast<long long>(batch) * gridDim.y + head) * gridDim.x + tile) * p.topk;
   const int row = threadIdx.x & 127;
-  const int tok = tile * kTile + row;
-  T* dst = static_cast<T*>(p.out) + batch * p.o_st.batch + head * p.o_st.head +
-           tok * p.o_st.token;
+  // this thread's row of the result, or null (computed where it is needed: the
+  // softmax has no registers to spare)
+  auto out_row = [&]() -> uint4* {
+    const int tok = static_cast<int>(blockIdx.x) * kTile + static_cast<int>(threadIdx.x);
+    if (threadIdx.x >= kTile || tok >= p.q_len) return nullptr;
+    return reinterpret_cast<uint4*>(static_cast<T*>(p.out) + blockIdx.z * p.o_st.batch +
+                                    blockIdx.y * p.o_st.head + tok * p.o_st.token);
+  };
   if (steps == 0) {  // no valid key: zeros
-    if (threadIdx.x < kTile && tok < p.q_len) {
+    if (uint4* dst = out_row()) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < 8; ++i) dst[i] = make_uint4(0u, 0u, 0u, 0u);
     }
     return;
   }
   volatile int* abort = &bars->abort;
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(&bars->q_full), 1);
-    for (int s = 0; s < kKStages; ++s) {
-      mbar_init(smem_u32(&bars->k_full[s]), 1);
-      mbar_init(smem_u32(&bars->k_empty[s]), 1);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(smem_u32(&bars->k_full[i]), 1);
+      mbar_init(smem_u32(&bars->v_full[i]), 1);
     }
-    for (int s = 0; s < kVStages; ++s) {
-      mbar_init(smem_u32(&bars->v_full[s]), 1);
-      mbar_init(smem_u32(&bars->v_empty[s]), 1);
-    }
-    for (int i = 0; i < kBufs; ++i) {
-      mbar_init(smem_u32(&bars->s_full[i]), 1);
-      mbar_init(smem_u32(&bars->p_full[i]), kTile);
-    }
-    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&bars->o_done[i]), 1);
-    mbar_init(smem_u32(&bars->drain), 1);
+    mbar_init(smem_u32(&bars->s_full), 1);
+    mbar_init(smem_u32(&bars->p_full), 4);  // one arrival a softmax warp
+    mbar_init(smem_u32(&bars->o_done), 1);
     bars->abort = 0;
     fence_mbar_init();
   }
   if (warp == 4) {
-    tmem_alloc(smem_u32(&bars->tmem_base), 256);
+    tmem_alloc(smem_u32(&bars->tmem_base), 2 * kHalf);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -528,188 +619,144 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   const uint32_t tmem = bars->tmem_base;
 
   if (warp == 4) {
-    // ------------------------------------------------------------ producer
+    // --------------------------------------------------- loads and products
     if (elect_one()) {
       tma_prefetch_desc(&tmap_q);
       tma_prefetch_desc(&tmap_k);
       tma_prefetch_desc(&tmap_v);
-      const int kv_head = head / p.per;
-      const uint32_t q_bar = smem_u32(&bars->q_full);
-      mbar_arrive_expect_tx(q_bar, kTileBytes);
-      tma_load_5d(sQ, &tmap_q, q_bar, 0, tile * kTile, head, batch, 0);
-      int j = 0;
-      uint32_t ks = 0, kph = 0, vs = 0, vph = 0;
-      for (; j < steps; ++j) {
-        const int key = piece_key(p, list, j);
-        if (!mbar_wait(smem_u32(&bars->k_empty[ks]), kph ^ 1, abort, p.status,
-                       kStatusTimeoutProducer))
-          break;
-        const uint32_t kb = smem_u32(&bars->k_full[ks]);
-        mbar_arrive_expect_tx(kb, kPieceBytes);
-        tma_load_5d(sK + ks * kPieceBytes, &tmap_k, kb, 0, key, kv_head, batch, 0);
-        if (++ks == kKStages) ks = 0, kph ^= 1;
-        if (!mbar_wait(smem_u32(&bars->v_empty[vs]), vph ^ 1, abort, p.status,
-                       kStatusTimeoutProducer))
-          break;
-        const uint32_t vb = smem_u32(&bars->v_full[vs]);
-        mbar_arrive_expect_tx(vb, kPieceBytes);
-        tma_load_5d(sV + vs * kPieceBytes, &tmap_v, vb, 0, key, kv_head, batch, 0);
-        if (++vs == kVStages) vs = 0, vph ^= 1;
-      }
-      if (*abort) {
-        // Let every load this thread may have started land before the CTA exits.
-        mbar_wait_drain(q_bar, 0);
-        for (int d = max(0, j - kKStages); d <= j && d < steps; ++d) {
-          mbar_wait_drain(smem_u32(&bars->k_full[d % kKStages]), (d / kKStages) & 1);
-          mbar_wait_drain(smem_u32(&bars->v_full[d % kVStages]), (d / kVStages) & 1);
-        }
-      }
-    }
-  } else if (warp == 5) {
-    // ---------------------------------------------------------- MMA issuer
-    if (elect_one()) {
       constexpr uint32_t id_qk = idesc<kBf16>(kTile, kHalf, false);
       constexpr uint32_t id_pv = idesc<kBf16>(kTile, kDim, true);
-      const uint32_t tO = tmem + kBufs * kHalf;
+      const uint32_t tO = tmem + kHalf;
       const uint64_t dq = sdesc_sw128(sQ, 16, 1024);
       const uint64_t dk0 = sdesc_sw128(sK, 16, 1024), dv0 = sdesc_sw128(sV, 1024, 1024);
-      uint32_t ks = 0, kph = 0, vs = 0, vph = 0;  // next stages to be read
-      uint32_t qb = 0;                            // next score buffer to be written
-      // S of the next piece.  Its buffer's P was read by a product issued before:
-      // products execute in the order of their issue.
-      auto issue_qk = [&]() {
-        if (!mbar_wait(smem_u32(&bars->k_full[ks]), kph, abort, p.status, kStatusTimeoutMma))
-          return false;
-        tc_fence_after();
-        const uint64_t dk = dk0 + ks * (kPieceBytes / 16);
+      const int kv_head = head / p.per;
+      int k_issued = 0, v_issued = 0;
+      auto load_k = [&](int j, int key) {
+        const uint32_t bar = smem_u32(&bars->k_full[j & 1]);
+        mbar_arrive_expect_tx(bar, kPieceBytes);
+        tma_load_5d(sK + (j & 1) * kPieceBytes, &tmap_k, bar, 0, key, kv_head, batch, 0);
+        k_issued = j + 1;
+      };
+      auto load_v = [&](int j, int key) {
+        const uint32_t bar = smem_u32(&bars->v_full[j & 1]);
+        mbar_arrive_expect_tx(bar, kPieceBytes);
+        tma_load_5d(sV + (j & 1) * kPieceBytes, &tmap_v, bar, 0, key, kv_head, batch, 0);
+        v_issued = j + 1;
+      };
+      auto issue_qk = [&](int j) {
+        const uint64_t dk = dk0 + (j & 1) * (kPieceBytes / 16);
 #pragma unroll
         for (int k = 0; k < kDim / 16; ++k)
-          mma_bf16_ss(tmem + qb * kHalf, dq + 2 * k, dk + 2 * k, id_qk, k > 0);
-        mma_commit(smem_u32(&bars->s_full[qb]));
-        mma_commit(smem_u32(&bars->k_empty[ks]));
-        if (++ks == kKStages) ks = 0, kph ^= 1;
-        if (++qb == kBufs) qb = 0;
-        return true;
+          mma_bf16_ss(tmem, dq + 2 * k, dk + 2 * k, id_qk, k > 0);
+        mma_commit(smem_u32(&bars->s_full));
       };
-      bool ok = mbar_wait(smem_u32(&bars->q_full), 0, abort, p.status, kStatusTimeoutMma);
-      for (int j = 0; ok && j < kBufs && j < steps; ++j) ok = issue_qk();
-      uint32_t pb = 0, pph = 0;
-      for (int j = 0; ok && j < steps; ++j) {
-        if (!mbar_wait(smem_u32(&bars->v_full[vs]), vph, abort, p.status, kStatusTimeoutMma))
-          break;
-        if (!mbar_wait(smem_u32(&bars->p_full[pb]), pph, abort, p.status, kStatusTimeoutMma))
-          break;
+      const uint32_t q_bar = smem_u32(&bars->q_full);
+      // keys of the steps ahead, read before they are needed
+      const int key0 = piece_key(p, list, 0);
+      int key1 = steps > 1 ? piece_key(p, list, 1) : 0;
+      int key2 = steps > 2 ? piece_key(p, list, 2) : 0;
+      mbar_arrive_expect_tx(q_bar, kTileBytes);
+      tma_load_5d(sQ, &tmap_q, q_bar, 0, tile * kTile, head, batch, 0);
+      load_k(0, key0);
+      load_v(0, key0);
+      if (steps > 1) {
+        load_k(1, key1);
+        load_v(1, key1);
+      }
+      bool ok = mbar_wait(q_bar, 0, abort, p.status, kStatusTimeoutMma) &&
+                mbar_wait(smem_u32(&bars->k_full[0]), 0, abort, p.status, kStatusTimeoutMma);
+      if (ok) {
         tc_fence_after();
-        const uint64_t dv = dv0 + vs * (kPieceBytes / 16);
+        issue_qk(0);
+      }
+      for (int j = 0; ok && j < steps; ++j) {
+        const bool more = j + 1 < steps;
+        const int key3 = j + 3 < steps ? piece_key(p, list, j + 3) : 0;
+        ok = mbar_wait(smem_u32(&bars->v_full[j & 1]), (j >> 1) & 1, abort, p.status,
+                       kStatusTimeoutMma) &&
+             (!more || mbar_wait(smem_u32(&bars->k_full[(j + 1) & 1]), ((j + 1) >> 1) & 1, abort,
+                                 p.status, kStatusTimeoutMma)) &&
+             mbar_wait(smem_u32(&bars->p_full), j & 1, abort, p.status, kStatusTimeoutMma);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t dv = dv0 + (j & 1) * (kPieceBytes / 16);
 #pragma unroll
         for (int k = 0; k < kHalf / 16; ++k)
-          mma_bf16_ts(tO, tmem + pb * kHalf + k * 8, dv + k * (2048 / 16), id_pv,
+          mma_bf16_ts(tO, tmem + k * 8, dv + k * (2048 / 16), id_pv,
                       (j > 0 || k > 0) ? 1u : 0u);
-        mma_commit(smem_u32(&bars->o_done[j & 1]));
-        mma_commit(smem_u32(&bars->v_empty[vs]));
-        if (++vs == kVStages) vs = 0, vph ^= 1;
-        if (++pb == kBufs) pb = 0, pph ^= 1;
-        if (j + kBufs < steps) ok = issue_qk();
+        if (more) issue_qk(j + 1);
+        if (j + 2 < steps) load_k(j + 2, key2);
+        if (j > 0 && more) load_v(j + 1, key1);
+        key1 = key2;
+        key2 = key3;
       }
-      // Every product completes before TMEM is released.
-      mma_commit(smem_u32(&bars->drain));
-      mbar_wait_drain(smem_u32(&bars->drain), 0);
+      // Every product completes before TMEM is released, and every load lands.
+      mma_commit(smem_u32(&bars->o_done));
+      mbar_wait_drain(smem_u32(&bars->o_done), 0);
+      if (*abort) {
+        mbar_wait_drain(q_bar, 0);
+        for (int d = max(0, k_issued - 2); d < k_issued; ++d)
+          mbar_wait_drain(smem_u32(&bars->k_full[d & 1]), (d >> 1) & 1);
+        for (int d = max(0, v_issued - 2); d < v_issued; ++d)
+          mbar_wait_drain(smem_u32(&bars->v_full[d & 1]), (d >> 1) & 1);
+      }
     }
   } else {
     // ------------------------------------------------------------- softmax
     const uint32_t lane_off = static_cast<uint32_t>(warp * 32) << 16;
-    const uint32_t tO = tmem + kBufs * kHalf + lane_off;
+    const uint32_t tS = tmem + lane_off, tO = tS + kHalf;
     const float c = p.scale_log2;
     float m_run = -CUDART_INF_F, l_run = 0.f;  // running maximum (log2 domain) and sum
     bool ok = true;
-    uint32_t buf = 0, sph = 0;
-    // Whole-warp wait for P V of step j (called for every j, in order: the next
-    // phase of that barrier needs a P that this warp has not handed over yet).
-    auto pv_done = [&](int j) {
-      return __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->o_done[j & 1]), (j >> 1) & 1, abort,
-                                               p.status, kStatusTimeoutSoftmax));
-    };
     for (int j = 0; j < steps; ++j) {
-      const int n = min(len - piece_key(p, list, j), kHalf);  // valid keys of the piece
-      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->s_full[buf]), sph, abort, p.status,
+      // Valid keys of the piece: the list ascends, so only the last block's
+      // pieces can be short.
+      int n = kHalf;
+      if (j + 2 >= steps) n = min(len - piece_key(p, list, j), kHalf);
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->s_full), j & 1, abort, p.status,
                                              kStatusTimeoutSoftmax))) {
         ok = false;
         break;
       }
       tc_fence_after();
-      const uint32_t tS = tmem + buf * kHalf + lane_off;
-      uint32_t sr[kHalf];
-      tmem_ld_wait_64(tS, sr);
-      if (n < kHalf) {
-#pragma unroll
-        for (int i = 0; i < kHalf; ++i)
-          if (i >= n) sr[i] = __float_as_uint(-CUDART_INF_F);
-      }
-      float mx0 = -CUDART_INF_F, mx1 = -CUDART_INF_F, mx2 = -CUDART_INF_F, mx3 = -CUDART_INF_F;
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        mx0 = fmax3(mx0, __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
-        mx1 = fmax3(mx1, __uint_as_float(sr[16 + i]), __uint_as_float(sr[17 + i]));
-        mx2 = fmax3(mx2, __uint_as_float(sr[32 + i]), __uint_as_float(sr[33 + i]));
-        mx3 = fmax3(mx3, __uint_as_float(sr[48 + i]), __uint_as_float(sr[49 + i]));
-      }
-      const float m_tile = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * c;
-      float m_new = m_run;
-      bool rescale = false;
-      if (m_tile > m_run + kRescale) {
-        m_new = m_tile;
-        rescale = j > 0;
-      }
-      // Followed at a distance of two steps, so that no phase is missed.
-      if (j > 1 && !pv_done(j - 2)) {
-        ok = false;
-        break;
-      }
-      if (__any_sync(0xffffffffu, rescale)) {
-        if (!pv_done(j - 1)) {  // O holds every product so far
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const float alpha = rescale ? ex2_approx(m_run - m_new) : 1.0f;
-        l_run *= alpha;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t o[32];
-          tmem_ld_wait_32(tO + h * 32, o);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-          tmem_st32(tO + h * 32, o);
-        }
-      }
-      m_run = m_new;
-      // A row that has met only -inf so far weighs those keys 0.
-      const float neg_m = m_new == -CUDART_INF_F ? 0.f : -m_new;
-      float sum0 = 0.f, sum1 = 0.f;
+      // P against the maximum so far, the step's own maximum taken along the way
+      // (the exponentials, not the comparisons, set the pace).  P is bounded by
+      // 2^kRescale as long as no row's maximum has grown by more; where one has
+      // (and in the first step) the step is done over: the scores are still there.
       uint32_t pk[32];
+      float sum, m_tile;
+      weigh<T>(tS, c, m_run, n, pk, sum, m_tile);
+      const bool raise = m_tile > m_run + kRescale;
+      if (__any_sync(0xffffffffu, raise)) {
+        const float m_new = raise ? m_tile : m_run;
+        if (j > 0) {  // O holds the products up to step j - 1
+          const float alpha = raise ? ex2_approx(m_run - m_new) : 1.0f;
+          l_run *= alpha;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        float x0, x1;
-        fma2(x0, x1, __uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1]), c, c, neg_m,
-             neg_m);
-        const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-        add2(sum0, sum1, sum0, sum1, p0, p1);
-        pk[i] = pack2<T>(p0, p1);
+          for (int h = 0; h < 4; ++h) {
+            uint32_t o[16];
+            tmem_ld_wait_16(tO + h * 16, o);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st16(tO + h * 16, o);
+          }
+        }
+        m_run = m_new;
+        weigh<T>(tS, c, m_run, n, pk, sum, m_tile);
       }
       tmem_st32(tS, pk);
-      l_run += sum0 + sum1;
+      l_run += sum;
       // Rows of V behind the sequence's end may hold anything (0 * NaN is NaN):
       // they are cleared before the product reads them.
       if (n < kHalf && len < p.kv_len) {
-        const int vs = j % kVStages;
-        if (!__all_sync(0xffffffffu,
-                        mbar_wait(smem_u32(&bars->v_full[vs]), (j / kVStages) & 1, abort, p.status,
-                                  kStatusTimeoutSoftmax))) {
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->v_full[j & 1]), (j >> 1) & 1, abort,
+                                               p.status, kStatusTimeoutSoftmax))) {
           ok = false;
           break;
         }
         if (row < kHalf && row >= n) {
-          uint4* v = reinterpret_cast<uint4*>(smem + kTileSmemV + vs * kPieceBytes + row * 128);
+          uint4* v =
+              reinterpret_cast<uint4*>(smem + kTileSmemV + (j & 1) * kPieceBytes + row * 128);
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
         }
@@ -717,23 +764,31 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       }
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(smem_u32(&bars->p_full[buf]));
-      if (++buf == kBufs) buf = 0, sph ^= 1;
+      __syncwarp();
+      if (elect_one()) mbar_arrive(smem_u32(&bars->p_full));
     }
-    if (ok && (steps < 2 || pv_done(steps - 2)) && pv_done(steps - 1)) {
+    if (ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->o_done), 0, abort, p.status,
+                                                kStatusTimeoutEpilogue))) {
       tc_fence_after();
-      uint32_t o[64];
-      tmem_ld_wait_64(tO, o);
-      if (tok < p.q_len) {
-        const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
+      if (__all_sync(0xffffffffu, *abort == 0)) {
+        uint4* dst = out_row();
+        // every score was -inf: weights of nothing
+        const float inv = m_run == -CUDART_INF_F && l_run == l_run ? 0.f : 1.0f / l_run;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint32_t w[4];
+        for (int h = 0; h < 2; ++h) {
+          uint32_t o[32];
+          tmem_ld_wait_32(tO + h * 32, o);
+          if (dst != nullptr) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            w[k] = pack2<T>(__uint_as_float(o[8 * i + 2 * k]) * inv,
-                            __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
-          reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int i = 0; i < 4; ++i) {
+              uint32_t w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                w[k] = pack2<T>(__uint_as_float(o[8 * i + 2 * k]) * inv,
+                                __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
+              dst[h * 4 + i] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
         }
       }
     }
@@ -743,7 +798,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   if (warp == 4) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem, 256);
+    tmem_dealloc(tmem, 2 * kHalf);
   }
 }
 
