@@ -99,42 +99,53 @@ struct PoolParams {
   double* out;         // [batch][heads][blocks][64]
 };
 
-// One warp sums one block of four heads: a lane eight channels, one 16-byte
-// load a token.
+// One CTA sums one block of four heads: a lane eight channels (16 bytes) of a
+// token, a warp every fourth token, the warps' sums added in order.  (One warp a
+// block took 31 us at 3 x 2005 tokens, where there are 144 of them.)
+constexpr int kPoolWarps = 4;
 template <typename T>
-__device__ __forceinline__ void pool_block(const PoolParams& p, long long item, int lane) {
+__device__ __forceinline__ void pool_block(const PoolParams& p, long long item,
+                                           double (*part)[32][8]) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hg = (p.heads + 3) / 4;
   const int h = static_cast<int>(item % hg) * 4 + lane / 8;
   const long long bn = item / hg;
   const int n = static_cast<int>(bn % p.blocks), b = static_cast<int>(bn / p.blocks);
-  if (h >= p.heads) return;
   const int len = key_length(p.lengths, b, p.len);
   const int t0 = n * p.block, t1 = min(t0 + p.block, len);
-  const T* src =
-      static_cast<const T*>(p.x) + b * p.st.batch + h * p.st.head + (lane & 7) * 8;
   double sum[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum[i] = 0.0;
-  constexpr int U = 8;
-  int t = t0;
-  for (; t + U <= t1; t += U) {
-    uint4 v[U];
+  if (h < p.heads) {
+    const T* src = static_cast<const T*>(p.x) + b * p.st.batch + h * p.st.head + (lane & 7) * 8;
+    constexpr int U = 8;  // tokens requested together
+    for (int t = t0 + warp; t < t1; t += U * kPoolWarps) {
+      uint4 v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const uint4*>(src + (t + u) * p.st.token);
+      for (int u = 0; u < U; ++u) {
+        const int tu = t + u * kPoolWarps;
+        v[u] = make_uint4(0u, 0u, 0u, 0u);  // adds zeros behind the end
+        if (tu < t1) v[u] = *reinterpret_cast<const uint4*>(src + tu * p.st.token);
+      }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float f[8];
-      unpack8<T>(v[u], f);
+      for (int u = 0; u < U; ++u) {
+        float f[8];
+        unpack8<T>(v[u], f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum[i] += static_cast<double>(f[i]);
+        for (int i = 0; i < 8; ++i) sum[i] += static_cast<double>(f[i]);
+      }
     }
   }
-  for (; t < t1; ++t) {
-    float f[8];
-    unpack8<T>(*reinterpret_cast<const uint4*>(src + t * p.st.token), f);
+  if (warp > 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum[i] += static_cast<double>(f[i]);
+    for (int i = 0; i < 8; ++i) part[warp - 1][lane][i] = sum[i];
   }
+  __syncthreads();
+  if (warp > 0 || h >= p.heads) return;
+#pragma unroll
+  for (int w = 0; w < kPoolWarps - 1; ++w)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] += part[w][lane][i];
   if (p.mean && t1 > t0) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum[i] /= static_cast<double>(t1 - t0);
@@ -145,75 +156,85 @@ __device__ __forceinline__ void pool_block(const PoolParams& p, long long item, 
   for (int i = 0; i < 4; ++i) dst[i] = make_double2(sum[2 * i], sum[2 * i + 1]);
 }
 
-constexpr int kPoolWarps = 4;
 template <typename T>
 __global__ void __launch_bounds__(32 * kPoolWarps)
-    pool_kernel(const PoolParams a, const PoolParams b, long long items_a, long long items) {
-  const long long item = static_cast<long long>(blockIdx.x) * kPoolWarps + (threadIdx.x >> 5);
-  if (item >= items) return;
+    pool_kernel(const PoolParams a, const PoolParams b, long long items_a) {
+  __shared__ double part[kPoolWarps - 1][32][8];
+  const long long item = blockIdx.x;
   if (item < items_a)
-    pool_block<T>(a, item, threadIdx.x & 31);
+    pool_block<T>(a, item, part);
   else
-    pool_block<T>(b, item - items_a, threadIdx.x & 31);
+    pool_block<T>(b, item - items_a, part);
 }
 
 // ------------------------------------------------------------------- scores
-// scores[b][h][g][n] = q_sum[b][h][g] . k_mean[b][h / per][n], 64 x 64 a CTA,
-// 4 x 4 a thread.  0.5 G N d FP64 products; a small part of the attention.
-constexpr int kScoreTile = 64;
-constexpr int kScoreSmem = 2 * kDim * kScoreTile * 8;
-__global__ void __launch_bounds__(256)
+// scores[b][h][g][n] = q_sum[b][h][g] . k_mean[b][h / per][n] on the FP64 matrix
+// instruction (m8n8k4): 64 x 64 a CTA, 32 x 32 a warp.  Rows are padded to 68
+// doubles, so the fragments' reads meet no bank twice.
+constexpr int kScoreTile = 64, kScorePitch = kDim + 4;
+constexpr int kScoreSmem = 2 * kScoreTile * kScorePitch * 8;
+
+__device__ __forceinline__ void mma_f64(double (&d)[2], double a, double b) {
+  asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};"
+               : "+d"(d[0]), "+d"(d[1])
+               : "d"(a), "d"(b));
+}
+
+__global__ void __launch_bounds__(128)
     score_kernel(const double* q_sum, const double* k_mean, double* scores, int heads, int per,
                  int groups, int blocks) {
-  extern __shared__ double tiles[];  // [64 d][64 groups], [64 d][64 blocks]
+  extern __shared__ double tiles[];  // [64 groups][68], [64 blocks][68]
   double* sq = tiles;
-  double* sk = tiles + kDim * kScoreTile;
+  double* sk = tiles + kScoreTile * kScorePitch;
   const int n0 = blockIdx.x * kScoreTile, g0 = blockIdx.y * kScoreTile;
   const int bh = blockIdx.z;
   const int b = bh / heads, h = bh - b * heads;
   const long long kv = static_cast<long long>(b) * (heads / per) + h / per;
-  // 4 threads a row, 16 doubles each; a warp's stores fall on 8 rows of 4 columns
-  const int r = threadIdx.x / 4, c = threadIdx.x % 4 * 16;
-#pragma unroll
-  for (int i = 0; i < 16; i += 2) {
-    double2 a = make_double2(0.0, 0.0), k = make_double2(0.0, 0.0);
+  const double* qg = q_sum + static_cast<long long>(bh) * groups * kDim;
+  const double* kg = k_mean + kv * blocks * kDim;
+  for (int i = threadIdx.x; i < kScoreTile * kDim / 2; i += 128) {
+    const int r = i / (kDim / 2), c = i % (kDim / 2) * 2;
+    double2 q = make_double2(0.0, 0.0), k = make_double2(0.0, 0.0);
     if (g0 + r < groups)
-      a = *reinterpret_cast<const double2*>(
-          q_sum + (static_cast<long long>(bh) * groups + g0 + r) * kDim + c + i);
+      q = *reinterpret_cast<const double2*>(qg + (g0 + r) * static_cast<long long>(kDim) + c);
     if (n0 + r < blocks)
-      k = *reinterpret_cast<const double2*>(k_mean + (kv * blocks + n0 + r) * kDim + c + i);
-    sq[(c + i) * kScoreTile + r] = a.x;
-    sq[(c + i + 1) * kScoreTile + r] = a.y;
-    sk[(c + i) * kScoreTile + r] = k.x;
-    sk[(c + i + 1) * kScoreTile + r] = k.y;
+      k = *reinterpret_cast<const double2*>(kg + (n0 + r) * static_cast<long long>(kDim) + c);
+    *reinterpret_cast<double2*>(sq + r * kScorePitch + c) = q;
+    *reinterpret_cast<double2*>(sk + r * kScorePitch + c) = k;
   }
   __syncthreads();
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  double acc[4][4];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int wm = (warp & 1) * 32, wn = (warp >> 1) * 32;
+  double acc[4][4][2];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.0;
+    for (int j = 0; j < 4; ++j) acc[i][j][0] = acc[i][j][1] = 0.0;
+  const double* qa = sq + (wm + lane / 4) * kScorePitch + lane % 4;
+  const double* kb = sk + (wn + lane / 4) * kScorePitch + lane % 4;
 #pragma unroll 4
-  for (int d = 0; d < kDim; ++d) {
-    const double2* qa = reinterpret_cast<const double2*>(sq + d * kScoreTile + ty * 4);
-    const double2* ka = reinterpret_cast<const double2*>(sk + d * kScoreTile + tx * 4);
-    const double2 q01 = qa[0], q23 = qa[1], k01 = ka[0], k23 = ka[1];
-    const double qv[4] = {q01.x, q01.y, q23.x, q23.y}, kv4[4] = {k01.x, k01.y, k23.x, k23.y};
+  for (int d = 0; d < kDim; d += 4) {
+    double a[4], k[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = qa[i * 8 * kScorePitch + d];
+      k[i] = kb[i * 8 * kScorePitch + d];
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = fma(qv[i], kv4[j], acc[i][j]);
+      for (int j = 0; j < 4; ++j) mma_f64(acc[i][j], a[i], k[j]);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int g = g0 + ty * 4 + i;
+    const int g = g0 + wm + i * 8 + lane / 4;
     if (g >= groups) continue;
     double* dst = scores + (static_cast<long long>(bh) * groups + g) * blocks;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int n = n0 + tx * 4 + j;
-      if (n < blocks) dst[n] = acc[i][j];
+      const int n = n0 + wn + j * 8 + lane % 4 * 2;
+      if (n < blocks) dst[n] = acc[i][j][0];
+      if (n + 1 < blocks) dst[n + 1] = acc[i][j][1];
     }
   }
 }
@@ -264,7 +285,29 @@ __device__ __forceinline__ void select_topk(Key key, int n, int take, int topk, 
   uint32_t t = 0;
   bool exact = take >= n;  // everything is taken
   if (!exact) {
-    for (int bit = 31; bit >= 0; --bit) {
+    // bits that all upper words share need no step
+    uint32_t most = 0, least = 0xffffffffu;
+    if (kPer > 0) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        most = max(most, hi[j]);
+        if (j * 32 + lane < n) least = min(least, hi[j]);
+      }
+    } else {
+      for (int j = 0; j < rounds; ++j) {
+        const int i = j * 32 + lane;
+        if (i < n) {
+          const uint32_t w = static_cast<uint32_t>(key(i) >> 32);
+          most = max(most, w);
+          least = min(least, w);
+        }
+      }
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    least = __reduce_min_sync(0xffffffffu, least);
+    const int top = 31 - __clz(most ^ least);  // -1: they are all equal
+    t = top < 0 ? most : top == 31 ? 0u : most >> (top + 1) << (top + 1);
+    for (int bit = top; bit >= 0; --bit) {
       const uint32_t up = t | (1u << bit);
       const int c = at_least(up);
       if (c >= take) {
@@ -300,6 +343,20 @@ __device__ __forceinline__ void select_topk(Key key, int n, int take, int topk, 
     }
     ties = want - (low == 0xffffffffu ? 0 : low_at_least(low + 1));
   }
+  const uint32_t before = (1u << lane) - 1;
+  if (kPer > 0 && exact) {
+    int count = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int i = j * 32 + lane;
+      const bool yes = i < n && (take >= n || hi[j] >= t);
+      const uint32_t mask = __ballot_sync(0xffffffffu, yes);
+      if (yes) out[count + __popc(mask & before)] = i;
+      count += __popc(mask);
+    }
+    for (int i = take + lane; i < topk; i += 32) out[i] = -1;
+    return;
+  }
   int count = 0, tied = 0;
   const unsigned long long bound = (static_cast<unsigned long long>(t) << 32) | low;
   for (int j = 0; j < rounds; ++j) {
@@ -317,7 +374,6 @@ __device__ __forceinline__ void select_topk(Key key, int n, int take, int topk, 
       }
     }
     const uint32_t tie_mask = __ballot_sync(0xffffffffu, tie);
-    const uint32_t before = (1u << lane) - 1;
     if (tie && tied + __popc(tie_mask & before) < ties) yes = true;
     tied += __popc(tie_mask);
     const uint32_t mask = __ballot_sync(0xffffffffu, yes);
@@ -339,77 +395,6 @@ __global__ void __launch_bounds__(32 * kSelectWarps)
   const double* s = scores + row * blocks;
   select_topk<kPer>([&](int i) { return score_key(s[i]); }, n, min(topk, n), topk,
                     selection + row * topk, threadIdx.x & 31);
-}
-
-// Single queries: one CTA scores every block of a row (8 lanes a block, eight
-// channels each), and its first warp selects.
-struct RowSelectParams {
-  const void* q;
-  Strides q_st;
-  const double* k_mean;
-  const int* lengths;
-  int heads, per, q_len, kv_len, key_block, blocks, topk;
-  int* selection;
-};
-
-constexpr int kRowSelectWarps = 8;
-template <typename T>
-__global__ void __launch_bounds__(32 * kRowSelectWarps) row_select_kernel(const RowSelectParams p) {
-  extern __shared__ unsigned long long keys[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long row = blockIdx.x;  // (batch, head, query)
-  const int qi = static_cast<int>(row % p.q_len);
-  const int bh = static_cast<int>(row / p.q_len);
-  const int b = bh / p.heads, h = bh - b * p.heads;
-  const int len = key_length(p.lengths, b, p.kv_len);
-  const int n = (len + p.key_block - 1) / p.key_block;
-  const int take = min(p.topk, n);
-  int* out = p.selection + row * p.topk;
-  if (take < n) {
-    const T* q = static_cast<const T*>(p.q) + b * p.q_st.batch + h * p.q_st.head +
-                 qi * p.q_st.token + (lane & 7) * 8;
-    float f[8];
-    unpack8<T>(*reinterpret_cast<const uint4*>(q), f);
-    double qd[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) qd[i] = static_cast<double>(f[i]);
-    const double* mean =
-        p.k_mean +
-        (static_cast<long long>(b) * (p.heads / p.per) + h / p.per) * p.blocks * kDim +
-        (lane & 7) * 8;
-    constexpr int U = 4;  // blocks of a lane group requested together
-    for (int i0 = warp * 4; i0 < n; i0 += kRowSelectWarps * 4 * U) {
-      double2 v[U][4];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * kRowSelectWarps * 4 + lane / 8;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          v[u][j] = i < n ? *reinterpret_cast<const double2*>(mean + i * static_cast<long long>(kDim) + 2 * j)
-                          : make_double2(0.0, 0.0);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * kRowSelectWarps * 4 + lane / 8;
-        double s = 0.0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s = fma(qd[2 * j], v[u][j].x, s);
-          s = fma(qd[2 * j + 1], v[u][j].y, s);
-        }
-#pragma unroll
-        for (int d = 1; d < 8; d <<= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        if ((lane & 7) == 0 && i < n) keys[i] = score_key(s);
-      }
-    }
-  }
-  __syncthreads();
-  if (warp != 0) return;
-  auto key = [&](int i) { return keys[i]; };
-  if (n <= 32 * 16)
-    select_topk<16>(key, n, take, p.topk, out, lane);
-  else
-    select_topk<0>(key, n, take, p.topk, out, lane);
 }
 
 // -------------------------------------------------- attention of 128-row tiles
@@ -802,12 +787,14 @@ __global__ void __launch_bounds__(kTileThreads, 4)
   }
 }
 
-// ------------------------------------------------- attention of single queries
-// Eight lanes share a key (16 bytes each of its K and V rows); a lane group
-// takes eight neighbouring keys at a time, with its own running maximum and
-// sum, and the groups, warps and CTAs of a row are merged at the end, in a
-// fixed order.  Bound by the chosen blocks' bytes: 16 loads of 16 bytes a lane
-// are in flight.
+// -------------------------------------------------------------- single queries
+// A row (batch, head, query) is the work of a cluster of 1 to 8 CTAs, in one
+// launch.  Its CTAs share the blocks' scores (eight lanes a block, eight channels
+// each, FP64) and write each score's key into every CTA's shared memory; each
+// finds the choice by itself and attends its part of it: eight lanes a key (16
+// bytes each of its K and V rows), eight neighbouring keys a lane group at a
+// time, with running maximum and sum.  Groups, warps and CTAs are merged in a
+// fixed order.  Bound by the bytes of the means and the chosen blocks.
 constexpr int kRowWarps = 8;
 constexpr int kRowKeys = 8;
 constexpr int kMaxSplits = 8;
@@ -817,22 +804,29 @@ struct RowParams {
   Strides q_st, k_st, v_st, o_st;
   void* out;
   const int* lengths;
-  const int* selection;
-  int heads, per, q_len, kv_len, key_block, topk, splits;
+  const double* k_mean;
+  int* selection;
+  int heads, per, q_len, kv_len, key_block, blocks, topk, splits;
   float scale_log2;
 };
 
-__device__ __forceinline__ float ld_cluster_f32(const float* p, uint32_t rank) {
+__device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
   uint32_t at;
-  float v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return at;
+}
+__device__ __forceinline__ float ld_cluster_f32(const float* p, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_rank(p, rank)) : "memory");
   return v;
 }
-__device__ __forceinline__ void cluster_sync() {
+__device__ __forceinline__ void cluster_arrive() {
   __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
-                   : "memory");
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // Weight that a part with maximum m has under the common maximum `top`.
@@ -841,9 +835,11 @@ __device__ __forceinline__ float part_weight(float m, float top) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(32 * kRowWarps, 2) row_attn_kernel(const RowParams p) {
+__global__ void __launch_bounds__(32 * kRowWarps, 2) row_kernel(const RowParams p) {
   __shared__ float part_m[kRowWarps], part_l[kRowWarps], part_o[kRowWarps][kDim];
   __shared__ float cta[kDim + 2];  // this CTA's O, maximum, sum
+  extern __shared__ unsigned long long keys[];  // [blocks], then the choice
+  int* list = reinterpret_cast<int*>(keys + p.blocks);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = static_cast<int>(blockIdx.x % p.splits);  // also the rank in the cluster
   const long long row = blockIdx.x / p.splits;                // (batch, head, query)
@@ -851,12 +847,8 @@ __global__ void __launch_bounds__(32 * kRowWarps, 2) row_attn_kernel(const RowPa
   const int bh = static_cast<int>(row / p.q_len);
   const int b = bh / p.heads, h = bh - b * p.heads;
   const int len = key_length(p.lengths, b, p.kv_len);
-  const int kept = min(p.topk, (len + p.key_block - 1) / p.key_block);
-  const int shift = p.key_block >> 7;
-  const int pieces = kept << shift;
-  const int lo = static_cast<int>(static_cast<long long>(pieces) * split / p.splits);
-  const int hi = static_cast<int>(static_cast<long long>(pieces) * (split + 1) / p.splits);
-  const int* list = p.selection + row * p.topk;
+  const int n = (len + p.key_block - 1) / p.key_block;
+  const int take = min(p.topk, n);
   const int group = lane >> 3, c8 = (lane & 7) * 8;
   float q[8];
   {
@@ -864,6 +856,76 @@ __global__ void __launch_bounds__(32 * kRowWarps, 2) row_attn_kernel(const RowPa
                    qi * p.q_st.token + c8;
     unpack8<T>(*reinterpret_cast<const uint4*>(src), q);
   }
+  // ---------------------------------------------------------------- scores
+  // No CTA's shared memory is written before it has started.
+  if (p.splits > 1) {
+    cluster_arrive();
+    cluster_wait();
+  }
+  if (take < n) {
+    double qd[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) qd[i] = static_cast<double>(q[i]);
+    const double* mean =
+        p.k_mean +
+        (static_cast<long long>(b) * (p.heads / p.per) + h / p.per) * p.blocks * kDim + c8;
+    const int stride = p.splits * kRowWarps * 4;
+    constexpr int U = 4;  // blocks of a lane group requested together
+    for (int i0 = (split * kRowWarps + warp) * 4; i0 < n; i0 += stride * U) {
+      double2 v[U][4];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * stride + group;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          v[u][j] = i < n ? *reinterpret_cast<const double2*>(
+                                mean + i * static_cast<long long>(kDim) + 2 * j)
+                          : make_double2(0.0, 0.0);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * stride + group;
+        double s = 0.0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s = fma(qd[2 * j], v[u][j].x, s);
+          s = fma(qd[2 * j + 1], v[u][j].y, s);
+        }
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        // lane r of the group writes into CTA r
+        if ((lane & 7) < p.splits && i < n)
+          asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(map_rank(keys + i, lane & 7)),
+                       "l"(score_key(s))
+                       : "memory");
+      }
+    }
+  }
+  if (p.splits > 1) {
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
+  // ---------------------------------------------------------------- choice
+  if (warp == 0) {
+    auto key = [&](int i) { return keys[i]; };
+    if (n <= 32 * 16)
+      select_topk<16>(key, n, take, take, list, lane);
+    else
+      select_topk<0>(key, n, take, take, list, lane);
+    __syncwarp();
+    if (split == 0) {
+      int* out = p.selection + row * p.topk;
+      for (int i = lane; i < p.topk; i += 32) out[i] = i < take ? list[i] : -1;
+    }
+  }
+  __syncthreads();
+  // ------------------------------------------------------------- attention
+  const int shift = p.key_block >> 7;
+  const int pieces = take << shift;
+  const int lo = static_cast<int>(static_cast<long long>(pieces) * split / p.splits);
+  const int hi = static_cast<int>(static_cast<long long>(pieces) * (split + 1) / p.splits);
   const T* kp = static_cast<const T*>(p.k) + b * p.k_st.batch + h / p.per * p.k_st.head + c8;
   const T* vp = static_cast<const T*>(p.v) + b * p.v_st.batch + h / p.per * p.v_st.head + c8;
   float m = -CUDART_INF_F, l = 0.f, o[8];
@@ -871,8 +933,8 @@ __global__ void __launch_bounds__(32 * kRowWarps, 2) row_attn_kernel(const RowPa
   for (int i = 0; i < 8; ++i) o[i] = 0.f;
   // units of 32 keys: half a 64-key piece, eight keys a lane group
   for (int u = 2 * lo + warp; u < 2 * hi; u += kRowWarps) {
-    const int first = __ldg(list + ((u >> 1) >> shift)) * p.key_block +
-                      ((u >> 1) & shift) * kHalf + (u & 1) * 32 + group * kRowKeys;
+    const int first = list[(u >> 1) >> shift] * p.key_block + ((u >> 1) & shift) * kHalf +
+                      (u & 1) * 32 + group * kRowKeys;
     uint4 kv[kRowKeys], vv[kRowKeys];
 #pragma unroll
     for (int i = 0; i < kRowKeys; ++i) {
@@ -910,6 +972,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 2) row_attn_kernel(const RowPa
     }
     m = top;
   }
+  // ----------------------------------------------------------------- merge
   // the four lane groups of the warp
 #pragma unroll
   for (int x = 8; x < 32; x <<= 1) {
@@ -948,7 +1011,8 @@ __global__ void __launch_bounds__(32 * kRowWarps, 2) row_attn_kernel(const RowPa
       cta[kDim] = top;
       cta[kDim + 1] = lm;
     }
-    cluster_sync();
+    cluster_arrive();
+    cluster_wait();
     if (split == 0 && d < kDim) {
       float ms[kMaxSplits], ls[kMaxSplits], os[kMaxSplits];
 #pragma unroll
@@ -973,7 +1037,8 @@ __global__ void __launch_bounds__(32 * kRowWarps, 2) row_attn_kernel(const RowPa
         }
       }
     }
-    cluster_sync();  // the others' sums have been read
+    cluster_arrive();  // the others' sums have been read
+    cluster_wait();
   }
   if (split == 0 && d < kDim) {
     const float y = lm == 0.f ? 0.f : om / lm;
@@ -1029,11 +1094,10 @@ template <typename T>
 int launch_pool(const PoolParams* a, const PoolParams* b, int batch, cudaStream_t st) {
   const long long items_a = a == nullptr ? 0 : pool_items(*a, batch);
   const long long items = items_a + (b == nullptr ? 0 : pool_items(*b, batch));
-  const long long ctas = (items + kPoolWarps - 1) / kPoolWarps;
-  if (ctas > 0x7fffffffLL) return kErrTooLarge;
+  if (items > 0x7fffffffLL) return kErrTooLarge;
   const PoolParams none = {};
-  pool_kernel<T><<<static_cast<unsigned>(ctas), 32 * kPoolWarps, 0, st>>>(
-      a == nullptr ? none : *a, b == nullptr ? none : *b, items_a, items);
+  pool_kernel<T><<<static_cast<unsigned>(items), 32 * kPoolWarps, 0, st>>>(
+      a == nullptr ? none : *a, b == nullptr ? none : *b, items_a);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -1078,7 +1142,7 @@ int run(const Call& c, cudaStream_t st) {
     if (e != cudaSuccess) return static_cast<int>(e);
     const dim3 grid((blocks + kScoreTile - 1) / kScoreTile, (groups + kScoreTile - 1) / kScoreTile,
                     static_cast<unsigned>(c.batch * c.q_heads));
-    score_kernel<<<grid, 256, kScoreSmem, st>>>(q_sum, pool, scores, c.q_heads, per, groups,
+    score_kernel<<<grid, 128, kScoreSmem, st>>>(q_sum, pool, scores, c.q_heads, per, groups,
                                                 blocks);
     if ((e = cudaGetLastError()) != cudaSuccess) return static_cast<int>(e);
     const long long per_batch = static_cast<long long>(c.q_heads) * groups;
@@ -1106,29 +1170,25 @@ int run(const Call& c, cudaStream_t st) {
   }
 
   const long long rows = static_cast<long long>(c.batch) * c.q_heads * c.q_len;
-  const int key_bytes = blocks * 8;
-  cudaError_t e;
-  if (key_bytes > 48 * 1024) {
-    e = cudaFuncSetAttribute(row_select_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             key_bytes);
+  const int most = c.topk < blocks ? c.topk : blocks;  // chosen blocks of a row
+  const int smem = blocks * 8 + most * 4;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(
+        row_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return static_cast<int>(e);
   }
-  const RowSelectParams sp = {c.q, c.q_st, pool, c.lengths, c.q_heads, per, c.q_len, c.kv_len,
-                              c.key_block, blocks, c.topk, c.selection};
-  row_select_kernel<T>
-      <<<static_cast<unsigned>(rows), 32 * kRowSelectWarps, key_bytes, st>>>(sp);
-  if ((e = cudaGetLastError()) != cudaSuccess) return static_cast<int>(e);
-  RowParams p = {c.q, c.k, c.v, c.q_st, c.k_st, c.v_st, c.o_st, c.out, c.lengths, c.selection,
-                 c.q_heads, per, c.q_len, c.kv_len, c.key_block, c.topk, 1, scale_log2};
-  // Parts of a row: as many CTAs as two a multiprocessor hold, each with four
-  // 64-key pieces at least.
-  const long long most = static_cast<long long>(c.topk < blocks ? c.topk : blocks)
-                         << (c.key_block >> 7);
-  while (p.splits < kMaxSplits && rows * p.splits * 2 <= 2 * 148 * 2 && most / (p.splits * 2) >= 4)
+  RowParams p = {c.q, c.k, c.v, c.q_st, c.k_st, c.v_st, c.o_st, c.out, c.lengths, pool,
+                 c.selection, c.q_heads, per, c.q_len, c.kv_len, c.key_block, blocks, c.topk, 1,
+                 scale_log2};
+  // As many CTAs as two a multiprocessor hold at once, each with two 64-key pieces
+  // at least.
+  const long long pieces = static_cast<long long>(most) << (c.key_block >> 7);
+  while (p.splits < kMaxSplits && rows * p.splits * 2 <= 2 * 148 && pieces >= p.splits * 4)
     p.splits *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * p.splits));
   cfg.blockDim = dim3(32 * kRowWarps);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -1136,7 +1196,7 @@ int run(const Call& c, cudaStream_t st) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, row_attn_kernel<T>, p));
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, row_kernel<T>, p));
 }
 
 }  // namespace btk
@@ -1200,7 +1260,7 @@ extern "C" int erd_block_topk_attn(
       btk::workspace_sizes(batch, q_heads, kv_heads, q_len, kv_len, query_block, key_block,
                            key_means != nullptr);
   const long long rows = static_cast<long long>(batch) * q_heads * sz.groups;
-  if (rows > (1LL << 27) || (query_block == 1 && sz.blocks * 8 > 227 * 1024) ||
+  if (rows > (1LL << 27) || (query_block == 1 && sz.blocks * 12 > 220 * 1024) ||
       (sz.groups + 63) / 64 > 65535)
     return kErrTooLarge;
   if (sz.total > 0 && workspace == nullptr) return kErrNullPointer;

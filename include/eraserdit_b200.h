@@ -488,7 +488,7 @@ int erd_linear_act(int dtype, const void* x, int64_t ldx, const void* weight, in
  * [q_heads][ceil(q_len / query_block)][topk], receives the chosen blocks in
  * ascending order, then -1.  `workspace` (16-byte aligned) holds at least
  * erd_block_topk_workspace_bytes(...) bytes.  batch * q_heads is at most 65535;
- * query_block 1 takes at most 29056 key blocks.
+ * query_block 1 takes at most 18773 key blocks.
  */
 size_t erd_block_topk_workspace_bytes(int batch, int q_heads, int kv_heads, int q_len, int kv_len,
                                       int query_block, int key_block, int has_pool);

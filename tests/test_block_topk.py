@@ -47,7 +47,7 @@ def test_entries_reject_bad_arguments_before_any_device_call():
     for kw in (dict(q=p + 8), dict(v=p + 2), dict(out=p + 8), dict(qt=60), dict(ot=65), dict(means=p + 8),
                dict(lengths=p + 2), dict(sel=p + 1)):
         assert call(**kw) == -3, kw
-    for kw in (dict(batch=300, heads=300, nbytes=1 << 40), dict(kv_len=64 * 29057, nbytes=1 << 40),
+    for kw in (dict(batch=300, heads=300, nbytes=1 << 40), dict(kv_len=64 * 18774, nbytes=1 << 40),
                dict(q_len=1 << 28, nbytes=1 << 60)):
         assert call(**kw) == -6, kw
 
