@@ -113,7 +113,7 @@ def block_topk_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Te
         raise ValueError("query heads must be a positive multiple of the key heads")
     if query_block not in QUERY_BLOCKS or key_block not in KEY_BLOCKS:
         raise ValueError(f"query_block must be one of {QUERY_BLOCKS}, key_block of {KEY_BLOCKS}")
-    if not isinstance(topk, int) or topk < 1:
+    if not isinstance(topk, int) or not 1 <= topk < 2 ** 31:
         raise ValueError("topk must be a positive int")
     if not 0.0 < softmax_scale < float("inf"):
         raise ValueError("softmax_scale must be positive and finite")
@@ -125,10 +125,10 @@ def block_topk_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Te
     device, dtype = query.device, query.dtype
     groups = -(-q_len // query_block)
     if out is None:
-        out = query.new_empty(query.shape)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
     elif out.shape != query.shape or out.dtype != query.dtype or out.device != query.device:
         raise ValueError("out must have the query's shape, type and device")
-    selection = torch.empty(batch, heads, groups, topk, dtype=torch.int32, device=query.device)
+    selection = query.new_empty((batch, heads, groups, topk), dtype=torch.int32)
     if batch and q_len and kv_len:
         nbytes = 0
         workspace = None
@@ -138,14 +138,14 @@ def block_topk_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Te
                 int(key_pool is not None)))
             # from torch's allocator, call by call: it follows streams and captures
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
-        _native.call(
-            "erd_block_topk_attn", device, _native.DTYPE_CODES[dtype],
-            query.data_ptr(), key.data_ptr(), value.data_ptr(), *_strides("query", query),
-            *_strides("key", key), *_strides("value", value), batch, heads, kv_heads, q_len,
-            kv_len, HEAD_DIM, _native.ptr(key_lengths), _native.ptr(key_pool), topk, query_block,
-            key_block, float(softmax_scale), out.data_ptr(), *_strides("out", out),
-            selection.data_ptr(), _native.ptr(workspace), nbytes,
-            _native.status_pointer(device))
+        _native.call("erd_block_topk_attn", device, _native.pack(
+            "erd_block_topk_attn", query.data_ptr(), key.data_ptr(), value.data_ptr(),
+            0 if key_lengths is None else key_lengths.data_ptr(),
+            0 if key_pool is None else key_pool.data_ptr(), out.data_ptr(), selection.data_ptr(),
+            0 if workspace is None else workspace.data_ptr(), *_strides("query", query),
+            *_strides("key", key), *_strides("value", value), *_strides("out", out), nbytes,
+            _native.DTYPE_CODES[dtype], batch, heads, kv_heads, q_len, kv_len, HEAD_DIM, topk,
+            query_block, key_block, softmax_scale), _native.status_pointer(device))
     elif batch and q_len:  # no keys at all
         out.zero_()
         selection.fill_(-1)

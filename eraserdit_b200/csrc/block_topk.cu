@@ -1236,64 +1236,64 @@ extern "C" int erd_block_key_means(int dtype, const void* k, int64_t k_token_str
                            : btk::launch_pool<__half>(&p, nullptr, batch, s);
 }
 
-extern "C" int erd_block_topk_attn(
-    int dtype, const void* q, const void* k, const void* v, int64_t q_token_stride,
-    int64_t q_head_stride, int64_t q_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
-    int64_t k_batch_stride, int64_t v_token_stride, int64_t v_head_stride, int64_t v_batch_stride,
-    int batch, int q_heads, int kv_heads, int q_len, int kv_len, int head_dim,
-    const int32_t* key_lengths, const double* key_means, int topk, int query_block, int key_block,
-    float softmax_scale, void* out, int64_t o_token_stride, int64_t o_head_stride,
-    int64_t o_batch_stride, int32_t* selection, void* workspace, size_t workspace_bytes,
-    int* status, void* stream) {
-  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || selection == nullptr)
+extern "C" int erd_block_topk_attn(const erd_block_topk_args* args, int* status, void* stream) {
+  if (args == nullptr) return kErrNullPointer;
+  const erd_block_topk_args& a = *args;
+  if (a.struct_bytes != static_cast<int64_t>(sizeof(a))) return kErrBadShape;
+  if (a.q == nullptr || a.k == nullptr || a.v == nullptr || a.out == nullptr ||
+      a.selection == nullptr)
     return kErrNullPointer;
-  if ((dtype != ERD_BF16 && dtype != ERD_FP16) || head_dim != btk::kDim || batch <= 0 ||
-      q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || q_len <= 0 || kv_len <= 0 ||
-      topk <= 0 || (query_block != 1 && query_block != btk::kTile) ||
-      (key_block != 64 && key_block != 128) ||
-      !(softmax_scale > 0.f && softmax_scale <= 3.0e38f))
+  if ((a.dtype != ERD_BF16 && a.dtype != ERD_FP16) || a.head_dim != btk::kDim || a.batch <= 0 ||
+      a.q_heads <= 0 || a.kv_heads <= 0 || a.q_heads % a.kv_heads != 0 || a.q_len <= 0 ||
+      a.kv_len <= 0 || a.topk <= 0 || (a.query_block != 1 && a.query_block != btk::kTile) ||
+      (a.key_block != 64 && a.key_block != 128) ||
+      !(a.softmax_scale > 0.f && a.softmax_scale <= 3.0e38f))
     return kErrBadShape;
-  if (batch > 65535 || q_heads > 65535 || static_cast<long long>(batch) * q_heads > 65535 ||
-      kv_len > 0x7fff0000 || q_len > 0x7fff0000)
+  if (a.batch > 65535 || a.q_heads > 65535 ||
+      static_cast<long long>(a.batch) * a.q_heads > 65535 || a.kv_len > 0x7fff0000 ||
+      a.q_len > 0x7fff0000)
     return kErrTooLarge;
   const btk::Sizes sz =
-      btk::workspace_sizes(batch, q_heads, kv_heads, q_len, kv_len, query_block, key_block,
-                           key_means != nullptr);
-  const long long rows = static_cast<long long>(batch) * q_heads * sz.groups;
-  if (rows > (1LL << 27) || (query_block == 1 && sz.blocks * 12 > 220 * 1024) ||
+      btk::workspace_sizes(a.batch, a.q_heads, a.kv_heads, a.q_len, a.kv_len, a.query_block,
+                           a.key_block, a.key_means != nullptr);
+  const long long rows = static_cast<long long>(a.batch) * a.q_heads * sz.groups;
+  if (rows > (1LL << 27) || (a.query_block == 1 && sz.blocks * 12 > 220 * 1024) ||
       (sz.groups + 63) / 64 > 65535)
     return kErrTooLarge;
-  if (sz.total > 0 && workspace == nullptr) return kErrNullPointer;
-  if (workspace_bytes < sz.total) return kErrBadShape;
+  if (sz.total > 0 && a.workspace == nullptr) return kErrNullPointer;
+  if (a.workspace_bytes < 0 || static_cast<size_t>(a.workspace_bytes) < sz.total)
+    return kErrBadShape;
   btk::Call c = {};
-  c.q = q;
-  c.k = k;
-  c.v = v;
-  c.q_st = {q_token_stride, q_head_stride, q_batch_stride};
-  c.k_st = {k_token_stride, k_head_stride, k_batch_stride};
-  c.v_st = {v_token_stride, v_head_stride, v_batch_stride};
-  c.o_st = {o_token_stride, o_head_stride, o_batch_stride};
-  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) ||
-      !aligned16(workspace) || !aligned16(key_means) || !btk::strides_ok(c.q_st) ||
+  c.q = a.q;
+  c.k = a.k;
+  c.v = a.v;
+  c.q_st = {a.q_stride[0], a.q_stride[1], a.q_stride[2]};
+  c.k_st = {a.k_stride[0], a.k_stride[1], a.k_stride[2]};
+  c.v_st = {a.v_stride[0], a.v_stride[1], a.v_stride[2]};
+  c.o_st = {a.out_stride[0], a.out_stride[1], a.out_stride[2]};
+  if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.out) ||
+      !aligned16(a.workspace) || !aligned16(a.key_means) || !btk::strides_ok(c.q_st) ||
       !btk::strides_ok(c.k_st) || !btk::strides_ok(c.v_st) || !btk::strides_ok(c.o_st) ||
-      ((reinterpret_cast<uintptr_t>(key_lengths) | reinterpret_cast<uintptr_t>(selection)) & 3) != 0)
+      ((reinterpret_cast<uintptr_t>(a.key_lengths) | reinterpret_cast<uintptr_t>(a.selection)) &
+       3) != 0)
     return kErrMisaligned;
   if (int rc = check_device_sm100()) return rc;
-  c.batch = batch;
-  c.q_heads = q_heads;
-  c.kv_heads = kv_heads;
-  c.q_len = q_len;
-  c.kv_len = kv_len;
-  c.lengths = key_lengths;
-  c.pool = key_means;
-  c.topk = topk;
-  c.query_block = query_block;
-  c.key_block = key_block;
-  c.scale = softmax_scale;
-  c.out = out;
-  c.selection = selection;
-  c.workspace = static_cast<char*>(workspace);
+  c.batch = a.batch;
+  c.q_heads = a.q_heads;
+  c.kv_heads = a.kv_heads;
+  c.q_len = a.q_len;
+  c.kv_len = a.kv_len;
+  c.lengths = a.key_lengths;
+  c.pool = a.key_means;
+  c.topk = a.topk;
+  c.query_block = a.query_block;
+  c.key_block = a.key_block;
+  c.scale = a.softmax_scale;
+  c.out = a.out;
+  c.selection = a.selection;
+  c.workspace = static_cast<char*>(a.workspace);
   c.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == ERD_BF16 ? btk::run<__nv_bfloat16, true>(c, st) : btk::run<__half, false>(c, st);
+  return a.dtype == ERD_BF16 ? btk::run<__nv_bfloat16, true>(c, st)
+                             : btk::run<__half, false>(c, st);
 }

@@ -363,84 +363,75 @@ int dispatch(const Params& p, bool norm, bool interleaved, bool vector, cudaStre
 
 using namespace erd;
 
-extern "C" int erd_head_norm_rotary(
-    int dtype, const void* q, const void* k, int64_t q_token_stride, int64_t q_head_stride,
-    int64_t q_batch_stride, int64_t k_token_stride, int64_t k_head_stride, int64_t k_batch_stride,
-    int batch, int tokens, int q_heads, int k_heads, int head_dim, int rotary_dim, int interleaved,
-    int norm, const void* q_weight, const void* k_weight, int weight_fp32, float q_eps,
-    float k_eps, const double* turns, float amplitude, int inverse, int second_axis,
-    int third_axis, const void* positions, int positions_int64, int64_t pos_axis_stride,
-    int64_t pos_batch_stride, int64_t pos_token_stride, int64_t start, void* q_out, void* k_out,
-    int64_t q_out_token_stride, int64_t q_out_head_stride, int64_t q_out_batch_stride,
-    int64_t k_out_token_stride, int64_t k_out_head_stride, int64_t k_out_batch_stride,
-    void* stream) {
-  if (q == nullptr || q_out == nullptr || (k_heads > 0 && (k == nullptr || k_out == nullptr)) ||
-      (rotary_dim > 0 && turns == nullptr))
+extern "C" int erd_head_norm_rotary(const erd_head_norm_rotary_args* args, void* stream) {
+  if (args == nullptr) return kErrNullPointer;
+  const erd_head_norm_rotary_args& a = *args;
+  if (a.struct_bytes != static_cast<int64_t>(sizeof(a))) return kErrBadShape;
+  if (a.q == nullptr || a.q_out == nullptr ||
+      (a.k_heads > 0 && (a.k == nullptr || a.k_out == nullptr)) ||
+      (a.rotary_dim > 0 && a.turns == nullptr))
     return kErrNullPointer;
-  if (dtype < ERD_BF16 || dtype > ERD_FP32 || batch <= 0 || tokens <= 0 || q_heads <= 0 ||
-      k_heads < 0 || head_dim <= 0 || rotary_dim < 0 || rotary_dim > head_dim ||
-      (rotary_dim & 1) != 0)
+  if (a.dtype < ERD_BF16 || a.dtype > ERD_FP32 || a.batch <= 0 || a.tokens <= 0 ||
+      a.q_heads <= 0 || a.k_heads < 0 || a.head_dim <= 0 || a.rotary_dim < 0 ||
+      a.rotary_dim > a.head_dim || (a.rotary_dim & 1) != 0)
     return kErrBadShape;
-  if (head_dim > rot::kMaxHeadDim) return kErrTooLarge;
-  const uintptr_t elem = dtype == ERD_FP32 ? 4 : 2;
-  const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_out) |
-                        (k_heads > 0 ? reinterpret_cast<uintptr_t>(k) |
-                                           reinterpret_cast<uintptr_t>(k_out)
-                                     : 0);
-  const uintptr_t weights =
-      reinterpret_cast<uintptr_t>(q_weight) | reinterpret_cast<uintptr_t>(k_weight);
-  if ((all & (elem - 1)) != 0 || (weights & (weight_fp32 ? 3 : elem - 1)) != 0 ||
-      (reinterpret_cast<uintptr_t>(turns) & 7) != 0 ||
-      (reinterpret_cast<uintptr_t>(positions) & (positions_int64 ? 7 : 3)) != 0)
+  if (a.head_dim > rot::kMaxHeadDim) return kErrTooLarge;
+  auto address = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
+  const uintptr_t elem = a.dtype == ERD_FP32 ? 4 : 2;
+  const uintptr_t all = address(a.q) | address(a.q_out) |
+                        (a.k_heads > 0 ? address(a.k) | address(a.k_out) : 0);
+  const uintptr_t weights = address(a.q_weight) | address(a.k_weight);
+  if ((all & (elem - 1)) != 0 || (weights & (a.weight_fp32 ? 3 : elem - 1)) != 0 ||
+      (address(a.turns) & 7) != 0 || (address(a.positions) & (a.positions_int64 ? 7 : 3)) != 0)
     return kErrMisaligned;
   if (int rc = check_device_sm100()) return rc;
   rot::Params p = {};
-  p.in[0] = q;
-  p.in[1] = k;
-  p.out[0] = q_out;
-  p.out[1] = k_out;
-  p.weight[0] = norm ? q_weight : nullptr;
-  p.weight[1] = norm ? k_weight : nullptr;
-  p.in_ts[0] = q_token_stride, p.in_hs[0] = q_head_stride, p.in_bs[0] = q_batch_stride;
-  p.in_ts[1] = k_token_stride, p.in_hs[1] = k_head_stride, p.in_bs[1] = k_batch_stride;
-  p.out_ts[0] = q_out_token_stride, p.out_hs[0] = q_out_head_stride;
-  p.out_bs[0] = q_out_batch_stride, p.out_ts[1] = k_out_token_stride;
-  p.out_hs[1] = k_out_head_stride, p.out_bs[1] = k_out_batch_stride;
-  p.heads[0] = q_heads;
-  p.heads[1] = k_heads;
-  p.eps[0] = q_eps;
-  p.eps[1] = k_eps;
-  p.weight_fp32 = weight_fp32;
-  p.batch = batch;
-  p.tokens = tokens;
-  p.dim = head_dim;
-  p.rotary = rotary_dim;
-  p.turns = turns;
-  p.amplitude = amplitude;
-  p.sin_sign = inverse ? -1.f : 1.f;
-  p.axis1 = second_axis;
-  p.axis2 = third_axis;
-  p.pos = positions;
-  p.pos_wide = positions_int64;
-  p.pos_as = pos_axis_stride;
-  p.pos_bs = pos_batch_stride;
-  p.pos_ts = pos_token_stride;
-  p.start = start;
+  p.in[0] = a.q;
+  p.in[1] = a.k;
+  p.out[0] = a.q_out;
+  p.out[1] = a.k_out;
+  p.weight[0] = a.norm ? a.q_weight : nullptr;
+  p.weight[1] = a.norm ? a.k_weight : nullptr;
+  p.in_ts[0] = a.q_stride[0], p.in_hs[0] = a.q_stride[1], p.in_bs[0] = a.q_stride[2];
+  p.in_ts[1] = a.k_stride[0], p.in_hs[1] = a.k_stride[1], p.in_bs[1] = a.k_stride[2];
+  p.out_ts[0] = a.q_out_stride[0], p.out_hs[0] = a.q_out_stride[1];
+  p.out_bs[0] = a.q_out_stride[2], p.out_ts[1] = a.k_out_stride[0];
+  p.out_hs[1] = a.k_out_stride[1], p.out_bs[1] = a.k_out_stride[2];
+  p.heads[0] = a.q_heads;
+  p.heads[1] = a.k_heads;
+  p.eps[0] = a.q_eps;
+  p.eps[1] = a.k_eps;
+  p.weight_fp32 = a.weight_fp32;
+  p.batch = a.batch;
+  p.tokens = a.tokens;
+  p.dim = a.head_dim;
+  p.rotary = a.rotary_dim;
+  p.turns = a.turns;
+  p.amplitude = a.amplitude;
+  p.sin_sign = a.inverse ? -1.f : 1.f;
+  p.axis1 = a.second_axis;
+  p.axis2 = a.third_axis;
+  p.pos = a.positions;
+  p.pos_wide = a.positions_int64;
+  p.pos_as = a.pos_stride[0];
+  p.pos_bs = a.pos_stride[1];
+  p.pos_ts = a.pos_stride[2];
+  p.start = a.start;
   // Chunks of 16 bytes fit when every head starts on 16 bytes, the head is a
   // whole number of chunks (at most two a lane) and no chunk holds both turned
   // and other channels or, in the half layout, channels of both halves.
   const int n = static_cast<int>(16 / elem);
-  int64_t strides = q_token_stride | q_head_stride | q_batch_stride | q_out_token_stride |
-                    q_out_head_stride | q_out_batch_stride;
-  if (k_heads > 0)
-    strides |= k_token_stride | k_head_stride | k_batch_stride | k_out_token_stride |
-               k_out_head_stride | k_out_batch_stride;
-  const bool vector = (all & 15) == 0 && (strides & (n - 1)) == 0 && head_dim % n == 0 &&
-                      head_dim <= 64 * n && rotary_dim % (interleaved ? n : 2 * n) == 0;
+  int64_t strides = 0;
+  for (int i = 0; i < 3; ++i) {
+    strides |= a.q_stride[i] | a.q_out_stride[i];
+    if (a.k_heads > 0) strides |= a.k_stride[i] | a.k_out_stride[i];
+  }
+  const bool vector = (all & 15) == 0 && (strides & (n - 1)) == 0 && a.head_dim % n == 0 &&
+                      a.head_dim <= 64 * n && a.rotary_dim % (a.interleaved ? n : 2 * n) == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  switch (dtype) {
-    case ERD_BF16: return rot::dispatch<__nv_bfloat16>(p, norm, interleaved, vector, st);
-    case ERD_FP16: return rot::dispatch<__half>(p, norm, interleaved, vector, st);
-    default: return rot::dispatch<float>(p, norm, interleaved, vector, st);
+  switch (a.dtype) {
+    case ERD_BF16: return rot::dispatch<__nv_bfloat16>(p, a.norm, a.interleaved, vector, st);
+    case ERD_FP16: return rot::dispatch<__half>(p, a.norm, a.interleaved, vector, st);
+    default: return rot::dispatch<float>(p, a.norm, a.interleaved, vector, st);
   }
 }

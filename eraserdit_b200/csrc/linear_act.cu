@@ -1235,38 +1235,40 @@ int run(const Epilogue& e, const void* x, int64_t ldx, const void* w, int64_t ld
 
 using namespace erd;
 
-extern "C" int erd_linear_act(int dtype, const void* x, int64_t ldx, const void* weight,
-                              int64_t ldw, const void* bias, int activation, const void* gate,
-                              int gate_rows, const void* residual, int64_t ld_residual, void* y,
-                              int64_t ldy, int m, int n, int k, int* status, void* stream) {
-  if (x == nullptr || weight == nullptr || y == nullptr) return kErrNullPointer;
-  if ((dtype != ERD_BF16 && dtype != ERD_FP16) || activation < ERD_ACT_NONE ||
-      activation > ERD_ACT_GELU_TANH || m <= 0 || n <= 0 || k <= 0 || ldx < k || ldw < k ||
-      ldy < n || (residual != nullptr && ld_residual < n) || (gate != nullptr && gate_rows <= 0))
+extern "C" int erd_linear_act(const erd_linear_act_args* args, int* status, void* stream) {
+  if (args == nullptr) return kErrNullPointer;
+  const erd_linear_act_args& a = *args;
+  if (a.struct_bytes != static_cast<int64_t>(sizeof(a))) return kErrBadShape;
+  if (a.x == nullptr || a.weight == nullptr || a.y == nullptr) return kErrNullPointer;
+  if ((a.dtype != ERD_BF16 && a.dtype != ERD_FP16) || a.activation < ERD_ACT_NONE ||
+      a.activation > ERD_ACT_GELU_TANH || a.m <= 0 || a.n <= 0 || a.k <= 0 || a.ldx < a.k ||
+      a.ldw < a.k || a.ldy < a.n || (a.residual != nullptr && a.ld_residual < a.n) ||
+      (a.gate != nullptr && a.gate_rows <= 0))
     return kErrBadShape;
-  const uintptr_t values = reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(gate) |
-                           reinterpret_cast<uintptr_t>(residual) | reinterpret_cast<uintptr_t>(y);
-  if (!aligned16(x) || !aligned16(weight) || (ldx & 7) != 0 || (ldw & 7) != 0 || (values & 1) != 0)
+  auto address = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
+  const uintptr_t values = address(a.bias) | address(a.gate) | address(a.residual) | address(a.y);
+  if (!aligned16(a.x) || !aligned16(a.weight) || (a.ldx & 7) != 0 || (a.ldw & 7) != 0 ||
+      (values & 1) != 0)
     return kErrMisaligned;
-  if (m > 0x7fffff00 || n > 0x7fffff00 || k > 0x7fffff00) return kErrTooLarge;
+  if (a.m > 0x7fffff00 || a.n > 0x7fffff00 || a.k > 0x7fffff00) return kErrTooLarge;
   if (int rc = check_device_sm100()) return rc;
   lact::Epilogue e = {};
-  e.m = m;
-  e.n = n;
-  e.act = activation;
-  e.bias = bias;
-  e.gate = gate;
-  e.gate_rows = gate_rows;
-  e.residual = residual;
-  e.ld_res = ld_residual;
-  e.y = y;
-  e.ldy = ldy;
-  e.vec_bias = aligned16(bias);
-  e.vec_gate = aligned16(gate) && (n & 7) == 0;
-  e.vec_res = aligned16(residual) && (ld_residual & 7) == 0;
-  e.vec_y = aligned16(y) && (ldy & 7) == 0;
+  e.m = a.m;
+  e.n = a.n;
+  e.act = a.activation;
+  e.bias = a.bias;
+  e.gate = a.gate;
+  e.gate_rows = a.gate_rows;
+  e.residual = a.residual;
+  e.ld_res = a.ld_residual;
+  e.y = a.y;
+  e.ldy = a.ldy;
+  e.vec_bias = aligned16(a.bias);
+  e.vec_gate = aligned16(a.gate) && (a.n & 7) == 0;
+  e.vec_res = aligned16(a.residual) && (a.ld_residual & 7) == 0;
+  e.vec_y = aligned16(a.y) && (a.ldy & 7) == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == ERD_BF16
-             ? lact::run<__nv_bfloat16, true>(e, x, ldx, weight, ldw, k, status, st)
-             : lact::run<__half, false>(e, x, ldx, weight, ldw, k, status, st);
+  return a.dtype == ERD_BF16
+             ? lact::run<__nv_bfloat16, true>(e, a.x, a.ldx, a.weight, a.ldw, a.k, status, st)
+             : lact::run<__half, false>(e, a.x, a.ldx, a.weight, a.ldw, a.k, status, st);
 }

@@ -184,7 +184,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     if residual is not None and residual.shape != shape:
         raise ValueError("residual must be [..., n]")
     if out is None:
-        out = x.new_empty(shape)
+        out = torch.empty(shape, dtype=dtype, device=device)
     elif out.shape != shape or any(s == 0 and d > 1 for s, d in zip(out.stride(), out.shape)):
         raise ValueError("out must be [..., n] and no expanded view")
     m = x.numel() // k
@@ -214,9 +214,9 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     xp, wp = x.data_ptr(), weight.data_ptr()
     if (xp | wp) % 16 or (ldx | ldw) % 8:
         raise ValueError("rows of x and weight must start on 16 bytes (strides multiples of 8)")
-    _native.call("erd_linear_act", device, _native.DTYPE_CODES[dtype], xp, ldx, wp, ldw,
-                 None if bias is None else bias.data_ptr(), code,
-                 None if gate is None else gate.data_ptr(), gate_rows,
-                 None if residual is None else residual.data_ptr(), ldr, out.data_ptr(), ldy, m, n,
-                 k, _native.status_pointer(device))
+    _native.call("erd_linear_act", device, _native.pack(
+        "erd_linear_act", xp, wp, 0 if bias is None else bias.data_ptr(),
+        0 if gate is None else gate.data_ptr(), 0 if residual is None else residual.data_ptr(),
+        out.data_ptr(), ldx, ldw, ldr, ldy, _native.DTYPE_CODES[dtype], code, gate_rows, m, n, k),
+        _native.status_pointer(device))
     return out

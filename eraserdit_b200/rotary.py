@@ -246,7 +246,7 @@ def _positions_args(rotary: RotaryPositions, positions, batch: int, tokens: int)
     if isinstance(positions, int):
         if rotary.axes != 1:
             raise ValueError("positions on several axes are a tensor")
-        return None, 0, 0, 0, 0, positions
+        return 0, 0, 0, 0, 0, positions
     if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
         raise ValueError("positions must be an int or an int32 / int64 tensor")
     if positions.device != rotary.device:
@@ -289,7 +289,8 @@ def _check_out(what: str, out: torch.Tensor, x: torch.Tensor) -> tuple:
 def _new_out(x: torch.Tensor) -> tuple[torch.Tensor, tuple]:
     """An empty contiguous tensor of x's shape and its (token, head, batch) strides."""
     _, tokens, heads, dim = x.shape
-    return x.new_empty(x.shape), (heads * dim, dim, tokens * heads * dim)
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    return out, (heads * dim, dim, tokens * heads * dim)
 
 
 def head_rotary_call(what: str, query, key, rotary, positions, q_weight, k_weight, norm: bool,
@@ -297,7 +298,7 @@ def head_rotary_call(what: str, query, key, rotary, positions, q_weight, k_weigh
     """Checks and launch shared by the rotation with and without the norm."""
     q_strides, k_strides = _check_heads("query", query), (0, 0, 0)
     batch, tokens, heads, dim = query.shape
-    kv_heads, k_out, k_ptr, ko_ptr, ko_strides = 0, None, None, None, (0, 0, 0)
+    kv_heads, k_out, k_ptr, ko_ptr, ko_strides = 0, None, 0, 0, (0, 0, 0)
     if key is not None:
         k_strides = _check_heads("key", key, query)
         kv_heads, k_ptr = key.shape[2], key.data_ptr()
@@ -311,12 +312,12 @@ def head_rotary_call(what: str, query, key, rotary, positions, q_weight, k_weigh
         if rotary.device != query.device:
             raise ValueError("rotary lives on another device than the query")
         where = _positions_args(rotary, positions, batch, tokens)
-        turn = (rotary.turns.data_ptr(), rotary.amplitude, inverse, rotary.second_axis,
-                rotary.third_axis)
+        turns, amplitude = rotary.turns.data_ptr(), rotary.amplitude
+        axis1, axis2 = rotary.second_axis, rotary.third_axis
         rotary_dim, interleaved = rotary.rotary_dim, rotary.layout == "interleaved"
     else:
-        where, turn = (None, 0, 0, 0, 0, 0), (None, 1.0, 0, 0, 0)
-        rotary_dim = interleaved = 0
+        where, amplitude = (0, 0, 0, 0, 0, 0), 1.0
+        turns = axis1 = axis2 = rotary_dim = interleaved = 0
     if query_out is None:
         q_out, qo_strides = _new_out(query)
     else:
@@ -335,12 +336,14 @@ def head_rotary_call(what: str, query, key, rotary, positions, q_weight, k_weigh
         raise ValueError("the query needs at least one head")
     weight = q_weight if q_weight is not None else k_weight
     device = query.device
-    _native.call(
-        "erd_head_norm_rotary", device, _native.DTYPE_CODES[query.dtype], query.data_ptr(), k_ptr,
-        *q_strides, *k_strides, batch, tokens, heads, kv_heads, dim, rotary_dim, interleaved, norm,
-        _native.ptr(q_weight), _native.ptr(k_weight),
-        weight is not None and weight.dtype == torch.float32, q_eps, k_eps, *turn, *where,
-        q_out.data_ptr(), ko_ptr, *qo_strides, *ko_strides)
+    _native.call("erd_head_norm_rotary", device, _native.pack(
+        "erd_head_norm_rotary", query.data_ptr(), k_ptr,
+        0 if q_weight is None else q_weight.data_ptr(),
+        0 if k_weight is None else k_weight.data_ptr(), turns, where[0], q_out.data_ptr(), ko_ptr,
+        *q_strides, *k_strides, *qo_strides, *ko_strides, *where[2:],
+        _native.DTYPE_CODES[query.dtype], batch, tokens, heads, kv_heads, dim, rotary_dim,
+        interleaved, norm, weight is not None and weight.dtype == torch.float32, inverse, axis1,
+        axis2, where[1], q_eps, k_eps, amplitude))
     if rotary is not None and _native.raw_stream(device.index) != rotary._stream:
         rotary.turns.record_stream(torch.cuda.current_stream(device))
     return q_out, k_out

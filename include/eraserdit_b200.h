@@ -15,7 +15,8 @@
  *     inside a kernel that timed out (the kernel then returns early instead of
  *     hanging).  The caller reads them after synchronising.
  * BF16 tensors are passed as void* (16-bit words).
- * Entry points that take several value types name them with the ERD_* codes.
+ * Entry points that take several value types name them with the ERD_* codes;
+ * those with many arguments take them in a struct.
  */
 #ifndef ERASERDIT_B200_H_
 #define ERASERDIT_B200_H_
@@ -433,17 +434,21 @@ int erd_attn_fwd_fp8_static_scratch(
  * 16-byte chunks take 16-byte accesses; any other size or stride is read value
  * by value.
  */
-int erd_head_norm_rotary(
-    int dtype, const void* q, const void* k, int64_t q_token_stride, int64_t q_head_stride,
-    int64_t q_batch_stride, int64_t k_token_stride, int64_t k_head_stride, int64_t k_batch_stride,
-    int batch, int tokens, int q_heads, int k_heads, int head_dim, int rotary_dim, int interleaved,
-    int norm, const void* q_weight, const void* k_weight, int weight_fp32, float q_eps,
-    float k_eps, const double* turns, float amplitude, int inverse, int second_axis,
-    int third_axis, const void* positions, int positions_int64, int64_t pos_axis_stride,
-    int64_t pos_batch_stride, int64_t pos_token_stride, int64_t start, void* q_out, void* k_out,
-    int64_t q_out_token_stride, int64_t q_out_head_stride, int64_t q_out_batch_stride,
-    int64_t k_out_token_stride, int64_t k_out_head_stride, int64_t k_out_batch_stride,
-    void* stream);
+typedef struct {
+  int64_t struct_bytes; /* sizeof this struct, checked */
+  const void *q, *k, *q_weight, *k_weight;
+  const double* turns;
+  const void* positions;
+  void *q_out, *k_out;
+  int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3]; /* token, head, batch */
+  int64_t pos_stride[3];                                              /* axis, batch, token */
+  int64_t start;
+  int32_t dtype, batch, tokens, q_heads, k_heads, head_dim, rotary_dim, interleaved;
+  int32_t norm, weight_fp32, inverse, second_axis, third_axis, positions_int64;
+  float q_eps, k_eps, amplitude;
+} erd_head_norm_rotary_args;
+
+int erd_head_norm_rotary(const erd_head_norm_rotary_args* args, void* stream);
 
 /*
  * Matrix product with its epilogue:
@@ -464,10 +469,15 @@ enum {
   ERD_ACT_GELU_TANH = 4  /* x / 2 (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) */
 };
 
-int erd_linear_act(int dtype, const void* x, int64_t ldx, const void* weight, int64_t ldw,
-                   const void* bias, int activation, const void* gate, int gate_rows,
-                   const void* residual, int64_t ld_residual, void* y, int64_t ldy, int m, int n,
-                   int k, int* status, void* stream);
+typedef struct {
+  int64_t struct_bytes; /* sizeof this struct, checked */
+  const void *x, *weight, *bias, *gate, *residual;
+  void* y;
+  int64_t ldx, ldw, ld_residual, ldy;
+  int32_t dtype, activation, gate_rows, m, n, k;
+} erd_linear_act_args;
+
+int erd_linear_act(const erd_linear_act_args* args, int* status, void* stream);
 
 /*
  * Attention over key blocks that a cheap score selects, head_dim 64.
@@ -493,16 +503,21 @@ int erd_linear_act(int dtype, const void* x, int64_t ldx, const void* weight, in
 size_t erd_block_topk_workspace_bytes(int batch, int q_heads, int kv_heads, int q_len, int kv_len,
                                       int query_block, int key_block, int has_pool);
 
-int erd_block_topk_attn(int dtype, const void* q, const void* k, const void* v,
-                        int64_t q_token_stride, int64_t q_head_stride, int64_t q_batch_stride,
-                        int64_t k_token_stride, int64_t k_head_stride, int64_t k_batch_stride,
-                        int64_t v_token_stride, int64_t v_head_stride, int64_t v_batch_stride,
-                        int batch, int q_heads, int kv_heads, int q_len, int kv_len, int head_dim,
-                        const int32_t* key_lengths, const double* key_means, int topk,
-                        int query_block, int key_block, float softmax_scale, void* out,
-                        int64_t o_token_stride, int64_t o_head_stride, int64_t o_batch_stride,
-                        int32_t* selection, void* workspace, size_t workspace_bytes, int* status,
-                        void* stream);
+typedef struct {
+  int64_t struct_bytes; /* sizeof this struct, checked */
+  const void *q, *k, *v;
+  const int32_t* key_lengths;
+  const double* key_means;
+  void* out;
+  int32_t* selection;
+  void* workspace;
+  int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3]; /* token, head, batch */
+  int64_t workspace_bytes;
+  int32_t dtype, batch, q_heads, kv_heads, q_len, kv_len, head_dim, topk, query_block, key_block;
+  float softmax_scale;
+} erd_block_topk_args;
+
+int erd_block_topk_attn(const erd_block_topk_args* args, int* status, void* stream);
 
 /*
  * Means of every block of key_block keys over its valid keys, in FP64:

@@ -33,10 +33,14 @@ def test_entries_reject_bad_arguments_before_any_device_call():
     def call(dtype=0, q=p, k=p, v=p, qt=64, ot=64, batch=1, heads=2, kv_heads=1, q_len=5, kv_len=70,
              dim=64, lengths=None, means=None, topk=1, qb=1, kb=64, out=p, sel=p, ws=p, nbytes=1 << 20,
              scale=0.125):
-        return lib.erd_block_topk_attn(dtype, q, k, v, qt, 64, 64, 64, 64, 64, 64, 64, 64, batch,
-                                       heads, kv_heads, q_len, kv_len, dim, lengths, means, topk, qb,
-                                       kb, scale, out, ot, 64, 64, sel, ws, nbytes, None, None)
+        fields = (q, k, v, lengths, means, out, sel, ws, qt, *([64] * 8), ot, 64, 64, nbytes, dtype,
+                  batch, heads, kv_heads, q_len, kv_len, dim, topk, qb, kb, scale)
+        return lib.erd_block_topk_attn(
+            _native.pack("erd_block_topk_attn", *(0 if f is None else f for f in fields)), None, None)
 
+    assert lib.erd_block_topk_attn(None, None, None) == -1
+    other = _native.STRUCTS["erd_block_topk_attn"].pack(8, *([0] * 32))
+    assert lib.erd_block_topk_attn(other, None, None) == -2
     for kw in (dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(sel=None), dict(ws=None)):
         assert call(**kw) == -1, kw
     for kw in (dict(dtype=2), dict(dim=128), dict(batch=0), dict(heads=3, kv_heads=2), dict(kv_heads=0),

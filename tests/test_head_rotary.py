@@ -73,10 +73,15 @@ def test_entry_rejects_bad_arguments_before_any_device_call():
 
     def call(dtype=0, q=p, k=p, batch=1, tokens=1, heads=1, kv_heads=1, dim=64, rotary=64,
              turns=p, q_out=p, k_out=p, weight=None, weight_fp32=0, pos=None, wide=0):
-        return fn(dtype, q, k, *([64] * 6), batch, tokens, heads, kv_heads, dim, rotary, 0, 1,
-                  weight, weight, weight_fp32, 1e-6, 1e-6, turns, 1.0, 0, rotary // 2, rotary // 2,
-                  pos, wide, 0, 0, 1, 0, q_out, k_out, *([64] * 6), None)
+        fields = (q, k, weight, weight, turns, pos, q_out, k_out, *([64] * 12), 0, 0, 1, 0, dtype,
+                  batch, tokens, heads, kv_heads, dim, rotary, 0, 1, weight_fp32, 0, rotary // 2,
+                  rotary // 2, wide, 1e-6, 1e-6, 1.0)
+        return fn(_native.pack("erd_head_norm_rotary", *(0 if f is None else f for f in fields)), None)
 
+    assert fn(None, None) == -1
+    assert fn(_native.STRUCTS["erd_head_norm_rotary"].pack(8, *([0] * 41)), None) == -2  # another struct
+    with pytest.raises(ValueError):
+        call(tokens=2 ** 31)
     assert call(q=None) == -1 and call(q_out=None) == -1 and call(k_out=None) == -1
     assert call(turns=None) == -1
     assert call(dtype=3) == -2 and call(batch=0) == -2 and call(tokens=0) == -2

@@ -16,8 +16,11 @@ def test_entry_rejects_bad_arguments_before_any_device_call():
 
     def call(dtype=0, x=p, ldx=64, w=p, ldw=64, bias=None, act=0, gate=None, gate_rows=0, res=None,
              ldr=0, y=p, ldy=48, m=4, n=48, k=64):
-        return fn(dtype, x, ldx, w, ldw, bias, act, gate, gate_rows, res, ldr, y, ldy, m, n, k,
-                  None, None)
+        fields = (x, w, bias, gate, res, y, ldx, ldw, ldr, ldy, dtype, act, gate_rows, m, n, k)
+        return fn(_native.pack("erd_linear_act", *(0 if f is None else f for f in fields)), None, None)
+
+    assert fn(None, None, None) == -1
+    assert fn(_native.STRUCTS["erd_linear_act"].pack(8, *([0] * 16)), None, None) == -2  # another struct
 
     assert call(x=None) == -1 and call(w=None) == -1 and call(y=None) == -1
     assert call(dtype=2) == -2 and call(dtype=-1) == -2 and call(act=5) == -2 and call(act=-1) == -2
