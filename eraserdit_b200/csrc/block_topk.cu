@@ -249,138 +249,113 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
   return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
 }
 
-// One warp writes the indices of the `take` greatest of n keys (ties: lowest
-// index) in ascending order, then -1 up to topk.  `key(i)` gives key i; with
-// kPer > 0 (n <= 32 kPer) their upper words stay in registers.  Bisection over
-// the bits of the upper words, which ends as soon as a threshold splits off
-// exactly `take` keys (after some twenty steps for scores that differ), and
-// over the lower words of those that tie there only if they do.
-template <int kPer, typename Key>
-__device__ __forceinline__ void select_topk(Key key, int n, int take, int topk, int* out,
+// One warp writes the indices of the `take` greatest of n scores (ties: lowest
+// index; NaN below every number) in ascending order, then -1 up to topk.
+// `score(i)` gives score i.
+//
+// With kPer > 0 (n <= 32 kPer) the scores stay in registers, rounded to FP32, and
+// the threshold is bisected between the smallest and the greatest: rounding keeps
+// the order, so a threshold that exactly `take` rounded scores reach splits the
+// scores as they are.  That ends after about log2 of (range / gap at the
+// threshold) steps, ten at 510 blocks, where the bits of the scores from the top
+// took twenty.  Where FP32 cannot split them (ties, infinities, n > 32 kPer) the
+// bits of the keys decide, upper words first, lower words where those tie.
+template <int kPer, typename Score>
+__device__ __forceinline__ void select_topk(Score score, int n, int take, int topk, int* out,
                                             int lane) {
-  uint32_t hi[kPer > 0 ? kPer : 1];
   const int rounds = (n + 31) / 32;
+  const uint32_t before = (1u << lane) - 1;
+  for (int i = take + lane; i < topk; i += 32) out[i] = -1;
+  if (take >= n) {
+    for (int i = lane; i < n; i += 32) out[i] = i;
+    return;
+  }
   if (kPer > 0) {
+    float f[kPer > 0 ? kPer : 1];
+    float lo = CUDART_INF_F, hi = -CUDART_INF_F;
+    bool finite = true;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int i = j * 32 + lane;
-      hi[j] = i < n ? static_cast<uint32_t>(key(i) >> 32) : 0u;
+      f[j] = -CUDART_INF_F;
+      if (i < n) {
+        f[j] = __double2float_rn(score(i));
+        finite = finite && fabsf(f[j]) < CUDART_INF_F;  // false for NaN
+        lo = fminf(lo, f[j]);
+        hi = fmaxf(hi, f[j]);
+      }
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+    }
+    if (__all_sync(0xffffffffu, finite)) {
+      // take < n scores reach no threshold above hi, all n reach lo
+      for (int step = 0; step < 40; ++step) {
+        const float mid = 0.5f * lo + 0.5f * hi;
+        if (!(mid > lo && mid < hi)) break;
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) c += f[j] >= mid;
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (c == take) {
+          int count = 0;
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) {
+            const bool yes = f[j] >= mid;
+            const uint32_t mask = __ballot_sync(0xffffffffu, yes);
+            if (yes) out[count + __popc(mask & before)] = j * 32 + lane;
+            count += __popc(mask);
+          }
+          return;
+        }
+        (c > take ? lo : hi) = mid;
+      }
     }
   }
-  // number of keys whose upper word is at least t (t > 0: absent ones are 0)
-  auto at_least = [&](uint32_t t) {
+  // Keys of the scores: the greatest t whose upper word at least `take` keys
+  // reach, then the greatest lower word that as many reach as are still wanted.
+  auto count_keys = [&](auto reaches) {
     int c = 0;
-    if (kPer > 0) {
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) c += hi[j] >= t;
-    } else {
-      for (int j = 0; j < rounds; ++j) {
-        const int i = j * 32 + lane;
-        c += i < n && static_cast<uint32_t>(key(i) >> 32) >= t;
-      }
+    for (int j = 0; j < rounds; ++j) {
+      const int i = j * 32 + lane;
+      c += i < n && reaches(score_key(score(i)));
     }
     return __reduce_add_sync(0xffffffffu, c);
   };
-  // Greatest t with at_least(t) >= take (take <= n, so t = 0 always holds).
-  uint32_t t = 0;
-  bool exact = take >= n;  // everything is taken
-  if (!exact) {
-    // bits that all upper words share need no step
-    uint32_t most = 0, least = 0xffffffffu;
-    if (kPer > 0) {
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        most = max(most, hi[j]);
-        if (j * 32 + lane < n) least = min(least, hi[j]);
-      }
-    } else {
-      for (int j = 0; j < rounds; ++j) {
-        const int i = j * 32 + lane;
-        if (i < n) {
-          const uint32_t w = static_cast<uint32_t>(key(i) >> 32);
-          most = max(most, w);
-          least = min(least, w);
-        }
-      }
-    }
-    most = __reduce_max_sync(0xffffffffu, most);
-    least = __reduce_min_sync(0xffffffffu, least);
-    const int top = 31 - __clz(most ^ least);  // -1: they are all equal
-    t = top < 0 ? most : top == 31 ? 0u : most >> (top + 1) << (top + 1);
-    for (int bit = top; bit >= 0; --bit) {
-      const uint32_t up = t | (1u << bit);
-      const int c = at_least(up);
-      if (c >= take) {
-        t = up;
-        if (c == take) {
-          exact = true;
-          break;
-        }
-      }
-    }
+  uint32_t t = 0, low = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t up = t | (1u << bit);
+    if (count_keys([&](unsigned long long k) { return static_cast<uint32_t>(k >> 32) >= up; }) >=
+        take)
+      t = up;
   }
-  // Keys above t are taken, those at t as far as `ties` allows by their lower
-  // words.
-  uint32_t low = 0;
-  int ties = 0;  // keys equal to (t, low) that are taken
-  if (!exact) {
-    const int above = t == 0xffffffffu ? 0 : at_least(t + 1);
-    const int want = take - above;
-    auto low_at_least = [&](uint32_t v) {
-      int c = 0;
-      for (int j = 0; j < rounds; ++j) {
-        const int i = j * 32 + lane;
-        if (i < n) {
-          const unsigned long long k = key(i);
-          c += static_cast<uint32_t>(k >> 32) == t && static_cast<uint32_t>(k) >= v;
-        }
-      }
-      return __reduce_add_sync(0xffffffffu, c);
-    };
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t up = low | (1u << bit);
-      if (low_at_least(up) >= want) low = up;
-    }
-    ties = want - (low == 0xffffffffu ? 0 : low_at_least(low + 1));
+  const int want =
+      take - count_keys([&](unsigned long long k) { return static_cast<uint32_t>(k >> 32) > t; });
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t up = low | (1u << bit);
+    if (count_keys([&](unsigned long long k) {
+          return static_cast<uint32_t>(k >> 32) == t && static_cast<uint32_t>(k) >= up;
+        }) >= want)
+      low = up;
   }
-  const uint32_t before = (1u << lane) - 1;
-  if (kPer > 0 && exact) {
-    int count = 0;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int i = j * 32 + lane;
-      const bool yes = i < n && (take >= n || hi[j] >= t);
-      const uint32_t mask = __ballot_sync(0xffffffffu, yes);
-      if (yes) out[count + __popc(mask & before)] = i;
-      count += __popc(mask);
-    }
-    for (int i = take + lane; i < topk; i += 32) out[i] = -1;
-    return;
-  }
-  int count = 0, tied = 0;
   const unsigned long long bound = (static_cast<unsigned long long>(t) << 32) | low;
+  // keys equal to the bound that are taken
+  const int ties = take - count_keys([&](unsigned long long k) { return k > bound; });
+  int count = 0, tied = 0;
   for (int j = 0; j < rounds; ++j) {
     const int i = j * 32 + lane;
-    bool yes = false, tie = false;
-    if (i < n) {
-      const unsigned long long k = key(i);
-      if (take >= n)
-        yes = true;
-      else if (exact)
-        yes = static_cast<uint32_t>(k >> 32) >= t;
-      else {
-        yes = k > bound;
-        tie = k == bound;
-      }
-    }
+    const unsigned long long k = i < n ? score_key(score(i)) : 0ull;
+    const bool tie = i < n && k == bound;
     const uint32_t tie_mask = __ballot_sync(0xffffffffu, tie);
-    if (tie && tied + __popc(tie_mask & before) < ties) yes = true;
+    const bool yes =
+        (i < n && k > bound) || (tie && tied + __popc(tie_mask & before) < ties);
     tied += __popc(tie_mask);
     const uint32_t mask = __ballot_sync(0xffffffffu, yes);
     if (yes) out[count + __popc(mask & before)] = i;
     count += __popc(mask);
   }
-  for (int i = take + lane; i < topk; i += 32) out[i] = -1;
 }
 
 constexpr int kSelectWarps = 4;
@@ -393,7 +368,7 @@ __global__ void __launch_bounds__(32 * kSelectWarps)
   const int len = key_length(lengths, static_cast<int>(row / rows_per_batch), kv_len);
   const int n = (len + key_block - 1) / key_block;
   const double* s = scores + row * blocks;
-  select_topk<kPer>([&](int i) { return score_key(s[i]); }, n, min(topk, n), topk,
+  select_topk<kPer>([&](int i) { return s[i]; }, n, min(topk, n), topk,
                     selection + row * topk, threadIdx.x & 31);
 }
 
@@ -790,13 +765,13 @@ __global__ void __launch_bounds__(kTileThreads, 4)
 // -------------------------------------------------------------- single queries
 // A row (batch, head, query) is the work of a cluster of 1 to 8 CTAs, in one
 // launch.  Its CTAs share the blocks' scores (eight lanes a block, eight channels
-// each, FP64) and write each score's key into every CTA's shared memory; each
-// finds the choice by itself and attends its part of it: eight lanes a key (16
-// bytes each of its K and V rows), eight neighbouring keys a lane group at a
-// time, with running maximum and sum.  Groups, warps and CTAs are merged in a
-// fixed order.  Bound by the bytes of the means and the chosen blocks.
+// each, FP64) and write each score into every CTA's shared memory; each makes the
+// choice by itself and attends its part of it: eight lanes a key (16 bytes each of
+// its K and V rows), four neighbouring keys a lane group at a time and four more
+// on the way, with running maximum and sum.  Groups, warps and CTAs are merged in
+// a fixed order.  Bound by the bytes of the means and the chosen blocks.
 constexpr int kRowWarps = 8;
-constexpr int kRowKeys = 8;
+constexpr int kRowKeys = 4;
 constexpr int kMaxSplits = 8;
 
 struct RowParams {
@@ -838,8 +813,8 @@ template <typename T>
 __global__ void __launch_bounds__(32 * kRowWarps, 2) row_kernel(const RowParams p) {
   __shared__ float part_m[kRowWarps], part_l[kRowWarps], part_o[kRowWarps][kDim];
   __shared__ float cta[kDim + 2];  // this CTA's O, maximum, sum
-  extern __shared__ unsigned long long keys[];  // [blocks], then the choice
-  int* list = reinterpret_cast<int*>(keys + p.blocks);
+  extern __shared__ double scores[];  // [blocks], then the choice
+  int* list = reinterpret_cast<int*>(scores + p.blocks);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = static_cast<int>(blockIdx.x % p.splits);  // also the rank in the cluster
   const long long row = blockIdx.x / p.splits;                // (batch, head, query)
@@ -895,8 +870,8 @@ __global__ void __launch_bounds__(32 * kRowWarps, 2) row_kernel(const RowParams 
         for (int d = 1; d < 8; d <<= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
         // lane r of the group writes into CTA r
         if ((lane & 7) < p.splits && i < n)
-          asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(map_rank(keys + i, lane & 7)),
-                       "l"(score_key(s))
+          asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(map_rank(scores + i, lane & 7)),
+                       "d"(s)
                        : "memory");
       }
     }
@@ -909,11 +884,15 @@ __global__ void __launch_bounds__(32 * kRowWarps, 2) row_kernel(const RowParams 
   }
   // ---------------------------------------------------------------- choice
   if (warp == 0) {
-    auto key = [&](int i) { return keys[i]; };
-    if (n <= 32 * 16)
-      select_topk<16>(key, n, take, take, list, lane);
+    auto score = [&](int i) { return scores[i]; };
+    if (n <= 32 * 4)
+      select_topk<4>(score, n, take, take, list, lane);
+    else if (n <= 32 * 16)
+      select_topk<16>(score, n, take, take, list, lane);
+    else if (n <= 32 * 48)
+      select_topk<48>(score, n, take, take, list, lane);
     else
-      select_topk<0>(key, n, take, take, list, lane);
+      select_topk<0>(score, n, take, take, list, lane);
     __syncwarp();
     if (split == 0) {
       int* out = p.selection + row * p.topk;
@@ -931,29 +910,33 @@ __global__ void __launch_bounds__(32 * kRowWarps, 2) row_kernel(const RowParams 
   float m = -CUDART_INF_F, l = 0.f, o[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) o[i] = 0.f;
-  // units of 32 keys: half a 64-key piece, eight keys a lane group
-  for (int u = 2 * lo + warp; u < 2 * hi; u += kRowWarps) {
-    const int first = list[(u >> 1) >> shift] * p.key_block + ((u >> 1) & shift) * kHalf +
-                      (u & 1) * 32 + group * kRowKeys;
-    uint4 kv[kRowKeys], vv[kRowKeys];
+  // units of 16 keys: a quarter of a 64-key piece, four keys a lane group; the
+  // next unit is requested before the current one is used
+  uint4 kv[2][kRowKeys], vv[2][kRowKeys];
+  int first = 0, next_first = 0;
+  auto request = [&](int u, uint4 (&kk)[kRowKeys], uint4 (&v_)[kRowKeys], int& f0) {
+    f0 = list[(u >> 2) >> shift] * p.key_block + ((u >> 2) & shift) * kHalf + (u & 3) * 16 +
+         group * kRowKeys;
 #pragma unroll
     for (int i = 0; i < kRowKeys; ++i) {
-      kv[i] = vv[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (first + i < len) kv[i] = *reinterpret_cast<const uint4*>(kp + (first + i) * p.k_st.token);
+      kk[i] = v_[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (f0 + i < len) kk[i] = *reinterpret_cast<const uint4*>(kp + (f0 + i) * p.k_st.token);
     }
 #pragma unroll
     for (int i = 0; i < kRowKeys; ++i)
-      if (first + i < len) vv[i] = *reinterpret_cast<const uint4*>(vp + (first + i) * p.v_st.token);
+      if (f0 + i < len) v_[i] = *reinterpret_cast<const uint4*>(vp + (f0 + i) * p.v_st.token);
+  };
+  auto use = [&](const uint4 (&kk)[kRowKeys], const uint4 (&v_)[kRowKeys], int f0) {
     float s[kRowKeys], top = m;
 #pragma unroll
     for (int i = 0; i < kRowKeys; ++i) {
       float f[8], d = 0.f;
-      unpack8<T>(kv[i], f);
+      unpack8<T>(kk[i], f);
 #pragma unroll
       for (int j = 0; j < 8; ++j) d = fmaf(q[j], f[j], d);
 #pragma unroll
       for (int x = 1; x < 8; x <<= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
-      s[i] = first + i < len ? d * p.scale_log2 : -CUDART_INF_F;
+      s[i] = f0 + i < len ? d * p.scale_log2 : -CUDART_INF_F;
       top = fmaxf(top, s[i]);
     }
     const float zero = top == -CUDART_INF_F ? 0.f : top;
@@ -966,11 +949,25 @@ __global__ void __launch_bounds__(32 * kRowWarps, 2) row_kernel(const RowParams 
       const float w = ex2_approx(s[i] - zero);
       l += w;
       float f[8];
-      unpack8<T>(vv[i], f);
+      unpack8<T>(v_[i], f);
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[j] = fmaf(w, f[j], o[j]);
     }
     m = top;
+  };
+  {
+    const int end = 4 * hi;
+    int u = 4 * lo + warp;
+    if (u < end) request(u, kv[0], vv[0], first);
+    while (u < end) {
+      if (u + kRowWarps < end) request(u + kRowWarps, kv[1], vv[1], next_first);
+      use(kv[0], vv[0], first);
+      u += kRowWarps;
+      if (u >= end) break;
+      if (u + kRowWarps < end) request(u + kRowWarps, kv[0], vv[0], first);
+      use(kv[1], vv[1], next_first);
+      u += kRowWarps;
+    }
   }
   // ----------------------------------------------------------------- merge
   // the four lane groups of the warp
