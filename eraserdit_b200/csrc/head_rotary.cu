@@ -15,9 +15,9 @@
 // token (or, when there are few tokens, some of its heads), computes each
 // pair's cosine and sine once, one pair a lane, shares them through shared
 // memory, and then walks over the heads; the angles cost one 64-bit product
-// per token and pair and no table is read.  A lane owns two 16-byte chunks of
-// a head that hold whole pairs in either layout, so loads and stores are
-// 16 bytes wide and the norm's sum needs log2(lanes per head) shuffles.
+// per token and pair and no table is read.  A lane owns two chunks of a head that
+// hold whole pairs in either layout, so accesses are wide and the norm's sum needs
+// log2(lanes per head) shuffles.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -29,11 +29,11 @@
 namespace erd {
 namespace rot {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 constexpr int kMaxHeadDim = 1024;
-// Heads that one lane group loads before it computes: with 8 warps of two
-// 16-byte chunks a lane this keeps 8 KB a warp in flight.
-constexpr int kUnroll = 4;
+// Head groups that a warp requests together; the next ones are on the way while
+// these are turned, and the first ones while the angles are computed.
+constexpr int kUnroll = 1;
 
 struct Params {
   const void* in[2];  // queries, keys
@@ -42,7 +42,7 @@ struct Params {
   long long in_ts[2], in_hs[2], in_bs[2];
   long long out_ts[2], out_hs[2], out_bs[2];
   int heads[2];
-  float eps[2];
+  float eps[2], inv_dim;
   int weight_fp32;
   int batch, tokens, dim, rotary;
   int lanes, log2_lanes;  // lanes of a warp for one head (vector kernel)
@@ -54,6 +54,8 @@ struct Params {
   const void* pos;   // null: start + token
   int pos_wide;
   long long pos_as, pos_bs, pos_ts, start;
+  unsigned long long addresses;  // all data pointers and all strides, or-ed (host)
+  long long strides;
 };
 
 // Cosine and sine of every rotated pair of one token into this warp's slab.
@@ -75,89 +77,87 @@ __device__ __forceinline__ void angles(const Params& p, int b, int tok, int lane
   __syncwarp();
 }
 
+// One value, and 32-bit words of one or two values, as floats.
 template <typename T>
-struct Vec;  // 16 bytes of T as floats
+struct Value;
 template <>
-struct Vec<__nv_bfloat16> {
-  static constexpr int kN = 8;
-  static __device__ __forceinline__ void unpack(const uint4& v, float* f) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+struct Value<__nv_bfloat16> {
+  static constexpr int kPerWord = 2;
+  static __device__ __forceinline__ void unpack(uint32_t w, float* f) {
+    f[0] = __uint_as_float(w << 16);
+    f[1] = __uint_as_float(w & 0xffff0000u);
   }
-  static __device__ __forceinline__ uint4 pack(const float* f) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+  static __device__ __forceinline__ uint32_t pack(const float* f) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(f[0], f[1]);
+    return *reinterpret_cast<const uint32_t*>(&h);
   }
   static __device__ __forceinline__ float one(__nv_bfloat16 x) { return __bfloat162float(x); }
   static __device__ __forceinline__ __nv_bfloat16 round(float x) { return __float2bfloat16(x); }
 };
 template <>
-struct Vec<__half> {
-  static constexpr int kN = 8;
-  static __device__ __forceinline__ void unpack(const uint4& v, float* f) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      f[2 * i] = h.x;
-      f[2 * i + 1] = h.y;
-    }
+struct Value<__half> {
+  static constexpr int kPerWord = 2;
+  static __device__ __forceinline__ void unpack(uint32_t w, float* f) {
+    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    f[0] = h.x;
+    f[1] = h.y;
   }
-  static __device__ __forceinline__ uint4 pack(const float* f) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+  static __device__ __forceinline__ uint32_t pack(const float* f) {
+    const __half2 h = __floats2half2_rn(f[0], f[1]);
+    return *reinterpret_cast<const uint32_t*>(&h);
   }
   static __device__ __forceinline__ float one(__half x) { return __half2float(x); }
   static __device__ __forceinline__ __half round(float x) { return __float2half_rn(x); }
 };
 template <>
-struct Vec<float> {
-  static constexpr int kN = 4;
-  static __device__ __forceinline__ void unpack(const uint4& v, float* f) {
-    f[0] = __uint_as_float(v.x);
-    f[1] = __uint_as_float(v.y);
-    f[2] = __uint_as_float(v.z);
-    f[3] = __uint_as_float(v.w);
-  }
-  static __device__ __forceinline__ uint4 pack(const float* f) {
-    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
-                      __float_as_uint(f[3]));
-  }
+struct Value<float> {
+  static constexpr int kPerWord = 1;
+  static __device__ __forceinline__ void unpack(uint32_t w, float* f) { f[0] = __uint_as_float(w); }
+  static __device__ __forceinline__ uint32_t pack(const float* f) { return __float_as_uint(f[0]); }
   static __device__ __forceinline__ float one(float x) { return x; }
   static __device__ __forceinline__ float round(float x) { return x; }
 };
 
-// Weights of channels [c, c + kN) of one norm.
-template <typename T>
+// A chunk of N values, read and written at once.
+template <typename T, int N>
+struct __align__(sizeof(T) * N) Chunk {
+  static constexpr int kWords = N / Value<T>::kPerWord;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0u;
+  }
+  __device__ __forceinline__ void unpack(float* f) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) Value<T>::unpack(w[i], f + i * Value<T>::kPerWord);
+  }
+  __device__ __forceinline__ void pack(const float* f) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = Value<T>::pack(f + i * Value<T>::kPerWord);
+  }
+};
+
+// Weights of channels [c, c + N) of one norm.
+template <typename T, int N>
 __device__ __forceinline__ void load_weight(const Params& p, int which, int c, float* w) {
-  constexpr int N = Vec<T>::kN;
   if (p.weight_fp32) {
 #pragma unroll
     for (int i = 0; i < N; ++i) w[i] = static_cast<const float*>(p.weight[which])[c + i];
   } else {
     const T* base = static_cast<const T*>(p.weight[which]) + c;
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = Vec<T>::one(base[i]);
+    for (int i = 0; i < N; ++i) w[i] = Value<T>::one(base[i]);
   }
 }
 
-template <typename T, bool kNorm, bool kInterleaved>
-__global__ void __launch_bounds__(32 * kWarps) head_rotary_kernel(const Params p) {
-  constexpr int N = Vec<T>::kN;  // channels of a 16-byte chunk
+// N: channels of a chunk (16 bytes).  32 warps a multiprocessor hold the rotation
+// (64 registers; 6.5 TB/s), 24 the norm with it (80 registers, a lane's
+// coefficients double; 5.1 TB/s).  Two head groups at a time, more or fewer warps,
+// larger blocks, and 8-byte chunks for the norm (265 us, twice the sums to wait
+// for) were slower at 2 x 32640 tokens x 64 heads x 64.
+template <typename T, int N, bool kNorm, bool kInterleaved>
+__global__ void __launch_bounds__(32 * kWarps, kNorm ? 6 : 8) head_rotary_kernel(const Params p) {
+  using V = Chunk<T, N>;
   extern __shared__ float2 slabs[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long item = static_cast<long long>(blockIdx.x) * kWarps + warp;
@@ -166,8 +166,6 @@ __global__ void __launch_bounds__(32 * kWarps) head_rotary_kernel(const Params p
   const int part = static_cast<int>(item - token * p.chunks);
   const int b = static_cast<int>(token / p.tokens);
   const int tok = static_cast<int>(token - static_cast<long long>(b) * p.tokens);
-  float2* slab = slabs + warp * (p.rotary / 2);
-  angles(p, b, tok, lane, slab);
 
   // This lane's two chunks of every head it meets.
   const int sub = lane & (p.lanes - 1), slot = lane >> p.log2_lanes, per = 32 >> p.log2_lanes;
@@ -180,82 +178,123 @@ __global__ void __launch_bounds__(32 * kWarps) head_rotary_kernel(const Params p
     c1 = p.rotary / 2 + N * sub;
   }
   const bool has0 = c0 < p.dim, has1 = c1 < p.dim;
-  const bool turn0 = c0 < p.rotary, turn1 = c1 < p.rotary;
-  float2 cs[N];  // of this lane's N pairs
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    cs[i] = make_float2(1.f, 0.f);
-    if (kInterleaved) {
-      const int c = i < N / 2 ? c0 : c1;
-      if (c < p.rotary) cs[i] = slab[c / 2 + (i & (N / 2 - 1))];
-    } else if (turn0) {
-      cs[i] = slab[c0 + i];
-    }
-  }
-
   const int first = part * p.chunk, last = min(first + p.chunk, p.iters[0] + p.iters[1]);
-#pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
-    const int lo = max(first - (which ? p.iters[0] : 0), 0);
-    const int hi = min(last - (which ? p.iters[0] : 0), p.iters[which]);
-    if (lo >= hi) continue;
+  // Head group i of queries, then keys: its tensor and this lane's head.
+  auto place = [&](int i, int& which, int& head) {
+    which = i >= p.iters[0];
+    head = (which ? i - p.iters[0] : i) * per + slot;
+  };
+  auto request = [&](int it, V (&v0)[kUnroll], V (&v1)[kUnroll]) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      v0[u].clear();
+      v1[u].clear();
+      int which, head;
+      place(it + u, which, head);
+      if (it + u < last && head < p.heads[which]) {
+        const T* src = static_cast<const T*>(p.in[which]) + b * p.in_bs[which] +
+                       tok * p.in_ts[which] + head * p.in_hs[which];
+        if (has0) v0[u] = *reinterpret_cast<const V*>(src + c0);
+        if (has1) v1[u] = *reinterpret_cast<const V*>(src + c1);
+      }
+    }
+  };
+  V va0[kUnroll], va1[kUnroll], vb0[kUnroll], vb1[kUnroll];
+  request(first, va0, va1);
+
+  float2* slab = slabs + warp * (p.rotary / 2);
+  angles(p, b, tok, lane, slab);
+  // Of this lane's N pairs (a, d): a' = a ca - d sd, d' = a sa + d cd, with the
+  // norm's weights of their channels multiplied in (plain channels: 1, 0, 0, 1).
+  float ca[N], sd[kNorm ? N : 1], sa[N], cd[kNorm ? N : 1];
+  auto coefficients = [&](int which) {
     float w[2 * N];
     if (kNorm) {
 #pragma unroll
       for (int i = 0; i < 2 * N; ++i) w[i] = 1.f;
       if (p.weight[which] != nullptr) {
-        if (has0) load_weight<T>(p, which, c0, w);
-        if (has1) load_weight<T>(p, which, c1, w + N);
+        if (has0) load_weight<T, N>(p, which, c0, w);
+        if (has1) load_weight<T, N>(p, which, c1, w + N);
       }
     }
-    const T* src = static_cast<const T*>(p.in[which]) + b * p.in_bs[which] + tok * p.in_ts[which];
-    T* dst = static_cast<T*>(p.out[which]) + b * p.out_bs[which] + tok * p.out_ts[which];
-    const long long in_hs = p.in_hs[which], out_hs = p.out_hs[which];
-    const int heads = p.heads[which];
-#pragma unroll 1
-    for (int it = lo; it < hi; it += kUnroll) {
-      uint4 v0[kUnroll], v1[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int head = (it + u) * per + slot;
-        v0[u] = v1[u] = make_uint4(0u, 0u, 0u, 0u);
-        if (it + u < hi && head < heads) {
-          if (has0) v0[u] = *reinterpret_cast<const uint4*>(src + head * in_hs + c0);
-          if (has1) v1[u] = *reinterpret_cast<const uint4*>(src + head * in_hs + c1);
-        }
+    for (int i = 0; i < N; ++i) {
+      float2 cs = make_float2(1.f, 0.f);
+      if (kInterleaved) {
+        const int c = i < N / 2 ? c0 : c1;
+        if (c < p.rotary) cs = slab[c / 2 + (i & (N / 2 - 1))];
+      } else if (c0 < p.rotary) {
+        cs = slab[c0 + i];
+      }
+      ca[i] = cs.x;
+      sa[i] = cs.y;
+      if (kNorm) {
+        const float wa = w[kInterleaved ? 2 * i : i], wd = w[kInterleaved ? 2 * i + 1 : N + i];
+        ca[i] = cs.x * wa;
+        sa[i] = cs.y * wa;
+        cd[i] = cs.x * wd;
+        sd[i] = cs.y * wd;
+      }
+    }
+  };
+  int have = -1;
+  auto turn = [&](int it, const V (&v0)[kUnroll], const V (&v1)[kUnroll]) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (it + u >= last) break;  // the same for the whole warp
+      int which, head;
+      place(it + u, which, head);
+      if (kNorm ? which != have : have < 0) {
+        coefficients(which);
+        have = which;
+      }
+      float x[2 * N];
+      v0[u].unpack(x);
+      v1[u].unpack(x + N);
+      float r = 1.f;
+      if (kNorm) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2 * N; ++i) sum = fmaf(x[i], x[i], sum);
+        for (int d = 1; d < p.lanes; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        r = rsqrtf(fmaf(sum, p.inv_dim, p.eps[which]));
       }
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int head = (it + u) * per + slot;
-        if (it + u >= hi) break;  // the same for the whole warp
-        float x[2 * N];
-        Vec<T>::unpack(v0[u], x);
-        Vec<T>::unpack(v1[u], x + N);
+      for (int i = 0; i < N; ++i) {
+        float& a = kInterleaved ? x[2 * i] : x[i];
+        float& d = kInterleaved ? x[2 * i + 1] : x[N + i];
         if (kNorm) {
-          float sum = 0.f;
-#pragma unroll
-          for (int i = 0; i < 2 * N; ++i) sum = fmaf(x[i], x[i], sum);
-          for (int d = 1; d < p.lanes; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-          const float r = rsqrtf(sum / static_cast<float>(p.dim) + p.eps[which]);
-#pragma unroll
-          for (int i = 0; i < 2 * N; ++i) x[i] = x[i] * r * w[i];
+          a *= r;
+          d *= r;
         }
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          float& a = kInterleaved ? x[2 * i] : x[i];
-          float& d = kInterleaved ? x[2 * i + 1] : x[N + i];
-          if (kInterleaved ? (i < N / 2 ? turn0 : turn1) : turn0) {
-            const float a0 = a, d0 = d;
-            a = a0 * cs[i].x - d0 * cs[i].y;
-            d = a0 * cs[i].y + d0 * cs[i].x;
-          }
-        }
-        if (head < heads) {
-          if (has0) *reinterpret_cast<uint4*>(dst + head * out_hs + c0) = Vec<T>::pack(x);
-          if (has1) *reinterpret_cast<uint4*>(dst + head * out_hs + c1) = Vec<T>::pack(x + N);
+        // channels that are not turned pass as they are (0 * inf is NaN)
+        const bool turned = kInterleaved ? (i < N / 2 ? c0 : c1) < p.rotary : c0 < p.rotary;
+        const float a0 = a, d0 = d;
+        if (turned) {
+          a = a0 * ca[i] - d0 * (kNorm ? sd[kNorm ? i : 0] : sa[i]);
+          d = a0 * sa[i] + d0 * (kNorm ? cd[kNorm ? i : 0] : ca[i]);
+        } else if (kNorm) {
+          a = a0 * ca[i];
+          d = d0 * cd[kNorm ? i : 0];
         }
       }
+      if (head < p.heads[which]) {
+        T* dst = static_cast<T*>(p.out[which]) + b * p.out_bs[which] + tok * p.out_ts[which] +
+                 head * p.out_hs[which];
+        V y;
+        y.pack(x);
+        if (has0) *reinterpret_cast<V*>(dst + c0) = y;
+        y.pack(x + N);
+        if (has1) *reinterpret_cast<V*>(dst + c1) = y;
+      }
     }
+  };
+#pragma unroll 1
+  for (int it = first; it < last; it += 2 * kUnroll) {
+    request(it + kUnroll, vb0, vb1);
+    turn(it, va0, va1);
+    request(it + 2 * kUnroll, va0, va1);
+    turn(it + kUnroll, vb0, vb1);
   }
 }
 
@@ -287,19 +326,19 @@ __global__ void __launch_bounds__(32 * kWarps) head_rotary_scalar_kernel(const P
     if (kNorm) {
       float sum = 0.f;
       for (int c = lane; c < p.dim; c += 32) {
-        const float x = Vec<T>::one(src[c]);
+        const float x = Value<T>::one(src[c]);
         sum = fmaf(x, x, sum);
       }
       for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      r = rsqrtf(sum / static_cast<float>(p.dim) + p.eps[which]);
+      r = rsqrtf(fmaf(sum, p.inv_dim, p.eps[which]));
     }
     auto value = [&](int c) {
-      float x = Vec<T>::one(src[c]);
+      float x = Value<T>::one(src[c]);
       if (kNorm) {
         float w = 1.f;
         if (p.weight[which] != nullptr)
           w = p.weight_fp32 ? static_cast<const float*>(p.weight[which])[c]
-                            : Vec<T>::one(static_cast<const T*>(p.weight[which])[c]);
+                            : Value<T>::one(static_cast<const T*>(p.weight[which])[c]);
         x = x * r * w;
       }
       return x;
@@ -308,16 +347,22 @@ __global__ void __launch_bounds__(32 * kWarps) head_rotary_scalar_kernel(const P
       const int a = kInterleaved ? 2 * i : i, d = kInterleaved ? 2 * i + 1 : i + p.rotary / 2;
       const float x0 = value(a), x1 = value(d);
       const float2 cs = slab[i];
-      dst[a] = Vec<T>::round(x0 * cs.x - x1 * cs.y);
-      dst[d] = Vec<T>::round(x0 * cs.y + x1 * cs.x);
+      dst[a] = Value<T>::round(x0 * cs.x - x1 * cs.y);
+      dst[d] = Value<T>::round(x0 * cs.y + x1 * cs.x);
     }
-    for (int c = p.rotary + lane; c < p.dim; c += 32) dst[c] = Vec<T>::round(value(c));
+    for (int c = p.rotary + lane; c < p.dim; c += 32) dst[c] = Value<T>::round(value(c));
   }
 }
 
 template <typename T, bool kNorm, bool kInterleaved>
-int launch(Params p, bool vector, cudaStream_t stream) {
-  constexpr int N = Vec<T>::kN;
+int launch(Params p, cudaStream_t stream) {
+  constexpr int N = static_cast<int>(16 / sizeof(T));
+  // Chunks fit when every head starts on their size, the head is a whole number
+  // of them (at most two a lane) and no chunk holds both turned and other channels
+  // or, in the half layout, channels of both halves.
+  const bool vector = (p.addresses & (N * sizeof(T) - 1)) == 0 && (p.strides & (N - 1)) == 0 &&
+                      p.dim % N == 0 && p.dim <= 64 * N &&
+                      p.rotary % (kInterleaved ? N : 2 * N) == 0;
   if (vector) {
     const int tasks = (p.dim + 2 * N - 1) / (2 * N);
     p.lanes = 1;
@@ -341,7 +386,7 @@ int launch(Params p, bool vector, cudaStream_t stream) {
   if (blocks > 0x7fffffffLL) return kErrTooLarge;
   const size_t smem = static_cast<size_t>(kWarps) * (p.rotary / 2) * sizeof(float2);
   if (vector)
-    head_rotary_kernel<T, kNorm, kInterleaved>
+    head_rotary_kernel<T, N, kNorm, kInterleaved>
         <<<static_cast<unsigned>(blocks), 32 * kWarps, smem, stream>>>(p);
   else
     head_rotary_scalar_kernel<T, kNorm, kInterleaved>
@@ -350,12 +395,9 @@ int launch(Params p, bool vector, cudaStream_t stream) {
 }
 
 template <typename T>
-int dispatch(const Params& p, bool norm, bool interleaved, bool vector, cudaStream_t stream) {
-  if (norm)
-    return interleaved ? launch<T, true, true>(p, vector, stream)
-                       : launch<T, true, false>(p, vector, stream);
-  return interleaved ? launch<T, false, true>(p, vector, stream)
-                     : launch<T, false, false>(p, vector, stream);
+int dispatch(const Params& p, bool norm, bool interleaved, cudaStream_t stream) {
+  if (norm) return interleaved ? launch<T, true, true>(p, stream) : launch<T, true, false>(p, stream);
+  return interleaved ? launch<T, false, true>(p, stream) : launch<T, false, false>(p, stream);
 }
 
 }  // namespace rot
@@ -405,6 +447,7 @@ extern "C" int erd_head_norm_rotary(const erd_head_norm_rotary_args* args, void*
   p.batch = a.batch;
   p.tokens = a.tokens;
   p.dim = a.head_dim;
+  p.inv_dim = 1.0f / static_cast<float>(a.head_dim);
   p.rotary = a.rotary_dim;
   p.turns = a.turns;
   p.amplitude = a.amplitude;
@@ -417,21 +460,15 @@ extern "C" int erd_head_norm_rotary(const erd_head_norm_rotary_args* args, void*
   p.pos_bs = a.pos_stride[1];
   p.pos_ts = a.pos_stride[2];
   p.start = a.start;
-  // Chunks of 16 bytes fit when every head starts on 16 bytes, the head is a
-  // whole number of chunks (at most two a lane) and no chunk holds both turned
-  // and other channels or, in the half layout, channels of both halves.
-  const int n = static_cast<int>(16 / elem);
-  int64_t strides = 0;
+  p.addresses = all;
   for (int i = 0; i < 3; ++i) {
-    strides |= a.q_stride[i] | a.q_out_stride[i];
-    if (a.k_heads > 0) strides |= a.k_stride[i] | a.k_out_stride[i];
+    p.strides |= a.q_stride[i] | a.q_out_stride[i];
+    if (a.k_heads > 0) p.strides |= a.k_stride[i] | a.k_out_stride[i];
   }
-  const bool vector = (all & 15) == 0 && (strides & (n - 1)) == 0 && a.head_dim % n == 0 &&
-                      a.head_dim <= 64 * n && a.rotary_dim % (a.interleaved ? n : 2 * n) == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (a.dtype) {
-    case ERD_BF16: return rot::dispatch<__nv_bfloat16>(p, a.norm, a.interleaved, vector, st);
-    case ERD_FP16: return rot::dispatch<__half>(p, a.norm, a.interleaved, vector, st);
-    default: return rot::dispatch<float>(p, a.norm, a.interleaved, vector, st);
+    case ERD_BF16: return rot::dispatch<__nv_bfloat16>(p, a.norm, a.interleaved, st);
+    case ERD_FP16: return rot::dispatch<__half>(p, a.norm, a.interleaved, st);
+    default: return rot::dispatch<float>(p, a.norm, a.interleaved, st);
   }
 }

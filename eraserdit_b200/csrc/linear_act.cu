@@ -7,12 +7,13 @@
 // Three kernels, chosen by the host:
 //   row_kernel    up to two rows: FP32 products of W's stream, no tensor cores.
 //   pair_kernel   large products.  A persistent kernel of CTA pairs
-//                 (cta_group::2), one 256 x 256 (or 256 x 128) tile a pair: each
-//                 CTA stages 128 rows of x and half of W's tile, so an
-//                 instruction reads W from both shared memories and a CTA loads
-//                 32 KB per 64-deep step for 128 x 256 outputs.  An accumulator
-//                 is 256 TMEM columns, so two fit, and the epilogue of a tile
-//                 runs beside the products of the next.
+//                 (cta_group::2), one 256 x 256 tile a pair: each CTA stages 128
+//                 rows of x and half of W's tile, so an instruction reads W from
+//                 both shared memories and a CTA loads 32 KB per 64-deep step
+//                 for 128 x 256 outputs.  An accumulator is 256 TMEM columns, so
+//                 two fit, and the epilogue of a tile runs beside the products of
+//                 the next.  Where the last round of tiles would leave more than
+//                 half of the pairs idle, its tiles are cut into 256 x 128.
 //   split_kernel  few tiles (short row counts, narrow outputs).  One 128 x 64
 //                 or 128 x 128 tile a CTA, the reduction split over the CTAs of
 //                 a cluster, whose FP32 partial sums are added through
@@ -440,70 +441,76 @@ constexpr int kPairEpilogueWarps = 8;
 constexpr int kPairThreads = 32 * (2 + kPairEpilogueWarps);
 constexpr int kPairRows = 256;                      // rows of a pair's tile
 constexpr int kPairABytes = 128 * kRowBytes;        // x of one CTA and stage
-constexpr int kPairMaxStages = 7;
+constexpr int kPairStages = 5;
+constexpr int kPairBBytes = 128 * kRowBytes;        // W of one CTA and stage (wide tile)
 
 struct __align__(8) PairBarriers {
-  uint64_t full[kPairMaxStages];   // the leader's: bytes of both CTAs
-  uint64_t empty[kPairMaxStages];  // each CTA's own
-  uint64_t acc_full[2];            // each CTA's own
-  uint64_t acc_empty[2];           // the leader's: every epilogue warp of both CTAs
+  uint64_t full[kPairStages];   // the leader's: bytes of both CTAs
+  uint64_t empty[kPairStages];  // each CTA's own
+  uint64_t acc_full[2];         // each CTA's own
+  uint64_t acc_empty[2];        // the leader's: every epilogue warp of both CTAs
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
 };
 
-// Tiles of 256 columns, or of 128 where those end in a nearly empty wave.
-template <int BN>
-struct PairTile {
-  static constexpr int kBBytes = BN / 2 * kRowBytes;  // W of one CTA and stage
-  static constexpr int kStages = BN == 256 ? 5 : 7;
-  static constexpr int kPieces = BN / 2 / 64;         // of an epilogue warp
-  static constexpr int kSmemA = 0;
-  static constexpr int kSmemB = kSmemA + kStages * kPairABytes;
-  static constexpr int kSmemStage = kSmemB + kStages * kBBytes;
-  static constexpr int kSmemSlab = kSmemStage + kPairEpilogueWarps * kStageBytes;
-  static constexpr int kSmemBar = kSmemSlab + kPairEpilogueWarps * kSlabBytes;
-  static constexpr int kSmemLaunch = kSmemBar + 1024 + 1024;  // + base alignment
-  static_assert(kSmemLaunch <= 227 * 1024 && kStages <= kPairMaxStages, "shared memory budget");
-};
+constexpr int kPairSmemA = 0;
+constexpr int kPairSmemB = kPairSmemA + kPairStages * kPairABytes;
+constexpr int kPairSmemStage = kPairSmemB + kPairStages * kPairBBytes;
+constexpr int kPairSmemSlab = kPairSmemStage + kPairEpilogueWarps * kStageBytes;
+constexpr int kPairSmemBar = kPairSmemSlab + kPairEpilogueWarps * kSlabBytes;
+constexpr int kPairSmemLaunch = kPairSmemBar + 1024 + 1024;  // + base alignment
+static_assert(kPairSmemLaunch <= 227 * 1024, "shared memory budget");
 
 struct PairParams {
   Epilogue e;
   int k, tiles_m, tiles_n;
+  int wide;   // tiles that are taken whole
+  int items;  // these and the halves of the others
   int* status;
 };
 
-// Tiles in the order the pairs take them: bands of kBand tile rows, column by
-// column within a band, so that the tiles in flight form a block that reads
-// few distinct rows of x and of W.
+// The tile of an item: its first row and column, and whether it is 256 or 128
+// columns wide.  Pairs take tiles in bands of kBand tile rows, column by column
+// within a band, so that the tiles in flight form a block that reads few distinct
+// rows of x and of W.
 constexpr int kBand = 8;
-__device__ __forceinline__ void tile_place(const PairParams& p, int tile, int& tm, int& tn) {
+struct PairTile {
+  int m0, n0;
+  bool wide;
+};
+__device__ __forceinline__ PairTile pair_tile(const PairParams& p, int item) {
+  const bool wide = item < p.wide;
+  const int tile = wide ? item : p.wide + ((item - p.wide) >> 1);
   const int band = tile / (kBand * p.tiles_n);
   const int rows = min(kBand, p.tiles_m - band * kBand);
   const int r = tile - band * kBand * p.tiles_n;
-  tn = r / rows;
-  tm = band * kBand + r - tn * rows;
+  const int tn = r / rows;
+  PairTile t;
+  t.wide = wide;
+  t.m0 = (band * kBand + r - tn * rows) * kPairRows;
+  t.n0 = tn * 256 + (wide ? 0 : ((item - p.wide) & 1) * 128);
+  return t;
 }
 
-template <typename T, bool kBf16, int BN>
+template <typename T, bool kBf16>
 __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
-                const __grid_constant__ CUtensorMap tmap_b, const PairParams p) {
-  using P = PairTile<BN>;
+                const __grid_constant__ CUtensorMap tmap_b,
+                const __grid_constant__ CUtensorMap tmap_b_half, const PairParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  PairBarriers* bars = reinterpret_cast<PairBarriers*>(smem + P::kSmemBar);
-  const uint32_t sA = smem_u32(smem + P::kSmemA);
-  const uint32_t sB = smem_u32(smem + P::kSmemB);
+  PairBarriers* bars = reinterpret_cast<PairBarriers*>(smem + kPairSmemBar);
+  const uint32_t sA = smem_u32(smem + kPairSmemA);
+  const uint32_t sB = smem_u32(smem + kPairSmemB);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int tiles = p.tiles_m * p.tiles_n;
   volatile int* abort = &bars->abort;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < P::kStages; ++s) {
+    for (int s = 0; s < kPairStages; ++s) {
       mbar_init(smem_u32(&bars->full[s]), 1);
       mbar_init(smem_u32(&bars->empty[s]), 1);
     }
@@ -516,7 +523,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc_pair(smem_u32(&bars->tmem_base), 2 * BN);
+    tmem_alloc_pair(smem_u32(&bars->tmem_base), 512);
     tmem_relinquish_pair();
   }
   tc_fence_before();
@@ -529,16 +536,18 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     if (elect_one()) {
       tma_prefetch_desc(&tmap_a);
       tma_prefetch_desc(&tmap_b);
+      if (p.items > p.wide) tma_prefetch_desc(&tmap_b_half);
       RingPlace at;
       uint32_t issued = 0;
       bool ok = true;
       const uint32_t full0 = smem_u32(&bars->full[0]), empty0 = smem_u32(&bars->empty[0]);
       const uint32_t leader0 = map_rank(full0, 0);
-      for (int tile = pair; ok && tile < tiles; tile += pairs) {
-        int tm, tn;
-        tile_place(p, tile, tm, tn);
-        const int m0 = tm * kPairRows + static_cast<int>(rank) * 128;
-        const int n0 = tn * BN + static_cast<int>(rank) * (BN / 2);
+      for (int item = pair; ok && item < p.items; item += pairs) {
+        const PairTile t = pair_tile(p, item);
+        const int m0 = t.m0 + static_cast<int>(rank) * 128;
+        const int n0 = t.n0 + static_cast<int>(rank) * (t.wide ? 128 : 64);
+        const CUtensorMap* map_w = t.wide ? &tmap_b : &tmap_b_half;
+        const uint32_t bytes = 2 * (kPairABytes + (t.wide ? kPairBBytes : kPairBBytes / 2));
         for (int k0 = 0; k0 < p.k; k0 += kBK) {
           if (!mbar_wait(empty0 + 8 * at.s, at.phase ^ 1, abort, p.status,
                          kStatusTimeoutProducer)) {
@@ -547,18 +556,18 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
           }
           // The leader announces the bytes of both CTAs.  The other CTA's may
           // land first: the phase cannot end before the leader's arrival.
-          if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * at.s, 2 * (kPairABytes + P::kBBytes));
+          if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * at.s, bytes);
           const uint32_t bar = leader0 + 8 * at.s;
           tma_load_2d_pair(sA + at.s * kPairABytes, &tmap_a, bar, k0, m0);
-          tma_load_2d_pair(sB + at.s * P::kBBytes, &tmap_b, bar, k0, n0);
-          at.next(P::kStages);
+          tma_load_2d_pair(sB + at.s * kPairBBytes, map_w, bar, k0, n0);
+          at.next(kPairStages);
           ++issued;
         }
       }
       if (*abort && rank == 0) {
         // Let the loads that may be in flight land before exiting.
-        for (uint32_t d = 0; d < P::kStages && d < issued; ++d) {
-          at.back(P::kStages);
+        for (uint32_t d = 0; d < kPairStages && d < issued; ++d) {
+          at.back(kPairStages);
           mbar_wait_drain(full0 + 8 * at.s, at.phase);
         }
       }
@@ -566,7 +575,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   } else if (warp == 1) {
     // ------------------------------------------------- MMA issuer (the leader)
     if (rank == 0 && elect_one()) {
-      constexpr uint32_t id = idesc<kBf16>(256, BN);
       // Descriptors of stage 0; a stage or 32 bytes of K further is an addition
       // to the address field (16-byte units).
       const uint64_t da0 = sdesc_sw128(sA, 16, 1024), db0 = sdesc_sw128(sB, 16, 1024);
@@ -574,7 +582,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       RingPlace at;
       uint32_t count = 0;
       bool ok = true;
-      for (int tile = pair; ok && tile < tiles; tile += pairs, ++count) {
+      for (int item = pair; ok && item < p.items; item += pairs, ++count) {
+        const uint32_t id = item < p.wide ? idesc<kBf16>(256, 256) : idesc<kBf16>(256, 128);
         const uint32_t buf = count & 1;
         if (!mbar_wait(smem_u32(&bars->acc_empty[buf]), ((count >> 1) & 1) ^ 1, abort, p.status,
                        kStatusTimeoutMma)) {
@@ -582,7 +591,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
           break;
         }
         tc_fence_after();
-        const uint32_t d = tmem + buf * BN;
+        const uint32_t d = tmem + buf * 256;
         uint32_t acc = 0;
         for (int k0 = 0; k0 < p.k; k0 += kBK) {
           if (!mbar_wait(full0 + 8 * at.s, at.phase, abort, p.status, kStatusTimeoutMma)) {
@@ -591,14 +600,14 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
           }
           tc_fence_after();
           const uint64_t da = da0 + at.s * (kPairABytes / 16);
-          const uint64_t db = db0 + at.s * (P::kBBytes / 16);
+          const uint64_t db = db0 + at.s * (kPairBBytes / 16);
 #pragma unroll
           for (int k4 = 0; k4 < 4; ++k4) {
             mma_pair_ss(d, da + 2 * k4, db + 2 * k4, id, acc);
             acc = 1;
           }
           mma_commit_pair(empty0 + 8 * at.s);
-          at.next(P::kStages);
+          at.next(kPairStages);
         }
         if (!ok) break;
         mma_commit_pair(smem_u32(&bars->acc_full[buf]));
@@ -610,41 +619,43 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   } else {
     // ------------------------------------------------------------ epilogue
     const int w = warp - 2, quad = warp & 3, half = w >> 2;
-    uint8_t* stage = smem + P::kSmemStage + w * kStageBytes;
-    float* slab = reinterpret_cast<float*>(smem + P::kSmemSlab + w * kSlabBytes);
-    // This warp's corner of a tile; pieces without rows or columns are skipped.
-    auto corner = [&](int tile, int& row0, int& col0) {
-      int tm, tn;
-      tile_place(p, tile, tm, tn);
-      row0 = tm * kPairRows + static_cast<int>(rank) * 128 + quad * 32;
-      col0 = tn * BN + half * (BN / 2);
+    uint8_t* stage = smem + kPairSmemStage + w * kStageBytes;
+    float* slab = reinterpret_cast<float*>(smem + kPairSmemSlab + w * kSlabBytes);
+    // This warp's corner of a tile: 32 rows, half of the columns.  Pieces without
+    // rows or columns are skipped.
+    PairTile t;
+    int row0, col0;
+    auto corner = [&](int item) {
+      t = pair_tile(p, item);
+      row0 = t.m0 + static_cast<int>(rank) * 128 + quad * 32;
+      col0 = t.n0 + half * (t.wide ? 128 : 64);
     };
     Piece<T> piece;
-    int row0, col0;
-    if (pair < tiles) {
-      corner(pair, row0, col0);
+    if (pair < p.items) {
+      corner(pair);
       if (row0 < p.e.m && col0 < p.e.n) piece.request(p.e, row0, col0, lane);
     }
     uint32_t count = 0;
-    for (int tile = pair; tile < tiles; tile += pairs, ++count) {
+    for (int item = pair; item < p.items; item += pairs, ++count) {
       const uint32_t buf = count & 1;
       if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->acc_full[buf]), (count >> 1) & 1,
                                              abort, p.status, kStatusTimeoutEpilogue)))
         break;
       tc_fence_after();
-      const uint32_t taddr =
-          tmem + (static_cast<uint32_t>(quad * 32) << 16) + buf * BN + half * (BN / 2);
+      const int pieces = t.wide ? 2 : 1;
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16) + buf * 256 +
+                             half * (t.wide ? 128 : 64);
 #pragma unroll 1
-      for (int c = 0; c < P::kPieces; ++c) {
+      for (int c = 0; c < pieces; ++c) {
         const bool any = row0 < p.e.m && col0 + c * kPiece < p.e.n;
         const int row = row0, col = col0 + c * kPiece;
         const bool inside = piece.inside, one_group = piece.one_group;
         const int group = piece.group;
         if (any) piece.park(p.e, stage, slab, lane);
         // the next piece, of this tile or the next
-        const bool last = c == P::kPieces - 1;
-        if (last && tile + pairs < tiles) corner(tile + pairs, row0, col0);
-        if (!last || tile + pairs < tiles) {
+        const bool last = c == pieces - 1;
+        if (last && item + pairs < p.items) corner(item + pairs);
+        if (!last || item + pairs < p.items) {
           const int next = col0 + (last ? 0 : kPiece);
           if (row0 < p.e.m && next < p.e.n) piece.request(p.e, row0, next, lane);
         }
@@ -662,7 +673,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc_pair(tmem, 2 * BN);
+    tmem_dealloc_pair(tmem, 512);
   }
 }
 
@@ -1078,8 +1089,8 @@ struct Plan {
 
 // Which kernel for more than kRowMax rows, and how a small product is cut: the
 // least estimated time, in clocks, of
-//   the pair kernel: 512 (256 columns) or 400 a 64-deep step and tile, whole waves
-//   of sms / 2 tiles;
+//   the pair kernel: 512 a 64-deep step and round of sms / 2 tiles, 300 for a last
+//   round of half tiles;
 //   the split kernel with 64 or 128 columns and 1, 2 or 4 parts, one wave of CTAs
 //   (its steps wait for L2, and parts add a round trip through the cluster).
 Plan pick_plan(int m, int n, int k, int sms) {
@@ -1094,9 +1105,11 @@ Plan pick_plan(int m, int n, int k, int sms) {
     best.bn = bn;
     best.splits = splits;
   };
-  for (int bn = 256; bn >= 128; bn -= 128) {
-    const long long tiles = ((m + 255LL) / 256) * ((n + bn - 1LL) / bn);
-    offer(true, bn, 1, waves(tiles, sms / 2) * ksteps * (bn == 256 ? 512 : 400) + 9000);
+  {
+    const long long tiles = ((m + 255LL) / 256) * ((n + 255LL) / 256), pairs = sms / 2;
+    const long long whole = tiles / pairs, rest = tiles % pairs;
+    const long long last = rest == 0 ? 0 : 2 * rest <= pairs ? 300 : 512;
+    offer(true, 256, 1, ksteps * (whole * 512 + last) + 9000);
   }
   for (int bn = 64; bn <= 128; bn += 64) {
     const long long tiles = ((m + 127LL) / 128) * ((n + bn - 1LL) / bn);
@@ -1112,20 +1125,23 @@ Plan pick_plan(int m, int n, int k, int sms) {
   return best;
 }
 
-template <typename T, bool kBf16, int BN>
-int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, PairParams p, int sms,
-                cudaStream_t st) {
-  using P = PairTile<BN>;
-  const long long tm = (p.e.m + 255LL) / 256, tn = (p.e.n + BN - 1LL) / BN;
-  if (tm * tn > (1LL << 30)) return kErrTooLarge;
+template <typename T, bool kBf16>
+int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb_half,
+                PairParams p, int sms, cudaStream_t st) {
+  const long long tm = (p.e.m + 255LL) / 256, tn = (p.e.n + 255LL) / 256, tiles = tm * tn;
+  if (tiles > (1LL << 29)) return kErrTooLarge;
+  const int pairs = sms / 2;
+  const int rest = static_cast<int>(tiles % pairs);
   p.tiles_m = static_cast<int>(tm);
   p.tiles_n = static_cast<int>(tn);
-  cudaError_t e = cudaFuncSetAttribute(pair_kernel<T, kBf16, BN>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, P::kSmemLaunch);
+  p.wide = static_cast<int>(tiles) - (2 * rest <= pairs ? rest : 0);
+  p.items = p.wide + 2 * (static_cast<int>(tiles) - p.wide);
+  cudaError_t e = cudaFuncSetAttribute(pair_kernel<T, kBf16>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemLaunch);
   if (e != cudaSuccess) return static_cast<int>(e);
-  const long long pairs = tm * tn < sms / 2 ? tm * tn : sms / 2;
-  pair_kernel<T, kBf16, BN>
-      <<<static_cast<unsigned>(2 * pairs), kPairThreads, P::kSmemLaunch, st>>>(ta, tb, p);
+  const int used = p.items < pairs ? p.items : pairs;
+  pair_kernel<T, kBf16><<<static_cast<unsigned>(2 * used), kPairThreads, kPairSmemLaunch, st>>>(
+      ta, tb, tb_half, p);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -1209,12 +1225,13 @@ int run(const Epilogue& e, const void* x, int64_t ldx, const void* w, int64_t ld
   const Plan pl = pick_plan(e.m, e.n, k, sms);
   CUtensorMap ta, tb;
   if (pl.pair) {
+    CUtensorMap tb_half;
     if (operand_map(&ta, kBf16, x, e.m, k, ldx, 128) ||
-        operand_map(&tb, kBf16, w, e.n, k, ldw, pl.bn / 2))
+        operand_map(&tb, kBf16, w, e.n, k, ldw, 128) ||
+        operand_map(&tb_half, kBf16, w, e.n, k, ldw, 64))
       return kErrTensorMap;
-    const PairParams p = {e, k, 0, 0, status};
-    return pl.bn == 256 ? launch_pair<T, kBf16, 256>(ta, tb, p, sms, st)
-                        : launch_pair<T, kBf16, 128>(ta, tb, p, sms, st);
+    const PairParams p = {e, k, 0, 0, 0, 0, status};
+    return launch_pair<T, kBf16>(ta, tb, tb_half, p, sms, st);
   }
   if (operand_map(&ta, kBf16, x, e.m, k, ldx, pl.a_rows) ||
       operand_map(&tb, kBf16, w, e.n, k, ldw, pl.bn))

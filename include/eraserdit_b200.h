@@ -431,8 +431,8 @@ int erd_attn_fwd_fp8_static_scratch(
  * without positions; axis 1 serves the pairs from second_axis on, axis 2 those
  * from third_axis on (set both to rotary_dim / 2 for one axis).
  * Heads that start on 16 bytes and whose turned part is a whole number of
- * 16-byte chunks take 16-byte accesses; any other size or stride is read value
- * by value.
+ * 16-byte chunks take wide accesses; any other size or stride is read value by
+ * value.
  */
 typedef struct {
   int64_t struct_bytes; /* sizeof this struct, checked */
