@@ -178,6 +178,50 @@ def pack(name: str, *fields) -> bytes:
         raise ValueError(f"{name}: {error}") from None
 
 
+def _span(dims) -> int:
+    """Bytes from the first to the end of the last element over (size, byte stride) dims."""
+    return sum((n - 1) * step for n, step in dims)
+
+
+def may_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two strided tensors may share memory.  Tensors whose address ranges
+    interleave (columns of one buffer) are told apart by a stride that both have:
+    modulo it each covers one range."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    sides = []
+    for t in (a, b):
+        size = t.element_size()
+        dims = [(n, step * size) for n, step in zip(t.shape, t.stride()) if n > 1]
+        sides.append((t.data_ptr(), dims, size))
+    (pa, da, sa), (pb, db, sb) = sides
+    if pa + _span(da) + sa <= pb or pb + _span(db) + sb <= pa:
+        return False
+    for period in {step for _, step in da} & {step for _, step in db} - {0}:
+        widths = []
+        for _, dims, size in sides:
+            inner = _span([d for d in dims if d[1] < period]) + size
+            if inner > period or any(step % period for _, step in dims if step >= period):
+                break
+            widths.append(inner)
+        if len(widths) == 2:
+            gap = (pb - pa) % period  # where b's range starts behind a's
+            if gap >= widths[0] and gap + widths[1] <= period:
+                return False
+    return True
+
+
+def refuse_overlap(what: str, out: torch.Tensor, inputs, in_place: torch.Tensor | None = None) -> None:
+    """A caller's destination shares no memory with the inputs; ``in_place``, an input
+    that may be the destination itself (the same elements), shares all or none."""
+    if in_place is not None and not (out.data_ptr() == in_place.data_ptr()
+                                     and out.stride() == in_place.stride()):
+        inputs = (*inputs, in_place)
+    for t in inputs:
+        if t is not None and may_overlap(out, t):
+            raise ValueError(f"{what} overlaps an input")
+
+
 def refuse_gradients(what: str, *tensors) -> None:
     """The operators have no backward pass: an input that wants a gradient while
     gradients are recorded is an error, not a silently detached result."""

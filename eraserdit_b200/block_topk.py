@@ -77,6 +77,7 @@ def pool_key_blocks(key: torch.Tensor, key_block: int = 64, *,
                           dtype=torch.float64)
     else:
         _check_means(out, key, key_block)
+        _native.refuse_overlap("out", out, (key, key_lengths))
     if out.numel():
         _native.call("erd_block_key_means", key.device, _native.DTYPE_CODES[key.dtype],
                      key.data_ptr(), *_strides("key", key), batch, heads, length, key_block,
@@ -97,7 +98,7 @@ def block_topk_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Te
     or FP16.  ``query_block``: 128 or 1 consecutive queries that share a choice;
     ``key_block``: 64 or 128 keys.  ``key_lengths`` (int32 [B] on the device): keys
     from there on are left out, whatever they hold; a sequence without keys gives
-    zeros.  ``key_pool``: ``pool_key_blocks(key, key_block, key_lengths=...)`` that
+    zeros.  ``out`` may be ``query`` itself.  ``key_pool``: ``pool_key_blocks(key, key_block, key_lengths=...)`` that
     the caller keeps, else computed here.  With ``return_selection`` also the chosen
     blocks, int32 [B, H, query blocks, topk], ascending, -1 behind the last.
     """
@@ -128,6 +129,8 @@ def block_topk_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Te
         out = torch.empty_like(query, memory_format=torch.contiguous_format)
     elif out.shape != query.shape or out.dtype != query.dtype or out.device != query.device:
         raise ValueError("out must have the query's shape, type and device")
+    else:
+        _native.refuse_overlap("out", out, (key, value, key_lengths, key_pool), query)
     selection = query.new_empty((batch, heads, groups, topk), dtype=torch.int32)
     if batch and q_len and kv_len:
         nbytes = 0
@@ -135,7 +138,7 @@ def block_topk_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Te
         if key_pool is None or query_block != 1:
             nbytes = int(_native.load().erd_block_topk_workspace_bytes(
                 batch, heads, kv_heads, q_len, kv_len, query_block, key_block,
-                int(key_pool is not None)))
+                key_pool is not None))
             # from torch's allocator, call by call: it follows streams and captures
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
         _native.call("erd_block_topk_attn", device, _native.pack(

@@ -187,6 +187,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
         out = torch.empty(shape, dtype=dtype, device=device)
     elif out.shape != shape or any(s == 0 and d > 1 for s, d in zip(out.stride(), out.shape)):
         raise ValueError("out must be [..., n] and no expanded view")
+    else:
+        _native.refuse_overlap("out", out, (x, weight, bias, gate), residual)
     m = x.numel() // k
     gate_rows = 0
     if gate is not None:
@@ -211,6 +213,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
                        gate=gate[i] if gate is not None and gate.dim() == 2 else gate,
                        residual=None if residual is None else residual[i], out=out[i])
         return out
+    if ldx < k or ldw < k or ldy < n or (residual is not None and ldr < n):
+        raise ValueError("rows must not overlap (an expanded view is given in full)")
     xp, wp = x.data_ptr(), weight.data_ptr()
     if (xp | wp) % 16 or (ldx | ldw) % 8:
         raise ValueError("rows of x and weight must start on 16 bytes (strides multiples of 8)")

@@ -298,3 +298,16 @@ def test_empty_and_refusals():
             block_topk_attention(args["query"], args["key"], args["value"], SCALE, args["topk"], **rest)
     with pytest.raises(ValueError):
         block_topk_attention(q.requires_grad_(), k, v, SCALE, 3)
+
+
+@pytest.mark.parametrize("query_block", [1, 128])
+def test_destination_over_the_queries_but_not_the_keys(query_block):
+    from eraserdit_b200.block_topk import block_topk_attention
+    q, k, v = _inputs(2, 140, 300, 4, 4, torch.bfloat16, 13)
+    want = block_topk_attention(q, k, v, SCALE, 2, query_block=query_block)
+    own = q.clone()
+    assert block_topk_attention(own, k, v, SCALE, 2, query_block=query_block, out=own) is own
+    assert torch.equal(own, want)
+    for out in (k[:, :140], v[:, 20:160]):
+        with pytest.raises(ValueError):
+            block_topk_attention(q, k, v, SCALE, 2, query_block=query_block, out=out)

@@ -323,3 +323,15 @@ def test_offsets_beyond_32_bits():
     _close(got, _want(src, rotary, _pos(2, 4, start=1)))
     del buf, q, got
     torch.cuda.empty_cache()
+
+
+def test_overlapping_destinations_are_refused():
+    from eraserdit_b200.rotary import RotaryPositions, apply_rotary
+    rotary = RotaryPositions(64)
+    buf = _randn((2, 6, 8 * 64), torch.bfloat16, 25)
+    heads = lambda a, b: buf[..., a * 64:b * 64].unflatten(-1, (b - a, 64))
+    apply_rotary(heads(0, 2), heads(2, 4), rotary, 0, query_out=heads(4, 6), key_out=heads(6, 8))
+    for kw in (dict(query_out=heads(1, 3)), dict(query_out=heads(2, 4)), dict(key_out=heads(0, 2)),
+               dict(query_out=heads(4, 6), key_out=heads(5, 7))):
+        with pytest.raises(ValueError):
+            apply_rotary(heads(0, 2), heads(2, 4), rotary, 0, **kw)

@@ -251,3 +251,19 @@ def test_empty_and_refusals():
         linear_act(x, w.clone().requires_grad_(), b)
     with torch.no_grad():
         linear_act(x, w.clone().requires_grad_(), b)
+
+
+def test_overlapping_destinations_are_refused():
+    """The result may replace the residual, but nothing that other tiles still read."""
+    from eraserdit_b200.linear import linear_act
+    buf = torch.zeros(300, 256, device="cuda", dtype=torch.bfloat16)
+    x, w = buf[:, :128], torch.zeros(128, 128, device="cuda", dtype=torch.bfloat16)
+    linear_act(x, w, out=buf[:, 128:])  # other columns of the same rows
+    for kw in (dict(out=x), dict(out=buf[:, 64:192]), dict(out=buf[:, 128:], residual=buf[:, 120:248]),
+               dict(residual=buf[:1, :128].expand(300, 128))):
+        with pytest.raises(ValueError):
+            linear_act(x, w, **kw)
+    with pytest.raises(ValueError):
+        linear_act(x[:1].expand(300, 128), w)
+    with pytest.raises(ValueError):
+        linear_act(x[:128], w, out=w)
