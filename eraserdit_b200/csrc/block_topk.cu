@@ -89,6 +89,17 @@ __device__ __forceinline__ int key_length(const int* lengths, int b, int kv_len)
   return lengths == nullptr ? kv_len : min(max(__ldg(lengths + b), 0), kv_len);
 }
 
+// The kernels of one call follow each other by programmatic dependent launch: a
+// kernel lets the next one start as soon as all of its own CTAs have, and the next
+// one sets itself up and then waits here for the whole of the one before (and so,
+// in turn, of those before that) before it touches what they write.
+__device__ __forceinline__ void start_next() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // ---------------------------------------------------------------- block sums
 struct PoolParams {
   const void* x;
@@ -100,13 +111,15 @@ struct PoolParams {
 };
 
 // One CTA sums one block of four heads: a lane eight channels (16 bytes) of a
-// token, a warp every fourth token, the warps' sums added in order.  (One warp a
-// block took 31 us at 3 x 2005 tokens, where there are 144 of them.)
-constexpr int kPoolWarps = 4;
+// token, the warps take turns and their sums are added in order.  Eight warps
+// where there are few blocks (3 x 2005 tokens: 31 us with one warp a block, 10
+// with four, 7 with eight), four where the device is full anyway (32640 tokens x
+// 32 heads: 54 against 59 us).
+constexpr int kPoolWarps = 8;
 template <typename T>
 __device__ __forceinline__ void pool_block(const PoolParams& p, long long item,
                                            double (*part)[32][8]) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int hg = (p.heads + 3) / 4;
   const int h = static_cast<int>(item % hg) * 4 + lane / 8;
   const long long bn = item / hg;
@@ -119,11 +132,11 @@ __device__ __forceinline__ void pool_block(const PoolParams& p, long long item,
   if (h < p.heads) {
     const T* src = static_cast<const T*>(p.x) + b * p.st.batch + h * p.st.head + (lane & 7) * 8;
     constexpr int U = 8;  // tokens requested together
-    for (int t = t0 + warp; t < t1; t += U * kPoolWarps) {
+    for (int t = t0 + warp; t < t1; t += U * warps) {
       uint4 v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int tu = t + u * kPoolWarps;
+        const int tu = t + u * warps;
         v[u] = make_uint4(0u, 0u, 0u, 0u);  // adds zeros behind the end
         if (tu < t1) v[u] = *reinterpret_cast<const uint4*>(src + tu * p.st.token);
       }
@@ -142,8 +155,7 @@ __device__ __forceinline__ void pool_block(const PoolParams& p, long long item,
   }
   __syncthreads();
   if (warp > 0 || h >= p.heads) return;
-#pragma unroll
-  for (int w = 0; w < kPoolWarps - 1; ++w)
+  for (int w = 0; w < warps - 1; ++w)
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum[i] += part[w][lane][i];
   if (p.mean && t1 > t0) {
@@ -160,6 +172,7 @@ template <typename T>
 __global__ void __launch_bounds__(32 * kPoolWarps)
     pool_kernel(const PoolParams a, const PoolParams b, long long items_a) {
   __shared__ double part[kPoolWarps - 1][32][8];
+  start_next();
   const long long item = blockIdx.x;
   if (item < items_a)
     pool_block<T>(a, item, part);
@@ -192,6 +205,8 @@ __global__ void __launch_bounds__(128)
   const long long kv = static_cast<long long>(b) * (heads / per) + h / per;
   const double* qg = q_sum + static_cast<long long>(bh) * groups * kDim;
   const double* kg = k_mean + kv * blocks * kDim;
+  start_next();
+  wait_previous();
   for (int i = threadIdx.x; i < kScoreTile * kDim / 2; i += 128) {
     const int r = i / (kDim / 2), c = i % (kDim / 2) * 2;
     double2 q = make_double2(0.0, 0.0), k = make_double2(0.0, 0.0);
@@ -363,6 +378,8 @@ template <int kPer>
 __global__ void __launch_bounds__(32 * kSelectWarps)
     select_kernel(const double* scores, int* selection, const int* lengths, long long rows,
                   long long rows_per_batch, int blocks, int kv_len, int key_block, int topk) {
+  start_next();
+  wait_previous();
   const long long row = static_cast<long long>(blockIdx.x) * kSelectWarps + (threadIdx.x >> 5);
   if (row >= rows) return;
   const int len = key_length(lengths, static_cast<int>(row / rows_per_batch), kv_len);
@@ -550,6 +567,7 @@ __global__ void __launch_bounds__(kTileThreads, 4)
                                     blockIdx.y * p.o_st.head + tok * p.o_st.token);
   };
   if (steps == 0) {  // no valid key: zeros
+    wait_previous();
     if (uint4* dst = out_row()) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) dst[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -577,13 +595,16 @@ __global__ void __launch_bounds__(kTileThreads, 4)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
+  if (threadIdx.x == kTile) {
+    tma_prefetch_desc(&tmap_q);
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
+  wait_previous();  // the choice
 
   if (warp == 4) {
     // --------------------------------------------------- loads and products
     if (elect_one()) {
-      tma_prefetch_desc(&tmap_q);
-      tma_prefetch_desc(&tmap_k);
-      tma_prefetch_desc(&tmap_v);
       constexpr uint32_t id_qk = idesc<kBf16>(kTile, kHalf, false);
       constexpr uint32_t id_pv = idesc<kBf16>(kTile, kDim, true);
       const uint32_t tO = tmem + kHalf;
@@ -782,6 +803,7 @@ struct RowParams {
   const double* k_mean;
   int* selection;
   int heads, per, q_len, kv_len, key_block, blocks, topk, splits;
+  int follows;  // launched behind the kernel that computes the means
   float scale_log2;
 };
 
@@ -832,6 +854,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 2) row_kernel(const RowParams 
     unpack8<T>(*reinterpret_cast<const uint4*>(src), q);
   }
   // ---------------------------------------------------------------- scores
+  if (p.follows) wait_previous();  // the means of this call
   // No CTA's shared memory is written before it has started.
   if (p.splits > 1) {
     cluster_arrive();
@@ -1093,10 +1116,39 @@ int launch_pool(const PoolParams* a, const PoolParams* b, int batch, cudaStream_
   const long long items = items_a + (b == nullptr ? 0 : pool_items(*b, batch));
   if (items > 0x7fffffffLL) return kErrTooLarge;
   const PoolParams none = {};
-  pool_kernel<T><<<static_cast<unsigned>(items), 32 * kPoolWarps, 0, st>>>(
+  const int warps = items < 16 * 148 ? kPoolWarps : kPoolWarps / 2;
+  pool_kernel<T><<<static_cast<unsigned>(items), 32 * warps, 0, st>>>(
       a == nullptr ? none : *a, b == nullptr ? none : *b, items_a);
   return static_cast<int>(cudaGetLastError());
 }
+
+// Launch configuration of a kernel that may start while the call's previous one
+// still runs, or of a cluster launch.
+struct Config {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attrs[2];
+  Config(dim3 grid, int threads, size_t smem, cudaStream_t st) {
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attrs;
+    cfg.numAttrs = 0;
+  }
+  Config& follow() {
+    attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    return *this;
+  }
+  Config& cluster(int ctas) {
+    attrs[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attrs[cfg.numAttrs].val.clusterDim.x = static_cast<unsigned>(ctas);
+    attrs[cfg.numAttrs].val.clusterDim.y = attrs[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+    return *this;
+  }
+  Config(const Config&) = delete;
+};
 
 struct Call {
   const void *q, *k, *v;
@@ -1139,18 +1191,21 @@ int run(const Call& c, cudaStream_t st) {
     if (e != cudaSuccess) return static_cast<int>(e);
     const dim3 grid((blocks + kScoreTile - 1) / kScoreTile, (groups + kScoreTile - 1) / kScoreTile,
                     static_cast<unsigned>(c.batch * c.q_heads));
-    score_kernel<<<grid, 128, kScoreSmem, st>>>(q_sum, pool, scores, c.q_heads, per, groups,
-                                                blocks);
-    if ((e = cudaGetLastError()) != cudaSuccess) return static_cast<int>(e);
+    Config score(grid, 128, kScoreSmem, st);
+    e = cudaLaunchKernelEx(&score.follow().cfg, score_kernel, static_cast<const double*>(q_sum),
+                           pool, scores, c.q_heads, per, groups, blocks);
+    if (e != cudaSuccess) return static_cast<int>(e);
     const long long per_batch = static_cast<long long>(c.q_heads) * groups;
     const long long rows = c.batch * per_batch;
     const unsigned ctas = static_cast<unsigned>((rows + kSelectWarps - 1) / kSelectWarps);
     auto select = blocks <= 32 * 8 ? select_kernel<8>
                   : blocks <= 32 * 16 ? select_kernel<16>
                   : blocks <= 32 * 32 ? select_kernel<32> : select_kernel<0>;
-    select<<<ctas, 32 * kSelectWarps, 0, st>>>(scores, c.selection, c.lengths, rows, per_batch,
-                                               blocks, c.kv_len, c.key_block, c.topk);
-    if ((e = cudaGetLastError()) != cudaSuccess) return static_cast<int>(e);
+    Config choose(dim3(ctas), 32 * kSelectWarps, 0, st);
+    e = cudaLaunchKernelEx(&choose.follow().cfg, select, static_cast<const double*>(scores),
+                           c.selection, c.lengths, rows, per_batch, blocks, c.kv_len, c.key_block,
+                           c.topk);
+    if (e != cudaSuccess) return static_cast<int>(e);
     CUtensorMap tq, tk, tv;
     if (operand_map(&tq, kBf16, c.q, c.q_len, c.q_heads, c.batch, c.q_st, kTile) ||
         operand_map(&tk, kBf16, c.k, c.kv_len, c.kv_heads, c.batch, c.k_st, kHalf) ||
@@ -1161,9 +1216,9 @@ int run(const Call& c, cudaStream_t st) {
     if (e != cudaSuccess) return static_cast<int>(e);
     const TileParams p = {c.q_len, c.kv_len, per, c.key_block, c.topk, c.lengths, c.selection,
                           scale_log2, c.out, c.o_st, c.status};
-    tile_attn_kernel<T, kBf16>
-        <<<dim3(groups, c.q_heads, c.batch), kTileThreads, kTileSmemLaunch, st>>>(tq, tk, tv, p);
-    return static_cast<int>(cudaGetLastError());
+    Config attend(dim3(groups, c.q_heads, c.batch), kTileThreads, kTileSmemLaunch, st);
+    return static_cast<int>(
+        cudaLaunchKernelEx(&attend.follow().cfg, tile_attn_kernel<T, kBf16>, tq, tk, tv, p));
   }
 
   const long long rows = static_cast<long long>(c.batch) * c.q_heads * c.q_len;
@@ -1176,24 +1231,17 @@ int run(const Call& c, cudaStream_t st) {
   }
   RowParams p = {c.q, c.k, c.v, c.q_st, c.k_st, c.v_st, c.o_st, c.out, c.lengths, pool,
                  c.selection, c.q_heads, per, c.q_len, c.kv_len, c.key_block, blocks, c.topk, 1,
-                 scale_log2};
+                 c.pool == nullptr, scale_log2};
   // As many CTAs as two a multiprocessor hold at once, each with two 64-key pieces
   // at least.
   const long long pieces = static_cast<long long>(most) << (c.key_block >> 7);
   while (p.splits < kMaxSplits && rows * p.splits * 2 <= 2 * 148 && pieces >= p.splits * 4)
     p.splits *= 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(rows * p.splits));
-  cfg.blockDim = dim3(32 * kRowWarps);
-  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = static_cast<unsigned>(p.splits);
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, row_kernel<T>, p));
+  Config attend(dim3(static_cast<unsigned>(rows * p.splits)), 32 * kRowWarps,
+                static_cast<size_t>(smem), st);
+  attend.cluster(p.splits);
+  if (p.follows) attend.follow();
+  return static_cast<int>(cudaLaunchKernelEx(&attend.cfg, row_kernel<T>, p));
 }
 
 }  // namespace btk
