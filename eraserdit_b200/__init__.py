@@ -5,8 +5,13 @@ for the C ABI underneath):
 
 - :mod:`eraserdit_b200.attention` -- attention backend ABI, ``B200AttentionImpl``,
   ``B200FP8AttentionImpl``
-- :mod:`eraserdit_b200.operator_fusion` -- ``apply_fused_qk_rmsnorm_rope``
-- :mod:`eraserdit_b200.rotary` -- ``LTXVideoRotaryPosEmbed`` (factored table)
+- :mod:`eraserdit_b200.operator_fusion` -- ``apply_fused_qk_rmsnorm_rope``,
+  ``apply_fused_qk_head_rmsnorm_rotary`` (norms of single heads)
+- :mod:`eraserdit_b200.rotary` -- ``LTXVideoRotaryPosEmbed`` (factored table),
+  ``RotaryPositions`` / ``apply_rotary`` (rotation of single heads)
+- :mod:`eraserdit_b200.linear` -- ``linear_bf16``, ``linear_act`` (activation, gate and residual
+  in the epilogue)
+- :mod:`eraserdit_b200.block_topk` -- ``block_topk_attention`` over key blocks a score selects
 - :mod:`eraserdit_b200.layer` -- ``EraserDiTSelfAttention`` (one ``attn1``)
 - :mod:`eraserdit_b200.ulysses` -- Ulysses SP (peer-memory or NCCL exchange, head chunks)
 - :mod:`eraserdit_b200.ring` -- ring and Ulysses x Ring SP, ``piece`` (ring accumulator)

@@ -7,6 +7,11 @@
     python -m eraserdit_b200.profile_case ring --batch 1 --seq 16320 --iters 2
     python -m eraserdit_b200.profile_case linear --batch 1 --seq 16320 --iters 3
     python -m eraserdit_b200.profile_case cudnn --batch 1 --seq 16320 --iters 3
+    python -m eraserdit_b200.profile_case linear_act --batch 1 --seq 16320 --n 8192 --iters 3
+    python -m eraserdit_b200.profile_case rotary --batch 1 --seq 32640 --iters 3
+    python -m eraserdit_b200.profile_case head_norm --batch 1 --seq 32640 --iters 3
+    python -m eraserdit_b200.profile_case block_topk --batch 1 --seq 32640 --heads 8 --iters 3
+    python -m eraserdit_b200.profile_case block_token --batch 4 --seq 32640 --iters 3
 
 ``sparse`` runs the configuration-4 pattern (32640 tokens in tile order, the
 seeded ellipse mask) whatever ``--seq`` says.  ``ring`` attends ``--seq``
@@ -15,7 +20,11 @@ per-rank work of ring degree 2): per iteration, one launch writing the state
 and one reading it and writing the output.  ``linear`` runs the QKV
 projection (``--batch`` x ``--seq`` rows of 2048 into ``--n`` columns, 6144 by
 default, with bias)
-through ``erd_linear_bf16``.  ``cudnn`` runs torch's SDPA with the cuDNN backend
+through ``erd_linear_bf16``.  ``linear_act`` runs the same rows with the tanh GELU
+through ``erd_linear_act``, ``rotary`` and ``head_norm`` turn the query and key heads of
+a Q|K|V buffer (three position axes; with the per-head norms), ``block_topk`` attends 64
+of the 64-key blocks per 128 queries, and ``block_token`` one token a sequence 32 of them,
+with kept block means.  ``cudnn`` runs torch's SDPA with the cuDNN backend
 on the same [B, H, S, 64] BF16 shape: a library yardstick for the attention
 kernel, not part of the path.
 
@@ -34,7 +43,8 @@ import torch
 def main() -> None:
     ap = argparse.ArgumentParser()
     ap.add_argument("kernel", choices=["attention", "prologue", "fp8", "sparse", "ring",
-                                       "linear", "cudnn"])
+                                       "linear", "cudnn", "linear_act", "rotary", "head_norm",
+                                       "block_topk", "block_token"])
     ap.add_argument("--batch", type=int, default=1)
     ap.add_argument("--seq", type=int, default=16320)
     ap.add_argument("--heads", type=int, default=32)
@@ -54,7 +64,40 @@ def main() -> None:
                 torch.nn.functional.scaled_dot_product_attention(q, k, v, scale=0.125)
         torch.cuda.synchronize()
         return
-    if args.kernel == "linear":
+    if args.kernel == "linear_act":
+        from eraserdit_b200.linear import linear_act
+        x = torch.randn(args.batch * args.seq, 2048, generator=g, device=device).bfloat16()
+        w = (torch.randn(args.n, 2048, generator=g, device=device) * 0.02).bfloat16()
+        b = torch.zeros(args.n, device=device, dtype=torch.bfloat16)
+        for _ in range(args.iters):
+            linear_act(x, w, b, activation="gelu_tanh")
+    elif args.kernel in ("rotary", "head_norm"):
+        from eraserdit_b200.operator_fusion import apply_fused_qk_head_rmsnorm_rotary
+        from eraserdit_b200.rotary import RotaryPositions, apply_rotary
+        qkv = torch.randn(args.batch, args.seq, 3, args.heads, 64, generator=g,
+                          device=device).bfloat16()
+        q, k = qkv[:, :, 0], qkv[:, :, 1]
+        s = torch.arange(args.seq, device=device)
+        pos = torch.stack([s // 2040, s // 60 % 34, s % 60])
+        rot = RotaryPositions(64, axes_dim=(24, 20, 20))
+        norm = torch.nn.RMSNorm(64, eps=1e-6, device=device, dtype=torch.bfloat16)
+        norm.requires_grad_(False)
+        for _ in range(args.iters):
+            if args.kernel == "rotary":
+                apply_rotary(q, k, rot, pos)
+            else:
+                apply_fused_qk_head_rmsnorm_rotary(q, k, norm, norm, rot, pos)
+    elif args.kernel in ("block_topk", "block_token"):
+        from eraserdit_b200.block_topk import block_topk_attention, pool_key_blocks
+        q, k, v = (torch.randn(args.batch, args.seq, args.heads, 64, generator=g,
+                               device=device).bfloat16() for _ in range(3))
+        pool = pool_key_blocks(k)
+        for _ in range(args.iters):
+            if args.kernel == "block_topk":
+                block_topk_attention(q, k, v, 0.125, 64)
+            else:
+                block_topk_attention(q[:, -1:], k, v, 0.125, 32, query_block=1, key_pool=pool)
+    elif args.kernel == "linear":
         from eraserdit_b200.linear import linear_bf16
         x = torch.randn(args.batch * args.seq, 2048, generator=g, device=device).bfloat16()
         w = (torch.randn(args.n, 2048, generator=g, device=device) * 0.02).bfloat16()
