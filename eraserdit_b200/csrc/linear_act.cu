@@ -678,7 +678,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
 }
 
 // --------------------------------------------------------------- split kernel
-constexpr int kSplitEpilogueWarps = 4;
+constexpr int kSplitEpilogueWarps = 8;  // two for each quarter of the rows
 constexpr int kSplitThreads = 32 * (2 + kSplitEpilogueWarps);
 constexpr int kSplitMaxStages = 20;
 // Clusters of eight leave multiprocessors of a group idle (15 fit at a time
@@ -842,46 +842,38 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       mbar_wait_drain(smem_u32(&bars->acc_full), 0);
     }
   } else {
+    // A quarter of the rows and, of the columns, one half (a 64-column tile that is
+    // finished in place is one piece, and the second warp has none).
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    const int row0 = m0 + quad * 32, piece_col = half * kPiece;
+    const bool mine = row0 < p.e.m && piece_col < BN && n0 + piece_col < p.e.n;
     Piece<T> piece;
-    const int first_row = m0 + (warp & 3) * 32;
-    if (p.direct && first_row < p.e.m) piece.request(p.e, first_row, n0, lane);
+    if (p.direct && mine) piece.request(p.e, row0, n0 + piece_col, lane);
     have = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->acc_full), 0, abort, p.status,
                                              kStatusTimeoutEpilogue));
     // A reduction that was cut short has set the flag before it committed.
     have = have && __all_sync(0xffffffffu, *abort == 0);
     tc_fence_after();
-    const int quad = warp & 3;
-    const int row0 = m0 + quad * 32;
     const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    if (have && row0 < p.e.m) {
-      if (p.direct) {
-        uint8_t* stage = tail + (warp - 2) * kStageBytes;
-        float* slab = reinterpret_cast<float*>(tail + kSplitEpilogueWarps * kStageBytes +
-                                               (warp - 2) * kSlabBytes);
+    if (have && p.direct && mine) {
+      uint8_t* stage = tail + (warp - 2) * kStageBytes;
+      float* slab = reinterpret_cast<float*>(tail + kSplitEpilogueWarps * kStageBytes +
+                                             (warp - 2) * kSlabBytes);
+      piece.park(p.e, stage, slab, lane);
+      finish_piece<T>(p.e, taddr + piece_col, row0, n0 + piece_col, piece.inside, piece.one_group,
+                      piece.group, stage, slab, lane);
+    } else if (have && !p.direct && row0 < p.e.m) {
+      // The ring is free: every load has been consumed by a finished product.
+      const int r = quad * 32 + lane;
 #pragma unroll 1
-        for (int c = 0; c < BN; c += kPiece) {
-          if (n0 + c >= p.e.n) break;
-          const bool inside = piece.inside, one_group = piece.one_group;
-          const int group = piece.group;
-          piece.park(p.e, stage, slab, lane);
-          if (c + kPiece < BN && n0 + c + kPiece < p.e.n)
-            piece.request(p.e, row0, n0 + c + kPiece, lane);
-          finish_piece<T>(p.e, taddr + c, row0, n0 + c, inside, one_group, group, stage, slab,
-                          lane);
-        }
-      } else {
-        // The ring is free: every load has been consumed by a finished product.
-        const int r = quad * 32 + lane;
-#pragma unroll 1
-        for (int c = 0; c < BN; c += 32) {
-          uint32_t v[32];
-          tmem_ld_wait_32(taddr + c, v);
-          if (m0 + r < p.e.m) {
+      for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
+        uint32_t v[32];
+        tmem_ld_wait_32(taddr + c, v);
+        if (m0 + r < p.e.m) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<uint4*>(smem + partial_offset<BN>(r, c / 4 + i)) =
-                  make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-          }
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<uint4*>(smem + partial_offset<BN>(r, c / 4 + i)) =
+                make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
         }
       }
     }

@@ -311,3 +311,31 @@ def test_destination_over_the_queries_but_not_the_keys(query_block):
     for out in (k[:, :140], v[:, 20:160]):
         with pytest.raises(ValueError):
             block_topk_attention(q, k, v, SCALE, 2, query_block=query_block, out=out)
+
+
+@pytest.mark.parametrize("query_block", [1, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_scores_that_are_not_finite(query_block, dtype):
+    """Valid keys whose scores are NaN or infinite, in every kind of place of a block:
+    NaN and +inf make the row NaN, -inf weighs nothing, and a row with nothing but -inf
+    is zeros."""
+    q = torch.rand(1, 130, 1, 64, device="cuda").to(dtype) + 0.5  # positive: q . inf = inf
+    _, k0, v = _inputs(1, 1, 192, 1, 1, dtype, 14)
+    for place in (0, 1, 2, 7, 8, 9, 31, 62, 63, 64, 100, 191):
+        for bad in (math.nan, math.inf, -math.inf):
+            k = k0.clone()
+            k[0, place, 0, 5] = bad
+            out, _ = _run(q, k, v, 3, query_block=query_block)
+            if bad == -math.inf:
+                s = (q[0, :, 0].double() @ k[0, :, 0].double().T * SCALE)
+                want = torch.softmax(s, -1) @ v[0, :, 0].double()
+                assert float((out[0, :, 0].double() - want).abs().max()) <= 0.05
+            else:
+                assert bool(torch.isnan(out).all())
+    k = k0.clone()
+    k[..., 5] = -math.inf
+    out, _ = _run(q, k, v, 3, query_block=query_block)
+    assert bool((out == 0).all())
+    k[0, 150, 0, 5] = 0.0  # one finite score behind two blocks of -inf
+    out, _ = _run(q, k, v, 3, query_block=query_block)
+    assert torch.equal(out, v[:, 150:151].expand_as(out))
