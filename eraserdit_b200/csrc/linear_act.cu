@@ -280,6 +280,34 @@ __device__ __forceinline__ void store8(void* base, long long ld, int vec, int ro
       reinterpret_cast<uint16_t*>(p)[i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
 }
 
+// The same for four values.
+template <typename T>
+__device__ __forceinline__ uint2 load4(const void* base, long long ld, int vec, int row, int col,
+                                       int n) {
+  const T* p = static_cast<const T*>(base) + row * ld + col;
+  if (vec && col + 4 <= n) return *reinterpret_cast<const uint2*>(p);
+  uint32_t w[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (col + i < n)
+      w[i >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[i]) << (16 * (i & 1));
+  return make_uint2(w[0], w[1]);
+}
+template <typename T>
+__device__ __forceinline__ void store4(void* base, long long ld, int vec, int row, int col, int n,
+                                       const uint2& v) {
+  T* p = static_cast<T*>(base) + row * ld + col;
+  if (vec && col + 4 <= n) {
+    *reinterpret_cast<uint2*>(p) = v;
+    return;
+  }
+  const uint32_t w[2] = {v.x, v.y};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (col + i < n)
+      reinterpret_cast<uint16_t*>(p)[i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+}
+
 constexpr int kPiece = 64;                    // columns an epilogue warp takes at a time
 constexpr int kStageBytes = 32 * kPiece * 2;  // 32 rows of a piece, 16-byte chunks swizzled
 constexpr int kSlabBytes = 2 * kPiece * 4;    // bias and gate of a piece as floats
@@ -717,16 +745,16 @@ struct SplitSmem {
       kSplitEpilogueWarps * (kStageBytes + kSlabBytes) + 1024;  // staging, slabs, barriers
 };
 
-// Bias, gate and residual of eight columns of one row.
+// Bias, gate and residual of four columns of one row.
 template <typename T>
 struct Side {
-  uint4 bias, gate, res;
+  uint2 bias, gate, res;
   __device__ __forceinline__ void request(const Epilogue& e, int row, int col) {
-    bias = gate = res = make_uint4(0u, 0u, 0u, 0u);
-    if (e.bias != nullptr) bias = load8<T>(e.bias, 0, e.vec_bias, 0, col, e.n);
+    bias = gate = res = make_uint2(0u, 0u);
+    if (e.bias != nullptr) bias = load4<T>(e.bias, 0, e.vec_bias, 0, col, e.n);
     if (e.gate != nullptr)
-      gate = load8<T>(e.gate, e.n, e.vec_gate, row / e.gate_rows, col, e.n);
-    if (e.residual != nullptr) res = load8<T>(e.residual, e.ld_res, e.vec_res, row, col, e.n);
+      gate = load4<T>(e.gate, e.n, e.vec_gate, row / e.gate_rows, col, e.n);
+    if (e.residual != nullptr) res = load4<T>(e.residual, e.ld_res, e.vec_res, row, col, e.n);
   }
 };
 
@@ -778,16 +806,17 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
 
-  // Unless the accumulator is finished in place: the eight-column chunks of the
+  // Unless the accumulator is finished in place: the four-column chunks of the
   // tile that this CTA finishes; what a thread's first one needs is requested now.
-  const int chunks = min(128, p.e.m - m0) * (BN / 8);
+  constexpr int kRowChunks = BN / 4;
+  const int chunks = min(128, p.e.m - m0) * kRowChunks;
   const int share_lo = static_cast<int>(static_cast<long long>(chunks) * split / p.splits);
   const int share_hi = static_cast<int>(static_cast<long long>(chunks) * (split + 1) / p.splits);
   Side<T> side;
   if (!p.direct) {
     const int i = share_lo + static_cast<int>(threadIdx.x);
-    if (i < share_hi && n0 + i % (BN / 8) * 8 < p.e.n)
-      side.request(p.e, m0 + i / (BN / 8), n0 + i % (BN / 8) * 8);
+    if (i < share_hi && n0 + i % kRowChunks * 4 < p.e.n)
+      side.request(p.e, m0 + i / kRowChunks, n0 + i % kRowChunks * 4);
   }
 
   bool have = false;  // this warp's rows of the accumulator may be read
@@ -883,47 +912,38 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     __syncthreads();
   } else {
     cluster_sync();
-    // Each CTA adds and finishes its share of the tile, eight columns a thread.
-    // A split that gave up has set the status word; its partial sums are stale
-    // and the tile's values are then as undefined as those of any timed-out call.
+    // Each CTA adds and finishes its share of the tile, four columns a thread, so
+    // that a warp reads 512 neighbouring bytes of a peer.  A split that gave up has
+    // set the status word; its partial sums are stale and the tile's values are then
+    // as undefined as those of any timed-out call.
     const uint32_t base = smem_u32(smem);
     for (int i = share_lo + static_cast<int>(threadIdx.x); i < share_hi; i += kSplitThreads) {
-      const int r = i / (BN / 8), c8 = i % (BN / 8);
-      const int row = m0 + r, col = n0 + c8 * 8;
+      const int r = i / kRowChunks, c4 = i % kRowChunks;
+      const int row = m0 + r, col = n0 + c4 * 4;
       if (col >= p.e.n) continue;
       // All requests first: one round trip over the cluster, not one per part.
-      float4 a[kMaxSplits], b[kMaxSplits];
+      float4 a[kMaxSplits];
 #pragma unroll
-      for (int s = 0; s < kMaxSplits; ++s) {
-        if (s < p.splits) {
-          const uint32_t peer = map_rank(base, static_cast<uint32_t>(s));
-          a[s] = ld_cluster(peer + partial_offset<BN>(r, c8 * 2));
-          b[s] = ld_cluster(peer + partial_offset<BN>(r, c8 * 2 + 1));
-        }
-      }
+      for (int s = 0; s < kMaxSplits; ++s)
+        if (s < p.splits)
+          a[s] = ld_cluster(map_rank(base, static_cast<uint32_t>(s)) + partial_offset<BN>(r, c4));
       if (i >= share_lo + kSplitThreads) side.request(p.e, row, col);
-      float v[8];
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 0.f;
+      for (int s = 0; s < kMaxSplits; ++s)
+        if (s < p.splits) v[0] += a[s].x, v[1] += a[s].y, v[2] += a[s].z, v[3] += a[s].w;
+      const uint32_t bias[2] = {side.bias.x, side.bias.y};
+      const uint32_t gate[2] = {side.gate.x, side.gate.y};
+      const uint32_t res[2] = {side.res.x, side.res.y};
 #pragma unroll
-      for (int s = 0; s < kMaxSplits; ++s) {
-        if (s < p.splits) {
-          v[0] += a[s].x, v[1] += a[s].y, v[2] += a[s].z, v[3] += a[s].w;
-          v[4] += b[s].x, v[5] += b[s].y, v[6] += b[s].z, v[7] += b[s].w;
-        }
-      }
-      const uint32_t bias[4] = {side.bias.x, side.bias.y, side.bias.z, side.bias.w};
-      const uint32_t gate[4] = {side.gate.x, side.gate.y, side.gate.z, side.gate.w};
-      const uint32_t res[4] = {side.res.x, side.res.y, side.res.z, side.res.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 2; ++j) {
         const float2 f = unpack2<T>(bias[j]);
         v[2 * j] += f.x;
         v[2 * j + 1] += f.y;
       }
       activate(v, p.e.act);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 2; ++j) {
         if (p.e.gate != nullptr) {
           const float2 g = unpack2<T>(gate[j]);
           v[2 * j] *= g.x;
@@ -933,9 +953,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
         v[2 * j] += f.x;
         v[2 * j + 1] += f.y;
       }
-      store8<T>(p.e.y, p.e.ldy, p.e.vec_y, row, col, p.e.n,
-                make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]),
-                           pack2<T>(v[6], v[7])));
+      store4<T>(p.e.y, p.e.ldy, p.e.vec_y, row, col, p.e.n,
+                make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])));
     }
     cluster_sync();  // the peers have read this CTA's sums
   }
@@ -1141,7 +1160,7 @@ template <typename T, bool kBf16, int BN>
 int launch_split(const CUtensorMap& ta, const CUtensorMap& tb, SplitParams p, const Plan& pl,
                  cudaStream_t st) {
   using S = SplitSmem<BN>;
-  // Few rows or several parts: all threads finish eight-column chunks of the sums
+  // Few rows or several parts: all threads finish four-column chunks of the sums
   // in shared memory (few rows would leave a whole piece to one or two warps,
   // some 3500 clocks).
   p.direct = pl.splits == 1 && p.e.m > 64;
