@@ -150,8 +150,8 @@ __device__ __forceinline__ void load_weight(const Params& p, int which, int c, f
   }
 }
 
-// N: channels of a chunk (16 bytes).  32 warps a multiprocessor hold the rotation
-// (64 registers; 6.5 TB/s), 24 the norm with it (80 registers, a lane's
+// N: channels of a chunk.  With 16-byte chunks 32 warps a multiprocessor hold the
+// rotation (64 registers; 6.5 TB/s), 24 the norm with it (80 registers, a lane's
 // coefficients double; 5.1 TB/s).  Two head groups at a time, more or fewer warps,
 // larger blocks, and 8-byte chunks for the norm (265 us, twice the sums to wait
 // for) were slower at 2 x 32640 tokens x 64 heads x 64.
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(32 * kWarps, kNorm ? 6 : 8) head_rotary_kernel
   }
 }
 
-// The same for sizes and strides that 16-byte chunks do not fit: a warp takes
+// The same for sizes and strides that no chunk fits: a warp takes
 // one head at a time, a lane every 32nd pair and every 32nd channel behind the
 // pairs, value by value.  The norm reads the head twice (the second time from
 // L1); every lane has the sum before any lane writes, so in-place calls hold.
@@ -354,43 +354,63 @@ __global__ void __launch_bounds__(32 * kWarps) head_rotary_scalar_kernel(const P
   }
 }
 
-template <typename T, bool kNorm, bool kInterleaved>
-int launch(Params p, cudaStream_t stream) {
-  constexpr int N = static_cast<int>(16 / sizeof(T));
-  // Chunks fit when every head starts on their size, the head is a whole number
-  // of them (at most two a lane) and no chunk holds both turned and other channels
-  // or, in the half layout, channels of both halves.
-  const bool vector = (p.addresses & (N * sizeof(T) - 1)) == 0 && (p.strides & (N - 1)) == 0 &&
-                      p.dim % N == 0 && p.dim <= 64 * N &&
-                      p.rotary % (kInterleaved ? N : 2 * N) == 0;
-  if (vector) {
-    const int tasks = (p.dim + 2 * N - 1) / (2 * N);
-    p.lanes = 1;
-    p.log2_lanes = 0;
-    while (p.lanes < tasks) p.lanes *= 2, ++p.log2_lanes;
-    const int per = 32 / p.lanes;
-    for (int w = 0; w < 2; ++w) p.iters[w] = (p.heads[w] + per - 1) / per;
-  } else {
-    p.lanes = 32;
-    p.log2_lanes = 5;
-    for (int w = 0; w < 2; ++w) p.iters[w] = p.heads[w];
-  }
-  // A warp walks over all heads of a token, unless that leaves the device
-  // short of warps (32 on each of 148 multiprocessors).
+// Chunks of N fit when every head starts on their size, the head is a whole number
+// of them (at most two a lane) and no chunk holds both turned and other channels or,
+// in the half layout, channels of both halves.
+template <typename T, int N>
+bool chunks_fit(const Params& p, bool interleaved) {
+  return (p.addresses & (N * sizeof(T) - 1)) == 0 && (p.strides & (N - 1)) == 0 && p.dim % N == 0 &&
+         p.dim <= 64 * N && p.rotary % (interleaved ? N : 2 * N) == 0;
+}
+
+// A warp walks over all head groups of a token, unless that leaves the device short
+// of warps (32 on each of 148 multiprocessors).
+int share_tokens(Params& p, unsigned* blocks) {
   const long long tokens = static_cast<long long>(p.batch) * p.tokens;
   const int iters = p.iters[0] + p.iters[1];
   const long long share = tokens * iters / (148 * 32);
   p.chunk = static_cast<int>(share < 1 ? 1 : share > iters ? iters : share);
   p.chunks = (iters + p.chunk - 1) / p.chunk;
-  const long long blocks = (tokens * p.chunks + kWarps - 1) / kWarps;
-  if (blocks > 0x7fffffffLL) return kErrTooLarge;
+  const long long n = (tokens * p.chunks + kWarps - 1) / kWarps;
+  if (n > 0x7fffffffLL) return kErrTooLarge;
+  *blocks = static_cast<unsigned>(n);
+  return kErrOk;
+}
+
+template <typename T, int N, bool kNorm, bool kInterleaved>
+int launch_chunks(Params p, size_t smem, cudaStream_t stream) {
+  const int tasks = (p.dim + 2 * N - 1) / (2 * N);
+  p.lanes = 1;
+  p.log2_lanes = 0;
+  while (p.lanes < tasks) p.lanes *= 2, ++p.log2_lanes;
+  const int per = 32 / p.lanes;
+  for (int w = 0; w < 2; ++w) p.iters[w] = (p.heads[w] + per - 1) / per;
+  unsigned blocks;
+  if (int rc = share_tokens(p, &blocks)) return rc;
+  head_rotary_kernel<T, N, kNorm, kInterleaved><<<blocks, 32 * kWarps, smem, stream>>>(p);
+  return static_cast<int>(cudaGetLastError());
+}
+
+// The widest chunks that fit (16, 8 or 4 bytes), else value by value.
+template <typename T, bool kNorm, bool kInterleaved>
+int launch(Params p, cudaStream_t stream) {
+  constexpr int N = static_cast<int>(16 / sizeof(T));
   const size_t smem = static_cast<size_t>(kWarps) * (p.rotary / 2) * sizeof(float2);
-  if (vector)
-    head_rotary_kernel<T, N, kNorm, kInterleaved>
-        <<<static_cast<unsigned>(blocks), 32 * kWarps, smem, stream>>>(p);
-  else
-    head_rotary_scalar_kernel<T, kNorm, kInterleaved>
-        <<<static_cast<unsigned>(blocks), 32 * kWarps, smem, stream>>>(p);
+  if (chunks_fit<T, N>(p, kInterleaved))
+    return launch_chunks<T, N, kNorm, kInterleaved>(p, smem, stream);
+  if (chunks_fit<T, N / 2>(p, kInterleaved))
+    return launch_chunks<T, N / 2, kNorm, kInterleaved>(p, smem, stream);
+  if constexpr (N > 4) {
+    if (chunks_fit<T, N / 4>(p, kInterleaved))
+      return launch_chunks<T, N / 4, kNorm, kInterleaved>(p, smem, stream);
+  }
+  p.lanes = 32;
+  p.log2_lanes = 5;
+  for (int w = 0; w < 2; ++w) p.iters[w] = p.heads[w];
+  unsigned blocks;
+  if (int rc = share_tokens(p, &blocks)) return rc;
+  head_rotary_scalar_kernel<T, kNorm, kInterleaved>
+      <<<blocks, 32 * kWarps, smem, stream>>>(p);
   return static_cast<int>(cudaGetLastError());
 }
 

@@ -252,35 +252,7 @@ struct Epilogue {
   int vec_bias, vec_gate, vec_res, vec_y;  // rows start on 16 bytes
 };
 
-// Eight values from column `col` of row `row` (what lies behind column n is 0).
-template <typename T>
-__device__ __forceinline__ uint4 load8(const void* base, long long ld, int vec, int row, int col,
-                                       int n) {
-  const T* p = static_cast<const T*>(base) + row * ld + col;
-  if (vec && col + 8 <= n) return *reinterpret_cast<const uint4*>(p);
-  uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (col + i < n)
-      w[i >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[i]) << (16 * (i & 1));
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-template <typename T>
-__device__ __forceinline__ void store8(void* base, long long ld, int vec, int row, int col, int n,
-                                       const uint4& v) {
-  T* p = static_cast<T*>(base) + row * ld + col;
-  if (vec && col + 8 <= n) {
-    *reinterpret_cast<uint4*>(p) = v;
-    return;
-  }
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (col + i < n)
-      reinterpret_cast<uint16_t*>(p)[i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
-}
-
-// The same for four values.
+// Four values from column `col` of row `row` (what lies behind column n is 0).
 template <typename T>
 __device__ __forceinline__ uint2 load4(const void* base, long long ld, int vec, int row, int col,
                                        int n) {
@@ -311,6 +283,11 @@ __device__ __forceinline__ void store4(void* base, long long ld, int vec, int ro
 constexpr int kPiece = 64;                    // columns an epilogue warp takes at a time
 constexpr int kStageBytes = 32 * kPiece * 2;  // 32 rows of a piece, 16-byte chunks swizzled
 constexpr int kSlabBytes = 2 * kPiece * 4;    // bias and gate of a piece as floats
+
+// Byte of value (row, column) in a staging block.
+__device__ __forceinline__ int staged(int r, int c) {
+  return r * 128 + (((c >> 3) ^ (r & 7)) * 16) + (c & 7) * 2;
+}
 
 // What an epilogue warp reads from global memory for one piece (32 rows x 64
 // columns), requested a piece ahead so that its latency lies under the products
@@ -355,13 +332,6 @@ struct Piece {
 #pragma unroll
         for (int q = 0; q < 8; ++q)
           res[q] = *reinterpret_cast<const uint4*>(p + 4 * q * e.ld_res);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          res[q] = make_uint4(0u, 0u, 0u, 0u);
-          if (r + 4 * q < e.m && c < e.n)
-            res[q] = load8<T>(e.residual, e.ld_res, e.vec_res, r + 4 * q, c, e.n);
-        }
       }
     }
   }
@@ -370,11 +340,22 @@ struct Piece {
   // registers for the next request.
   __device__ __forceinline__ void park(const Epilogue& e, uint8_t* stage, float* slab, int lane) {
     const int sub = lane >> 3, chunk = lane & 7;  // row within a group of 4, 16-byte chunk
-    if (e.residual != nullptr) {
+    if (e.residual != nullptr && inside) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
         const int rr = 4 * q + sub;
         *reinterpret_cast<uint4*>(stage + rr * 128 + ((chunk ^ (rr & 7)) * 16)) = res[q];
+      }
+    } else if (e.residual != nullptr) {
+      // ragged or unaligned: value by value, 32 neighbouring ones a warp
+      const int rows = min(32, e.m - row0);
+#pragma unroll 4
+      for (int i = 0; i < 2 * rows; ++i) {
+        const int rr = i >> 1, c = lane + 32 * (i & 1);
+        uint16_t v = 0;
+        if (col0 + c < e.n)
+          v = static_cast<const uint16_t*>(e.residual)[(row0 + rr) * e.ld_res + col0 + c];
+        *reinterpret_cast<uint16_t*>(stage + staged(rr, c)) = v;
       }
     }
 #pragma unroll
@@ -453,12 +434,15 @@ __device__ __forceinline__ void finish_piece(const Epilogue& e, uint32_t taddr, 
       *reinterpret_cast<uint4*>(p + 4 * q * e.ldy) = *reinterpret_cast<const uint4*>(
           stage + (4 * q + sub) * 128 + ((chunk ^ ((4 * q + sub) & 7)) * 16));
   } else {
-#pragma unroll 1
-    for (int q = 0; q < 8; ++q) {
-      const int rr = 4 * q + sub;
-      if (row0 + rr < e.m && c < e.n)
-        store8<T>(e.y, e.ldy, e.vec_y, row0 + rr, c, e.n,
-                  *reinterpret_cast<const uint4*>(stage + rr * 128 + ((chunk ^ (rr & 7)) * 16)));
+    // ragged or unaligned: value by value, 32 neighbouring ones a warp (pieces of 16
+    // bytes, whose values are apart by lanes, took twice the time of the products)
+    const int rows = min(32, e.m - row0);
+#pragma unroll 4
+    for (int i = 0; i < 2 * rows; ++i) {
+      const int rr = i >> 1, cc = lane + 32 * (i & 1);
+      if (col0 + cc < e.n)
+        static_cast<uint16_t*>(e.y)[(row0 + rr) * e.ldy + col0 + cc] =
+            *reinterpret_cast<const uint16_t*>(stage + staged(rr, cc));
     }
   }
   __syncwarp();
