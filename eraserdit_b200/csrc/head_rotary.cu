@@ -31,9 +31,6 @@ namespace rot {
 
 constexpr int kWarps = 4;
 constexpr int kMaxHeadDim = 1024;
-// Head groups that a warp requests together; the next ones are on the way while
-// these are turned, and the first ones while the angles are computed.
-constexpr int kUnroll = 1;
 
 struct Params {
   const void* in[2];  // queries, keys
@@ -48,6 +45,9 @@ struct Params {
   int lanes, log2_lanes;  // lanes of a warp for one head (vector kernel)
   int iters[2];           // head groups of queries and of keys
   int chunk, chunks;      // head groups of one warp, warps of one token
+  long long items;        // warps with work
+  // Bytes from one token, head and head group to the next (vector kernel).
+  unsigned in_token[2], out_token[2], in_head[2], out_head[2], in_step[2], out_step[2];
   const double* turns;    // [rotary / 2] turns per position step
   float amplitude, sin_sign;
   int axis1, axis2;  // first pair of the second and third position axis
@@ -56,10 +56,15 @@ struct Params {
   long long pos_as, pos_bs, pos_ts, start;
   unsigned long long addresses;  // all data pointers and all strides, or-ed (host)
   long long strides;
+  unsigned long long weights;  // the norm's weight pointers, or-ed (host)
 };
 
+// Cosines of all rotated pairs of a warp's token, then sines; each part is as long as
+// eight-value reads from any chunk's first pair need.
+__host__ __device__ __forceinline__ int slab_part(int rotary) { return (rotary / 2 + 7) & ~7; }
+
 // Cosine and sine of every rotated pair of one token into this warp's slab.
-__device__ __forceinline__ void angles(const Params& p, int b, int tok, int lane, float2* slab) {
+__device__ __forceinline__ void angles(const Params& p, int b, int tok, int lane, float* slab) {
   for (int i = lane; i < p.rotary / 2; i += 32) {
     long long where = p.start + tok;
     if (p.pos != nullptr) {
@@ -72,7 +77,8 @@ __device__ __forceinline__ void angles(const Params& p, int b, int tok, int lane
     t -= rint(t);
     float s, c;
     sincospif(2.0f * static_cast<float>(t), &s, &c);
-    slab[i] = make_float2(c * p.amplitude, s * p.amplitude * p.sin_sign);
+    slab[i] = c * p.amplitude;
+    slab[slab_part(p.rotary) + i] = s * p.amplitude * p.sin_sign;
   }
   __syncwarp();
 }
@@ -137,78 +143,148 @@ struct __align__(sizeof(T) * N) Chunk {
   }
 };
 
-// Weights of channels [c, c + N) of one norm.
-template <typename T, int N>
-__device__ __forceinline__ void load_weight(const Params& p, int which, int c, float* w) {
-  if (p.weight_fp32) {
+// N (2, 4 or 8) neighbouring floats of shared or global memory, in reads of 16 bytes
+// at most.
+template <int N>
+__device__ __forceinline__ void load_floats(const float* src, float* f) {
+  if constexpr (N >= 4) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = static_cast<const float*>(p.weight[which])[c + i];
+    for (int i = 0; i < N; i += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(src + i);
+      f[i] = v.x, f[i + 1] = v.y, f[i + 2] = v.z, f[i + 3] = v.w;
+    }
   } else {
-    const T* base = static_cast<const T*>(p.weight[which]) + c;
-#pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = Value<T>::one(base[i]);
+    const float2 v = *reinterpret_cast<const float2*>(src);
+    f[0] = v.x, f[1] = v.y;
   }
 }
 
-// N: channels of a chunk.  With 16-byte chunks 32 warps a multiprocessor hold the
-// rotation (64 registers; 6.5 TB/s), 24 the norm with it (80 registers, a lane's
-// coefficients double; 5.1 TB/s).  Two head groups at a time, more or fewer warps,
-// larger blocks, and 8-byte chunks for the norm (265 us, twice the sums to wait
-// for) were slower at 2 x 32640 tokens x 64 heads x 64.
+// Weights of channels [c, c + N) of one norm.
+template <typename T, int N>
+__device__ __forceinline__ void load_weight(const Params& p, int which, int c, float* w) {
+  if (p.weight_fp32)
+    load_floats<N>(static_cast<const float*>(p.weight[which]) + c, w);
+  else
+    reinterpret_cast<const Chunk<T, N>*>(static_cast<const T*>(p.weight[which]) + c)->unpack(w);
+}
+
+// Two floats in one register pair: one instruction does both.
+struct Two {
+  unsigned long long v;
+};
+__device__ __forceinline__ Two two(float lo, float hi) {
+  Two t;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(t.v) : "f"(lo), "f"(hi));
+  return t;
+}
+__device__ __forceinline__ void split(Two t, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(t.v));
+}
+__device__ __forceinline__ Two mul(Two a, Two b) {
+  Two t;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(t.v) : "l"(a.v), "l"(b.v));
+  return t;
+}
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+  Two t;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(t.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return t;
+}
+
+// N: channels of a chunk.  A warp walks over head groups, the next group's values on
+// the way while this one is turned, the first one's while the angles are computed.
+//
+// Besides memory, instructions bound it: counted at 213 a head group and 256 with the
+// norm, three quarters of all issue slots went to them.  So the norm and its
+// coefficients are computed two values at a time (the rotation alone is not: a factor's
+// sign is free in the plain form, and eight registers fewer let 32 warps reside),
+// addresses advance by a constant, and weights and angles are read 16 bytes at a time:
+// 121 and 167 a group.
+//
+// 32640 tokens with 64 values a head, rotation and norm with it: 64 heads 84 and 100 us
+// (6.4 and 5.4 TB/s; 86 and 107 before), 8 heads 22 and 34 us (3.0 and 1.9 TB/s; 24 and
+// 39 before; here the angles and coefficients of a token, used once or twice, are most
+// of the instructions).  Two head groups at a time, more or fewer warps, larger blocks,
+// several tokens a warp, and 8-byte chunks for the norm (twice the sums to wait for)
+// were slower.
 template <typename T, int N, bool kNorm, bool kInterleaved>
 __global__ void __launch_bounds__(32 * kWarps, kNorm ? 6 : 8) head_rotary_kernel(const Params p) {
   using V = Chunk<T, N>;
-  extern __shared__ float2 slabs[];
+  constexpr int P = N / 2;  // couples of this lane's N pairs
+  extern __shared__ __align__(16) float slabs[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long item = static_cast<long long>(blockIdx.x) * kWarps + warp;
-  const long long token = item / p.chunks;
-  if (token >= static_cast<long long>(p.batch) * p.tokens) return;
-  const int part = static_cast<int>(item - token * p.chunks);
-  const int b = static_cast<int>(token / p.tokens);
-  const int tok = static_cast<int>(token - static_cast<long long>(b) * p.tokens);
-
-  // This lane's two chunks of every head it meets.
-  const int sub = lane & (p.lanes - 1), slot = lane >> p.log2_lanes, per = 32 >> p.log2_lanes;
-  int c0, c1;
-  if (kInterleaved || sub >= p.rotary / (2 * N)) {
-    c0 = 2 * N * sub;  // also behind the rotated channels of the half layout
-    c1 = c0 + N;
+  if (item >= p.items) return;
+  int part = 0, b, tok;
+  if (p.items <= 0x7fffffffLL) {  // divisions of 64 bits are long
+    unsigned token = static_cast<unsigned>(item);
+    if (p.chunks > 1) {
+      token /= static_cast<unsigned>(p.chunks);
+      part = static_cast<int>(item) - static_cast<int>(token) * p.chunks;
+    }
+    b = static_cast<int>(token / static_cast<unsigned>(p.tokens));
+    tok = static_cast<int>(token) - b * p.tokens;
   } else {
-    c0 = N * sub;
-    c1 = p.rotary / 2 + N * sub;
+    const long long token = item / p.chunks;
+    part = static_cast<int>(item - token * p.chunks);
+    b = static_cast<int>(token / p.tokens);
+    tok = static_cast<int>(token - static_cast<long long>(b) * p.tokens);
   }
+
+  // This lane's two chunks of every head it meets: N pairs from N * sub on, or plain
+  // channels.  In the interleaved layout the second chunk may be plain alone.
+  const int sub = lane & (p.lanes - 1), slot = lane >> p.log2_lanes, per = 32 >> p.log2_lanes;
+  const bool adjoin = kInterleaved || sub >= p.rotary / (2 * N);
+  auto first_of = [](int i) { return kInterleaved ? 2 * i : i; };  // pair i in a lane's values
+  auto second_of = [](int i) { return kInterleaved ? 2 * i + 1 : N + i; };
+  const int c0 = adjoin ? 2 * N * sub : N * sub;
+  const int c1 = adjoin ? c0 + N : p.rotary / 2 + c0;
   const bool has0 = c0 < p.dim, has1 = c1 < p.dim;
+  const bool turned0 = c0 < p.rotary, turned1 = kInterleaved ? c1 < p.rotary : turned0;
+  const int apart = (c1 - c0) * static_cast<int>(sizeof(T));
   const int first = part * p.chunk, last = min(first + p.chunk, p.iters[0] + p.iters[1]);
-  // Head group i of queries, then keys: its tensor and this lane's head.
-  auto place = [&](int i, int& which, int& head) {
-    which = i >= p.iters[0];
-    head = (which ? i - p.iters[0] : i) * per + slot;
+
+  int which = first >= p.iters[0], head = (first - (which ? p.iters[0] : 0)) * per + slot;
+  auto place = [&](const void* base, const long long* bs, const unsigned* ts,
+                   const unsigned* hs) {
+    const unsigned long long at = static_cast<unsigned long long>(static_cast<unsigned>(tok)) *
+                                      ts[which] +
+                                  static_cast<unsigned long long>(static_cast<unsigned>(head)) *
+                                      hs[which];
+    return static_cast<const char*>(base) + at + b * bs[which] * static_cast<int>(sizeof(T)) +
+           c0 * static_cast<int>(sizeof(T));
   };
-  auto request = [&](int it, V (&v0)[kUnroll], V (&v1)[kUnroll]) {
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      v0[u].clear();
-      v1[u].clear();
-      int which, head;
-      place(it + u, which, head);
-      if (it + u < last && head < p.heads[which]) {
-        const T* src = static_cast<const T*>(p.in[which]) + b * p.in_bs[which] +
-                       tok * p.in_ts[which] + head * p.in_hs[which];
-        if (has0) v0[u] = *reinterpret_cast<const V*>(src + c0);
-        if (has1) v1[u] = *reinterpret_cast<const V*>(src + c1);
-      }
+  const char* src = place(p.in[which], p.in_bs, p.in_token, p.in_head);
+  V v0, v1;  // lanes and channels outside of a head keep the zeros
+  v0.clear();
+  v1.clear();
+  auto request = [&] {
+    if (head < p.heads[which]) {
+      if (has0) v0 = *reinterpret_cast<const V*>(src);
+      if (has1) v1 = *reinterpret_cast<const V*>(src + apart);
     }
   };
-  V va0[kUnroll], va1[kUnroll], vb0[kUnroll], vb1[kUnroll];
-  request(first, va0, va1);
+  request();
 
-  float2* slab = slabs + warp * (p.rotary / 2);
+  const int half = slab_part(p.rotary);
+  float* slab = slabs + warp * 2 * half;
   angles(p, b, tok, lane, slab);
-  // Of this lane's N pairs (a, d): a' = a ca - d sd, d' = a sa + d cd, with the
+
+  // Of this lane's N pairs (a, d): a' = a ca + d nd, d' = a sa + d cd, with the
   // norm's weights of their channels multiplied in (plain channels: 1, 0, 0, 1).
-  float ca[N], sd[kNorm ? N : 1], sa[N], cd[kNorm ? N : 1];
-  auto coefficients = [&](int which) {
-    float w[2 * N];
+  Two ca[P], nd[kNorm ? P : 1], sa[P], cd[kNorm ? P : 1];
+  auto coefficients = [&] {
+    float w[2 * N], c[N], s[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) c[i] = 1.f, s[i] = 0.f;
+    if (turned0) {
+      load_floats<N>(slab + N * sub, c);
+      load_floats<N>(slab + half + N * sub, s);
+    }
+    if (!turned1) {
+#pragma unroll
+      for (int i = N / 2; i < N; ++i) c[i] = 1.f, s[i] = 0.f;
+    }
     if (kNorm) {
 #pragma unroll
       for (int i = 0; i < 2 * N; ++i) w[i] = 1.f;
@@ -218,83 +294,99 @@ __global__ void __launch_bounds__(32 * kWarps, kNorm ? 6 : 8) head_rotary_kernel
       }
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float2 cs = make_float2(1.f, 0.f);
-      if (kInterleaved) {
-        const int c = i < N / 2 ? c0 : c1;
-        if (c < p.rotary) cs = slab[c / 2 + (i & (N / 2 - 1))];
-      } else if (c0 < p.rotary) {
-        cs = slab[c0 + i];
-      }
-      ca[i] = cs.x;
-      sa[i] = cs.y;
+    for (int j = 0; j < P; ++j) {
+      const Two cc = two(c[2 * j], c[2 * j + 1]), ss = two(s[2 * j], s[2 * j + 1]);
+      ca[j] = cc, sa[j] = ss;
       if (kNorm) {
-        const float wa = w[kInterleaved ? 2 * i : i], wd = w[kInterleaved ? 2 * i + 1 : N + i];
-        ca[i] = cs.x * wa;
-        sa[i] = cs.y * wa;
-        cd[i] = cs.x * wd;
-        sd[i] = cs.y * wd;
+        const Two ns = two(-s[2 * j], -s[2 * j + 1]);
+        const Two wa = two(w[first_of(2 * j)], w[first_of(2 * j + 1)]);
+        const Two wd = two(w[second_of(2 * j)], w[second_of(2 * j + 1)]);
+        ca[j] = mul(cc, wa), sa[j] = mul(ss, wa), cd[j] = mul(cc, wd), nd[j] = mul(ns, wd);
       }
     }
   };
-  int have = -1;
-  auto turn = [&](int it, const V (&v0)[kUnroll], const V (&v1)[kUnroll]) {
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (it + u >= last) break;  // the same for the whole warp
-      int which, head;
-      place(it + u, which, head);
-      if (kNorm ? which != have : have < 0) {
-        coefficients(which);
-        have = which;
-      }
-      float x[2 * N];
-      v0[u].unpack(x);
-      v1[u].unpack(x + N);
-      float r = 1.f;
-      if (kNorm) {
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 2 * N; ++i) sum = fmaf(x[i], x[i], sum);
-        for (int d = 1; d < p.lanes; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        r = rsqrtf(fmaf(sum, p.inv_dim, p.eps[which]));
-      }
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        float& a = kInterleaved ? x[2 * i] : x[i];
-        float& d = kInterleaved ? x[2 * i + 1] : x[N + i];
-        if (kNorm) {
-          a *= r;
-          d *= r;
-        }
-        // channels that are not turned pass as they are (0 * inf is NaN)
-        const bool turned = kInterleaved ? (i < N / 2 ? c0 : c1) < p.rotary : c0 < p.rotary;
-        const float a0 = a, d0 = d;
-        if (turned) {
-          a = a0 * ca[i] - d0 * (kNorm ? sd[kNorm ? i : 0] : sa[i]);
-          d = a0 * sa[i] + d0 * (kNorm ? cd[kNorm ? i : 0] : ca[i]);
-        } else if (kNorm) {
-          a = a0 * ca[i];
-          d = d0 * cd[kNorm ? i : 0];
-        }
-      }
-      if (head < p.heads[which]) {
-        T* dst = static_cast<T*>(p.out[which]) + b * p.out_bs[which] + tok * p.out_ts[which] +
-                 head * p.out_hs[which];
-        V y;
-        y.pack(x);
-        if (has0) *reinterpret_cast<V*>(dst + c0) = y;
-        y.pack(x + N);
-        if (has1) *reinterpret_cast<V*>(dst + c1) = y;
-      }
-    }
-  };
+
+  coefficients();
+  char* dst = const_cast<char*>(place(p.out[which], p.out_bs, p.out_token, p.out_head));
+
 #pragma unroll 1
-  for (int it = first; it < last; it += 2 * kUnroll) {
-    request(it + kUnroll, vb0, vb1);
-    turn(it, va0, va1);
-    request(it + 2 * kUnroll, va0, va1);
-    turn(it + kUnroll, vb0, vb1);
+  for (int it = first; it < last; ++it) {  // the same for the whole warp
+    Two a[P], d[P];
+    {
+      float x[2 * N];
+      v0.unpack(x);
+      v1.unpack(x + N);
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        a[j] = two(x[first_of(2 * j)], x[first_of(2 * j + 1)]);
+        d[j] = two(x[second_of(2 * j)], x[second_of(2 * j + 1)]);
+      }
+    }
+    const bool live = head < p.heads[which];
+    const float eps = kNorm ? p.eps[which] : 0.f;
+    if (it + 1 < last) {
+      head += per;
+      src += p.in_step[which];
+      if (it + 1 == p.iters[0]) {
+        which = 1;
+        head = slot;
+        src = place(p.in[1], p.in_bs, p.in_token, p.in_head);
+      }
+      request();
+    }
+    if (kNorm) {
+      Two s0 = mul(a[0], a[0]), s1 = mul(d[0], d[0]);
+#pragma unroll
+      for (int j = 1; j < P; ++j) s0 = fma(a[j], a[j], s0), s1 = fma(d[j], d[j], s1);
+      float t0, t1, t2, t3;
+      split(s0, t0, t1);
+      split(s1, t2, t3);
+      float sum = (t0 + t1) + (t2 + t3);
+      for (int m = 1; m < p.lanes; m <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+      const float r = rsqrtf(fmaf(sum, p.inv_dim, eps));
+      const Two rr = two(r, r);
+#pragma unroll
+      for (int j = 0; j < P; ++j) a[j] = mul(a[j], rr), d[j] = mul(d[j], rr);
+    }
+    float y[2 * N];
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      Two e = mul(a[j], ca[j]), f = mul(d[j], kNorm ? cd[kNorm ? j : 0] : ca[j]);
+      // channels that are not turned pass as they are (0 * inf is NaN)
+      const bool turned = j < N / 4 || N < 4 ? turned0 : turned1;
+      if (kNorm && turned) f = fma(a[j], sa[j], f);
+      if (kNorm && turned) e = fma(d[j], nd[kNorm ? j : 0], e);
+      float &e0 = y[first_of(2 * j)], &e1 = y[first_of(2 * j + 1)];
+      split(e, e0, e1);
+      if (!kNorm && turned) {  // a factor's sign costs nothing here, a register above
+        float d0, d1, s0, s1;
+        split(d[j], d0, d1);
+        split(sa[j], s0, s1);
+        e0 = fmaf(d0, -s0, e0);
+        e1 = fmaf(d1, -s1, e1);
+      }
+      float &f0 = y[second_of(2 * j)], &f1 = y[second_of(2 * j + 1)];
+      split(f, f0, f1);
+      if (!kNorm && turned) {
+        float a0, a1, s0, s1;
+        split(a[j], a0, a1);
+        split(sa[j], s0, s1);
+        f0 = fmaf(a0, s0, f0);
+        f1 = fmaf(a1, s1, f1);
+      }
+    }
+    if (live) {
+      V out;
+      out.pack(y);
+      if (has0) *reinterpret_cast<V*>(dst) = out;
+      out.pack(y + N);
+      if (has1) *reinterpret_cast<V*>(dst + apart) = out;
+    }
+    dst += p.out_step[which];
+    if (it + 1 == p.iters[0] && it + 1 < last) {  // keys from here on
+      dst = const_cast<char*>(place(p.out[1], p.out_bs, p.out_token, p.out_head));
+      if (kNorm) coefficients();
+    }
   }
 }
 
@@ -304,15 +396,16 @@ __global__ void __launch_bounds__(32 * kWarps, kNorm ? 6 : 8) head_rotary_kernel
 // L1); every lane has the sum before any lane writes, so in-place calls hold.
 template <typename T, bool kNorm, bool kInterleaved>
 __global__ void __launch_bounds__(32 * kWarps) head_rotary_scalar_kernel(const Params p) {
-  extern __shared__ float2 slabs[];
+  extern __shared__ __align__(16) float slabs[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long item = static_cast<long long>(blockIdx.x) * kWarps + warp;
+  if (item >= p.items) return;
   const long long token = item / p.chunks;
-  if (token >= static_cast<long long>(p.batch) * p.tokens) return;
   const int part = static_cast<int>(item - token * p.chunks);
   const int b = static_cast<int>(token / p.tokens);
   const int tok = static_cast<int>(token - static_cast<long long>(b) * p.tokens);
-  float2* slab = slabs + warp * (p.rotary / 2);
+  const int half_slab = slab_part(p.rotary);
+  float* slab = slabs + warp * 2 * half_slab;
   angles(p, b, tok, lane, slab);
   const int first = part * p.chunk, last = min(first + p.chunk, p.heads[0] + p.heads[1]);
 #pragma unroll 1
@@ -346,21 +439,30 @@ __global__ void __launch_bounds__(32 * kWarps) head_rotary_scalar_kernel(const P
     for (int i = lane; i < p.rotary / 2; i += 32) {
       const int a = kInterleaved ? 2 * i : i, d = kInterleaved ? 2 * i + 1 : i + p.rotary / 2;
       const float x0 = value(a), x1 = value(d);
-      const float2 cs = slab[i];
-      dst[a] = Value<T>::round(x0 * cs.x - x1 * cs.y);
-      dst[d] = Value<T>::round(x0 * cs.y + x1 * cs.x);
+      const float c = slab[i], s = slab[half_slab + i];
+      dst[a] = Value<T>::round(x0 * c - x1 * s);
+      dst[d] = Value<T>::round(x0 * s + x1 * c);
     }
     for (int c = p.rotary + lane; c < p.dim; c += 32) dst[c] = Value<T>::round(value(c));
   }
 }
 
-// Chunks of N fit when every head starts on their size, the head is a whole number
-// of them (at most two a lane) and no chunk holds both turned and other channels or,
-// in the half layout, channels of both halves.
+// Chunks of N fit when every head and the norm's weights start on their size, the head
+// is a whole number of them (at most two a lane) and no chunk holds both turned and
+// other channels or, in the half layout, channels of both halves.  Chunks of two pairs
+// in the interleaved layout are turned together, so both are or neither is.  Steps
+// from token to token and from head group to head group have 32 bits.
 template <typename T, int N>
 bool chunks_fit(const Params& p, bool interleaved) {
+  for (int w = 0; w < 2; ++w) {
+    for (long long n : {p.in_ts[w], p.out_ts[w], 32 * p.in_hs[w], 32 * p.out_hs[w]})
+      if (n < 0 || n > 0x7fffffffLL / 4) return false;
+  }
   return (p.addresses & (N * sizeof(T) - 1)) == 0 && (p.strides & (N - 1)) == 0 && p.dim % N == 0 &&
-         p.dim <= 64 * N && p.rotary % (interleaved ? N : 2 * N) == 0;
+         p.dim <= 64 * N && p.rotary % (interleaved && N != 2 ? N : 2 * N) == 0 &&
+         (p.weights & (N * (p.weight_fp32 ? 4 : sizeof(T)) < 16
+                           ? N * (p.weight_fp32 ? 4 : sizeof(T)) - 1
+                           : 15)) == 0;
 }
 
 // A warp walks over all head groups of a token, unless that leaves the device short
@@ -371,7 +473,8 @@ int share_tokens(Params& p, unsigned* blocks) {
   const long long share = tokens * iters / (148 * 32);
   p.chunk = static_cast<int>(share < 1 ? 1 : share > iters ? iters : share);
   p.chunks = (iters + p.chunk - 1) / p.chunk;
-  const long long n = (tokens * p.chunks + kWarps - 1) / kWarps;
+  p.items = tokens * p.chunks;
+  const long long n = (p.items + kWarps - 1) / kWarps;
   if (n > 0x7fffffffLL) return kErrTooLarge;
   *blocks = static_cast<unsigned>(n);
   return kErrOk;
@@ -384,7 +487,16 @@ int launch_chunks(Params p, size_t smem, cudaStream_t stream) {
   p.log2_lanes = 0;
   while (p.lanes < tasks) p.lanes *= 2, ++p.log2_lanes;
   const int per = 32 / p.lanes;
-  for (int w = 0; w < 2; ++w) p.iters[w] = (p.heads[w] + per - 1) / per;
+  for (int w = 0; w < 2; ++w) {
+    p.iters[w] = (p.heads[w] + per - 1) / per;
+    auto bytes = [](long long n) { return static_cast<unsigned>(n * sizeof(T)); };
+    p.in_token[w] = bytes(p.in_ts[w]);
+    p.out_token[w] = bytes(p.out_ts[w]);
+    p.in_head[w] = bytes(p.in_hs[w]);
+    p.out_head[w] = bytes(p.out_hs[w]);
+    p.in_step[w] = bytes(p.in_hs[w] * per);
+    p.out_step[w] = bytes(p.out_hs[w] * per);
+  }
   unsigned blocks;
   if (int rc = share_tokens(p, &blocks)) return rc;
   head_rotary_kernel<T, N, kNorm, kInterleaved><<<blocks, 32 * kWarps, smem, stream>>>(p);
@@ -395,7 +507,7 @@ int launch_chunks(Params p, size_t smem, cudaStream_t stream) {
 template <typename T, bool kNorm, bool kInterleaved>
 int launch(Params p, cudaStream_t stream) {
   constexpr int N = static_cast<int>(16 / sizeof(T));
-  const size_t smem = static_cast<size_t>(kWarps) * (p.rotary / 2) * sizeof(float2);
+  const size_t smem = static_cast<size_t>(kWarps) * 2 * slab_part(p.rotary) * sizeof(float);
   if (chunks_fit<T, N>(p, kInterleaved))
     return launch_chunks<T, N, kNorm, kInterleaved>(p, smem, stream);
   if (chunks_fit<T, N / 2>(p, kInterleaved))
@@ -416,7 +528,8 @@ int launch(Params p, cudaStream_t stream) {
 
 template <typename T>
 int dispatch(const Params& p, bool norm, bool interleaved, cudaStream_t stream) {
-  if (norm) return interleaved ? launch<T, true, true>(p, stream) : launch<T, true, false>(p, stream);
+  if (norm)
+    return interleaved ? launch<T, true, true>(p, stream) : launch<T, true, false>(p, stream);
   return interleaved ? launch<T, false, true>(p, stream) : launch<T, false, false>(p, stream);
 }
 
@@ -481,6 +594,7 @@ extern "C" int erd_head_norm_rotary(const erd_head_norm_rotary_args* args, void*
   p.pos_ts = a.pos_stride[2];
   p.start = a.start;
   p.addresses = all;
+  p.weights = a.norm ? weights : 0;
   for (int i = 0; i < 3; ++i) {
     p.strides |= a.q_stride[i] | a.q_out_stride[i];
     if (a.k_heads > 0) p.strides |= a.k_stride[i] | a.k_out_stride[i];
