@@ -492,16 +492,16 @@ struct PairTile {
   bool wide;
 };
 __device__ __forceinline__ PairTile pair_tile(const PairParams& p, int item) {
-  const bool wide = item < p.wide;
-  const int tile = wide ? item : p.wide + ((item - p.wide) >> 1);
+  const bool whole = item < p.wide;
+  const int tile = whole ? item : p.wide + ((item - p.wide) >> 1);
   const int band = tile / (kBand * p.tiles_n);
   const int rows = min(kBand, p.tiles_m - band * kBand);
   const int r = tile - band * kBand * p.tiles_n;
   const int tn = r / rows;
   PairTile t;
-  t.wide = wide;
   t.m0 = (band * kBand + r - tn * rows) * kPairRows;
-  t.n0 = tn * 256 + (wide ? 0 : ((item - p.wide) & 1) * 128);
+  t.n0 = tn * 256 + (whole ? 0 : ((item - p.wide) & 1) * 128);
+  t.wide = whole && p.e.n - t.n0 > 128;  // a narrow last column is a narrow tile
   return t;
 }
 
@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     if (elect_one()) {
       tma_prefetch_desc(&tmap_a);
       tma_prefetch_desc(&tmap_b);
-      if (p.items > p.wide) tma_prefetch_desc(&tmap_b_half);
+      tma_prefetch_desc(&tmap_b_half);
       RingPlace at;
       uint32_t issued = 0;
       bool ok = true;
@@ -595,7 +595,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       uint32_t count = 0;
       bool ok = true;
       for (int item = pair; ok && item < p.items; item += pairs, ++count) {
-        const uint32_t id = item < p.wide ? idesc<kBf16>(256, 256) : idesc<kBf16>(256, 128);
+        const uint32_t id =
+            pair_tile(p, item).wide ? idesc<kBf16>(256, 256) : idesc<kBf16>(256, 128);
         const uint32_t buf = count & 1;
         if (!mbar_wait(smem_u32(&bars->acc_empty[buf]), ((count >> 1) & 1) ^ 1, abort, p.status,
                        kStatusTimeoutMma)) {
