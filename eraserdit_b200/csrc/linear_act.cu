@@ -300,7 +300,7 @@ struct Piece {
   bool inside;     // every row and column exists and rows start on 16 bytes
   bool one_group;  // the 32 rows share a gate
   int group;
-  float b[2], g[2];
+  T b[2], g[2];  // as they are: a conversion here would wait for them
   uint4 res[8];
 
   __device__ __forceinline__ void request(const Epilogue& e, int row, int col, int lane) {
@@ -317,12 +317,12 @@ struct Piece {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int c = col + lane + 32 * i;
-      b[i] = 0.f;
-      g[i] = 1.f;
+      b[i] = T(0.f);
+      g[i] = T(1.f);
       if (c < e.n) {
-        if (e.bias != nullptr) b[i] = to_float(static_cast<const T*>(e.bias)[c]);
+        if (e.bias != nullptr) b[i] = static_cast<const T*>(e.bias)[c];
         if (e.gate != nullptr && one_group)
-          g[i] = to_float(static_cast<const T*>(e.gate)[static_cast<long long>(group) * e.n + c]);
+          g[i] = static_cast<const T*>(e.gate)[static_cast<long long>(group) * e.n + c];
       }
     }
     if (e.residual != nullptr) {
@@ -360,8 +360,8 @@ struct Piece {
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      slab[lane + 32 * i] = b[i];
-      slab[kPiece + lane + 32 * i] = g[i];
+      slab[lane + 32 * i] = to_float(b[i]);
+      slab[kPiece + lane + 32 * i] = to_float(g[i]);
     }
     __syncwarp();
   }
