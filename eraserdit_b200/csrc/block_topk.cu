@@ -13,13 +13,13 @@
 //   pool_kernel     one pass over k (and, for blocks of 128, q): block sums.
 //                   Bound by memory; a caller that keeps the key means next to
 //                   its keys (key_pool) skips it for single queries.
+//   few_blocks_kernel   blocks of 128, at most 64 key blocks: scores and choice.
 //   score_kernel    blocks of 128: scores = sums times means, FP64 tiles.
 //   select_kernel   blocks of 128: one warp a row finds the topk-th key by
 //                   bisection over the bits of the scores.
-//   row_select_kernel   single queries: scores and choice in one CTA a row.
 //   tile_attn_kernel    blocks of 128: tcgen05 attention over the chosen blocks.
-//   row_attn_kernel     single queries: a stream over the chosen blocks, split
-//                   over a cluster when there are few rows.
+//   row_kernel      single queries: scores, choice and a stream over the chosen
+//                   blocks, split over a cluster when there are few rows.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -387,6 +387,66 @@ __global__ void __launch_bounds__(32 * kSelectWarps)
   const double* s = scores + row * blocks;
   select_topk<kPer>([&](int i) { return s[i]; }, n, min(topk, n), topk,
                     selection + row * topk, threadIdx.x & 31);
+}
+
+// Scores and choice in one kernel where a row's scores are one tile (64 blocks): 16
+// query blocks a CTA, 16 x 16 scores and then four rows a warp.  One launch and one
+// round trip through memory less: the whole call for 3 x 2005 queries and keys of 8
+// heads with 16 blocks 38.4 -> 34.0 us, for 3 x 128 queries of 32 heads and 64 blocks
+// 31.6 -> 24.8.  (With 64 rows a CTA each warp would choose for 16 rows in turn.)
+constexpr int kFewGroups = 16;
+__global__ void __launch_bounds__(128)
+    few_blocks_kernel(const double* q_sum, const double* k_mean, int* selection,
+                      const int* lengths, int heads, int per, int groups, int blocks, int kv_len,
+                      int key_block, int topk) {
+  __shared__ double sq[kFewGroups * kScorePitch], sk[kScoreTile * kScorePitch];
+  const int g0 = blockIdx.x * kFewGroups, bh = blockIdx.y;
+  const int b = bh / heads, h = bh - b * heads;
+  const long long kv = static_cast<long long>(b) * (heads / per) + h / per;
+  const double* qg = q_sum + static_cast<long long>(bh) * groups * kDim;
+  const double* kg = k_mean + kv * blocks * kDim;
+  start_next();
+  wait_previous();
+  for (int i = threadIdx.x; i < (kFewGroups + kScoreTile) * kDim / 2; i += 128) {
+    const int r = i / (kDim / 2), c = i % (kDim / 2) * 2;
+    double2 v = make_double2(0.0, 0.0);
+    if (r < kFewGroups) {
+      if (g0 + r < groups)
+        v = *reinterpret_cast<const double2*>(qg + (g0 + r) * static_cast<long long>(kDim) + c);
+      *reinterpret_cast<double2*>(sq + r * kScorePitch + c) = v;
+    } else {
+      const int n = r - kFewGroups;
+      if (n < blocks) v = *reinterpret_cast<const double2*>(kg + n * kDim + c);
+      *reinterpret_cast<double2*>(sk + n * kScorePitch + c) = v;
+    }
+  }
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  double acc[2][2][2] = {};
+  const double* qa = sq + lane / 4 * kScorePitch + lane % 4;
+  const double* kb = sk + (warp * 16 + lane / 4) * kScorePitch + lane % 4;
+#pragma unroll 4
+  for (int d = 0; d < kDim; d += 4) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        mma_f64(acc[i][j], qa[i * 8 * kScorePitch + d], kb[j * 8 * kScorePitch + d]);
+  }
+  __syncthreads();  // the query sums give way to the scores
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      *reinterpret_cast<double2*>(sq + (i * 8 + lane / 4) * kScorePitch + warp * 16 + j * 8 +
+                                  lane % 4 * 2) = make_double2(acc[i][j][0], acc[i][j][1]);
+  __syncthreads();
+  const int n = (key_length(lengths, b, kv_len) + key_block - 1) / key_block;
+  for (int r = warp; r < kFewGroups && g0 + r < groups; r += 4) {
+    const double* s = sq + r * kScorePitch;
+    select_topk<2>([&](int i) { return s[i]; }, n, min(topk, n), topk,
+                   selection + (static_cast<long long>(bh) * groups + g0 + r) * topk, lane);
+  }
 }
 
 // -------------------------------------------------- attention of 128-row tiles
@@ -1186,26 +1246,38 @@ int run(const Call& c, cudaStream_t st) {
       return rc;
   }
   if (tiles) {
-    cudaError_t e = cudaFuncSetAttribute(
-        score_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kScoreSmem);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    const dim3 grid((blocks + kScoreTile - 1) / kScoreTile, (groups + kScoreTile - 1) / kScoreTile,
-                    static_cast<unsigned>(c.batch * c.q_heads));
-    Config score(grid, 128, kScoreSmem, st);
-    e = cudaLaunchKernelEx(&score.follow().cfg, score_kernel, static_cast<const double*>(q_sum),
-                           pool, scores, c.q_heads, per, groups, blocks);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    const long long per_batch = static_cast<long long>(c.q_heads) * groups;
-    const long long rows = c.batch * per_batch;
-    const unsigned ctas = static_cast<unsigned>((rows + kSelectWarps - 1) / kSelectWarps);
-    auto select = blocks <= 32 * 8 ? select_kernel<8>
-                  : blocks <= 32 * 16 ? select_kernel<16>
-                  : blocks <= 32 * 32 ? select_kernel<32> : select_kernel<0>;
-    Config choose(dim3(ctas), 32 * kSelectWarps, 0, st);
-    e = cudaLaunchKernelEx(&choose.follow().cfg, select, static_cast<const double*>(scores),
-                           c.selection, c.lengths, rows, per_batch, blocks, c.kv_len, c.key_block,
-                           c.topk);
-    if (e != cudaSuccess) return static_cast<int>(e);
+    cudaError_t e;
+    if (blocks <= kScoreTile) {
+      Config choose(dim3((groups + kFewGroups - 1) / kFewGroups,
+                         static_cast<unsigned>(c.batch * c.q_heads)),
+                    128, 0, st);
+      e = cudaLaunchKernelEx(&choose.follow().cfg, few_blocks_kernel,
+                             static_cast<const double*>(q_sum), pool, c.selection, c.lengths,
+                             c.q_heads, per, groups, blocks, c.kv_len, c.key_block, c.topk);
+      if (e != cudaSuccess) return static_cast<int>(e);
+    } else {
+      e = cudaFuncSetAttribute(
+          score_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kScoreSmem);
+      if (e != cudaSuccess) return static_cast<int>(e);
+      const dim3 grid((blocks + kScoreTile - 1) / kScoreTile,
+                      (groups + kScoreTile - 1) / kScoreTile,
+                      static_cast<unsigned>(c.batch * c.q_heads));
+      Config score(grid, 128, kScoreSmem, st);
+      e = cudaLaunchKernelEx(&score.follow().cfg, score_kernel, static_cast<const double*>(q_sum),
+                             pool, scores, c.q_heads, per, groups, blocks);
+      if (e != cudaSuccess) return static_cast<int>(e);
+      const long long per_batch = static_cast<long long>(c.q_heads) * groups;
+      const long long rows = c.batch * per_batch;
+      const unsigned ctas = static_cast<unsigned>((rows + kSelectWarps - 1) / kSelectWarps);
+      auto select = blocks <= 32 * 8 ? select_kernel<8>
+                    : blocks <= 32 * 16 ? select_kernel<16>
+                    : blocks <= 32 * 32 ? select_kernel<32> : select_kernel<0>;
+      Config choose(dim3(ctas), 32 * kSelectWarps, 0, st);
+      e = cudaLaunchKernelEx(&choose.follow().cfg, select, static_cast<const double*>(scores),
+                             c.selection, c.lengths, rows, per_batch, blocks, c.kv_len, c.key_block,
+                             c.topk);
+      if (e != cudaSuccess) return static_cast<int>(e);
+    }
     CUtensorMap tq, tk, tv;
     if (operand_map(&tq, kBf16, c.q, c.q_len, c.q_heads, c.batch, c.q_st, kTile) ||
         operand_map(&tk, kBf16, c.k, c.kv_len, c.kv_heads, c.batch, c.k_st, kHalf) ||

@@ -182,6 +182,17 @@ def test_ties_go_to_the_lowest_index(query_block, blocks, topk):
     _check(out, sel, q, k, v, topk, query_block, 64)
 
 
+@pytest.mark.parametrize("q_len", [1, 2048, 2177])
+@pytest.mark.parametrize("kv_len", [4032, 4096, 4097])
+def test_rows_of_one_tile_of_scores_and_of_two(q_len, kv_len):
+    """63, 64 and 65 key blocks; one, 16 and 18 query blocks."""
+    q, k, v = _inputs(2, q_len, kv_len, 2, 1, torch.bfloat16, q_len + kv_len)
+    lengths = torch.tensor([kv_len, 1000], device="cuda", dtype=torch.int32)
+    for given in (None, lengths):
+        out, sel = _run(q, k, v, 40, query_block=128, key_lengths=given)
+        _check(out, sel, q, k, v, 40, 128, 64, lengths=given)
+
+
 def test_large_scores_and_far_rows():
     """Sharp softmaxes (scores of several hundred, so the running maximum moves);
     scales that masked keys' -inf cannot be multiplied with are refused."""
