@@ -115,6 +115,38 @@ def test_norm_and_rotation_match_formula(dtype, layout, dim, rotary_dim, weights
     _close(qn, _want(q, weight=norms[0].weight, eps=1e-6))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dim,rotary_dim", [(44, 40), (80, 12), (16, 8), (24, 6), (60, 60), (6, 2)])
+@pytest.mark.parametrize("offset", [0, 1, 2, 4])
+def test_every_width_of_reads(dtype, layout, dim, rotary_dim, offset):
+    """Heads and weights that allow 16, 8 and 4 bytes at a time or single values, with
+    plain channels beside turned ones in a lane; infinities in plain channels of the
+    rotation stay."""
+    from eraserdit_b200.operator_fusion import apply_fused_qk_head_rmsnorm_rotary
+    from eraserdit_b200.rotary import RotaryPositions, apply_rotary
+    rotary = RotaryPositions(dim, rotary_dim=rotary_dim, layout=layout)
+    q, k = _randn((2, 11, 7, dim), dtype, 13), _randn((2, 11, 2, dim), dtype, 14)
+    norms = []
+    for seed in (15, 16):
+        n = torch.nn.RMSNorm(dim, eps=1e-6, device="cuda", dtype=dtype).requires_grad_(False)
+        n.weight.data = _randn((dim + 8,), dtype, seed)[offset:offset + dim]
+        norms.append(n)
+    pos = _pos(2, 11, start=70)
+    qo, ko = apply_fused_qk_head_rmsnorm_rotary(q, k, *norms, rotary, 70)
+    _close(qo, _want(q, rotary, pos, weight=norms[0].weight, eps=1e-6))
+    _close(ko, _want(k, rotary, pos, weight=norms[1].weight, eps=1e-6))
+    wide = _randn((2, 11, 7, dim + 8), dtype, 17)
+    q = wide[..., offset:offset + dim]
+    if rotary_dim < dim:
+        q[0, 0, 0, rotary_dim:] = math.inf
+    qo, ko = apply_rotary(q, k, rotary, 70)
+    _close(qo[1], tuple(t[1] for t in _want(q, rotary, pos)))
+    _close(qo[..., :rotary_dim], tuple(t[..., :rotary_dim] for t in _want(q, rotary, pos)))
+    _close(ko, _want(k, rotary, pos))
+    assert torch.equal(qo[..., rotary_dim:], q[..., rotary_dim:])
+
+
 @pytest.mark.parametrize("tokens", [1, 2, 33, 1777])
 @pytest.mark.parametrize("heads,kv_heads", [(1, 1), (32, 8), (33, 1)])
 def test_views_of_a_projection_buffer_in_place(tokens, heads, kv_heads):

@@ -149,6 +149,25 @@ def test_views_and_in_place_residual(m):
     _check(own, x, w, b, "none", None, res)
 
 
+@pytest.mark.parametrize("m", [37, 200, 3001])
+@pytest.mark.parametrize("n", [65, 190, 1099, 1102])
+@pytest.mark.parametrize("res_at", [(0, 0), (2, 6), (1, 5), (3, 4)])
+@pytest.mark.parametrize("out_at", [(0, 0), (2, 6), (1, 5)])
+def test_rows_on_two_and_four_bytes(m, n, res_at, out_at):
+    """Residual and result whose rows start on 4 bytes or on 2, with even and odd
+    strides and numbers of columns; what lies around the result stays."""
+    from eraserdit_b200.linear import linear_act
+    x, w, b, gate, res = _operands(m, n, 136, torch.float16, m + n, groups=1, residual=True)
+    (ro, rp), (oo, op) = res_at, out_at  # columns in front, and in front and behind together
+    wide = torch.full((m, n + rp), 9.0, device="cuda", dtype=torch.float16)
+    wide[:, ro:ro + n] = res
+    buf = torch.full((m, n + op), 7.0, device="cuda", dtype=torch.float16)
+    out = buf[:, oo:oo + n]
+    linear_act(x, w, b, activation="silu", gate=gate, residual=wide[:, ro:ro + n], out=out)
+    _check(out, x, w, b, "silu", gate, res)
+    assert bool((buf[:, :oo] == 7.0).all()) and bool((buf[:, oo + n:] == 7.0).all())
+
+
 def test_leading_dimensions_and_slots():
     from eraserdit_b200.linear import linear_act
     x, w, b, gate, res = _operands(2 * 70, 136, 128, torch.bfloat16, 4, groups=2, residual=True)
