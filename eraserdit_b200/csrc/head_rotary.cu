@@ -201,13 +201,18 @@ __device__ __forceinline__ Two fma(Two a, Two b, Two c) {
 // addresses advance by a constant, and weights and angles are read 16 bytes at a time:
 // 121 and 167 a group.
 //
-// 32640 tokens with 64 values a head, rotation and norm with it: 64 heads 84 and 100 us
-// (6.4 and 5.4 TB/s; 86 and 107 before), 8 heads 22 and 34 us (3.0 and 1.9 TB/s; 24 and
-// 39 before; here the angles and coefficients of a token, used once or twice, are most
-// of the instructions).  Two head groups at a time, more or fewer warps, larger blocks,
-// several tokens a warp, and 8-byte chunks for the norm (twice the sums to wait for)
-// were slower.
-template <typename T, int N, bool kNorm, bool kInterleaved>
+// kAhead: a warp of eight groups or more also asks L2 for the group behind the next,
+// which costs no registers: what 24 warps of the norm have requested at a time does not
+// cover the memory's latency (101 -> 92 us for 64 heads below).  With fewer groups the
+// instructions weigh more than that (4 heads of queries and of keys 35.4 -> 36.7 us).
+//
+// 32640 tokens with 64 values a head, rotation and norm with it: 64 heads 82 and 92 us
+// (6.5 and 5.8 TB/s; 86 and 107 before all this), 8 heads 21 and 34 us (3.2 and 2.0
+// TB/s; 24 and 39 before; here the angles and coefficients of a token, used once or
+// twice, are most of the instructions).  Two head groups at a time, more or fewer
+// warps, larger blocks, several tokens a warp, and 8-byte chunks for the norm (twice
+// the sums to wait for) were slower.
+template <typename T, int N, bool kNorm, bool kInterleaved, bool kAhead>
 __global__ void __launch_bounds__(32 * kWarps, kNorm ? 6 : 8) head_rotary_kernel(const Params p) {
   using V = Chunk<T, N>;
   constexpr int P = N / 2;  // couples of this lane's N pairs
@@ -265,6 +270,16 @@ __global__ void __launch_bounds__(32 * kWarps, kNorm ? 6 : 8) head_rotary_kernel
     }
   };
   request();
+  // Asks L2 for group `next`, the one behind the requested one, unless it is of the
+  // other tensor.
+  auto prefetch = [&](int next) {
+    if (kAhead && next < last && next != p.iters[0] && head + per < p.heads[which]) {
+      const char* at = src + p.in_step[which];
+      if (has0) asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+      if (!kInterleaved && has1) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + apart));
+    }
+  };
+  prefetch(first + 1);
 
   const int half = slab_part(p.rotary);
   float* slab = slabs + warp * 2 * half;
@@ -333,6 +348,7 @@ __global__ void __launch_bounds__(32 * kWarps, kNorm ? 6 : 8) head_rotary_kernel
         src = place(p.in[1], p.in_bs, p.in_token, p.in_head);
       }
       request();
+      prefetch(it + 2);
     }
     if (kNorm) {
       Two s0 = mul(a[0], a[0]), s1 = mul(d[0], d[0]);
@@ -499,7 +515,14 @@ int launch_chunks(Params p, size_t smem, cudaStream_t stream) {
   }
   unsigned blocks;
   if (int rc = share_tokens(p, &blocks)) return rc;
-  head_rotary_kernel<T, N, kNorm, kInterleaved><<<blocks, 32 * kWarps, smem, stream>>>(p);
+  if constexpr (N * sizeof(T) == 16) {
+    if (p.chunk >= 8) {
+      head_rotary_kernel<T, N, kNorm, kInterleaved, true>
+          <<<blocks, 32 * kWarps, smem, stream>>>(p);
+      return static_cast<int>(cudaGetLastError());
+    }
+  }
+  head_rotary_kernel<T, N, kNorm, kInterleaved, false><<<blocks, 32 * kWarps, smem, stream>>>(p);
   return static_cast<int>(cudaGetLastError());
 }
 

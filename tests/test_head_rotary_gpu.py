@@ -147,6 +147,32 @@ def test_every_width_of_reads(dtype, layout, dim, rotary_dim, offset):
     assert torch.equal(qo[..., rotary_dim:], q[..., rotary_dim:])
 
 
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("tokens,heads,kv_heads", [(4600, 61, 17), (2501, 157, 13), (9500, 62, 0)])
+def test_many_heads_of_many_tokens(layout, norm, tokens, heads, kv_heads):
+    """Warps that walk over eleven or eight head groups, one or two warps a token, with
+    the keys behind the queries of one of them, in place."""
+    from eraserdit_b200.operator_fusion import apply_fused_qk_head_rmsnorm_rotary
+    from eraserdit_b200.rotary import RotaryPositions, apply_rotary
+    rotary = RotaryPositions(64, layout=layout)
+    q = _randn((1, tokens, heads, 64), torch.bfloat16, 18)
+    k = _randn((1, tokens, kv_heads, 64), torch.bfloat16, 19) if kv_heads else None
+    q0, k0 = q.clone(), None if k is None else k.clone()
+    w, eps = None, None
+    if norm:
+        n = torch.nn.RMSNorm(64, eps=1e-6, device="cuda", dtype=torch.bfloat16).requires_grad_(False)
+        n.weight.copy_(_randn((64,), torch.float32, 20))
+        w, eps = n.weight, 1e-6
+        apply_fused_qk_head_rmsnorm_rotary(q, k, n, n, rotary, 3, query_out=q, key_out=k)
+    else:
+        apply_rotary(q, k, rotary, 3, query_out=q, key_out=k)
+    pos = _pos(1, tokens, start=3)
+    _close(q, _want(q0, rotary, pos, weight=w, eps=eps))
+    if k is not None:
+        _close(k, _want(k0, rotary, pos, weight=w, eps=eps))
+
+
 @pytest.mark.parametrize("tokens", [1, 2, 33, 1777])
 @pytest.mark.parametrize("heads,kv_heads", [(1, 1), (32, 8), (33, 1)])
 def test_views_of_a_projection_buffer_in_place(tokens, heads, kv_heads):
