@@ -201,14 +201,16 @@ __device__ __forceinline__ Two fma(Two a, Two b, Two c) {
 // addresses advance by a constant, and weights and angles are read 16 bytes at a time:
 // 121 and 167 a group.
 //
-// kAhead: a warp of eight groups or more also asks L2 for the group behind the next,
-// which costs no registers: what 24 warps of the norm have requested at a time does not
-// cover the memory's latency (101 -> 92 us for 64 heads below).  With fewer groups the
-// instructions weigh more than that (4 heads of queries and of keys 35.4 -> 36.7 us).
+// kAhead, the norm with eight groups or more a warp: it also asks L2 for the group
+// behind the next, which costs no registers: what 24 warps have requested at a time
+// does not cover the memory's latency.  64 heads below 100 -> 90 us, in calls back to
+// back for a tenth of a second 202 -> 200 for two such clips.  With fewer groups the
+// instructions weigh more (4 heads of queries and of keys 35.4 -> 36.7 us), and the
+// rotation alone, whose 32 warps fill the memory, loses in a row of calls (169 -> 173).
 //
-// 32640 tokens with 64 values a head, rotation and norm with it: 64 heads 82 and 92 us
-// (6.5 and 5.8 TB/s; 86 and 107 before all this), 8 heads 21 and 34 us (3.2 and 2.0
-// TB/s; 24 and 39 before; here the angles and coefficients of a token, used once or
+// 32640 tokens with 64 values a head, rotation and norm with it: 64 heads 84 and 90 us
+// (6.4 and 5.9 TB/s; 86 and 107 before all this), 8 heads 22 and 35 us (3.0 and 1.9
+// TB/s; 25 and 40 before; here the angles and coefficients of a token, used once or
 // twice, are most of the instructions).  Two head groups at a time, more or fewer
 // warps, larger blocks, several tokens a warp, and 8-byte chunks for the norm (twice
 // the sums to wait for) were slower.
@@ -515,7 +517,7 @@ int launch_chunks(Params p, size_t smem, cudaStream_t stream) {
   }
   unsigned blocks;
   if (int rc = share_tokens(p, &blocks)) return rc;
-  if constexpr (N * sizeof(T) == 16) {
+  if constexpr (kNorm && N * sizeof(T) == 16) {
     if (p.chunk >= 8) {
       head_rotary_kernel<T, N, kNorm, kInterleaved, true>
           <<<blocks, 32 * kWarps, smem, stream>>>(p);
