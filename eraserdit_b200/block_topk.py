@@ -98,9 +98,10 @@ def block_topk_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Te
     or FP16.  ``query_block``: 128 or 1 consecutive queries that share a choice;
     ``key_block``: 64 or 128 keys.  ``key_lengths`` (int32 [B] on the device): keys
     from there on are left out, whatever they hold; a sequence without keys gives
-    zeros.  ``out`` may be ``query`` itself.  ``key_pool``: ``pool_key_blocks(key, key_block, key_lengths=...)`` that
-    the caller keeps, else computed here.  With ``return_selection`` also the chosen
-    blocks, int32 [B, H, query blocks, topk], ascending, -1 behind the last.
+    zeros.  ``out`` may be ``query`` itself.  ``key_pool``: what ``pool_key_blocks(key,
+    key_block, key_lengths=...)`` gave, kept by the caller; else computed here.  With
+    ``return_selection`` also the chosen blocks, int32 [B, H, query blocks, topk],
+    ascending, -1 behind the last.
     """
     for what, t in (("query", query), ("key", key), ("value", value)):
         _check_tensor(what, t)

@@ -430,8 +430,9 @@ int erd_attn_fwd_fp8_static_scratch(
  * pos_axis_stride + b * pos_batch_stride + t * pos_token_stride], or start + t
  * without positions; axis 1 serves the pairs from second_axis on, axis 2 those
  * from third_axis on (set both to rotary_dim / 2 for one axis).
- * Accesses are as wide (16, 8 or 4 bytes) as heads start and their turned parts
- * divide; any other size or stride is read value by value.
+ * Accesses are as wide (16, 8 or 4 bytes) as heads and weights start and their
+ * turned parts divide; any other size, and token strides of 2^29 elements or
+ * more, are read value by value.
  */
 typedef struct {
   int64_t struct_bytes; /* sizeof this struct, checked */
