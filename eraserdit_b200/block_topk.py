@@ -23,6 +23,7 @@ from . import _native
 HEAD_DIM = 64
 QUERY_BLOCKS = (1, 128)
 KEY_BLOCKS = (64, 128)
+MAX_TOPK = 0x7fff0000
 
 
 def _strides(what: str, t: torch.Tensor) -> tuple[int, int, int]:
@@ -115,8 +116,8 @@ def block_topk_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Te
         raise ValueError("query heads must be a positive multiple of the key heads")
     if query_block not in QUERY_BLOCKS or key_block not in KEY_BLOCKS:
         raise ValueError(f"query_block must be one of {QUERY_BLOCKS}, key_block of {KEY_BLOCKS}")
-    if not isinstance(topk, int) or not 1 <= topk < 2 ** 31:
-        raise ValueError("topk must be a positive int")
+    if not isinstance(topk, int) or not 1 <= topk <= MAX_TOPK:
+        raise ValueError(f"topk must be an int from 1 to {MAX_TOPK}")
     if not 0.0 < softmax_scale < float("inf"):
         raise ValueError("softmax_scale must be positive and finite")
     _check_lengths(key_lengths, key)

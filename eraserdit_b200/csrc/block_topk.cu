@@ -1368,7 +1368,7 @@ extern "C" int erd_block_topk_attn(const erd_block_topk_args* args, int* status,
     return kErrBadShape;
   if (a.batch > 65535 || a.q_heads > 65535 ||
       static_cast<long long>(a.batch) * a.q_heads > 65535 || a.kv_len > 0x7fff0000 ||
-      a.q_len > 0x7fff0000)
+      a.q_len > 0x7fff0000 || a.topk > 0x7fff0000)  // int indices step past these by 128 at most
     return kErrTooLarge;
   const btk::Sizes sz =
       btk::workspace_sizes(a.batch, a.q_heads, a.kv_heads, a.q_len, a.kv_len, a.query_block,

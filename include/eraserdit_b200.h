@@ -497,8 +497,8 @@ int erd_linear_act(const erd_linear_act_args* args, int* status, void* stream);
  * writes them, or NULL to compute them in this call.  selection: int32 [batch]
  * [q_heads][ceil(q_len / query_block)][topk], receives the chosen blocks in
  * ascending order, then -1.  `workspace` (16-byte aligned) holds at least
- * erd_block_topk_workspace_bytes(...) bytes.  batch * q_heads is at most 65535;
- * query_block 1 takes at most 18773 key blocks.
+ * erd_block_topk_workspace_bytes(...) bytes.  batch * q_heads is at most 65535,
+ * topk at most 0x7fff0000; query_block 1 takes at most 18773 key blocks.
  */
 size_t erd_block_topk_workspace_bytes(int batch, int q_heads, int kv_heads, int q_len, int kv_len,
                                       int query_block, int key_block, int has_pool);

@@ -61,3 +61,15 @@ def test_entries_reject_bad_arguments_before_any_device_call():
     assert means(k=None) == -1 and means(out=None) == -1
     assert means(dtype=2) == -2 and means(kb=63) == -2 and means(kv_len=0) == -2 and means(heads=0) == -2
     assert means(kt=4) == -3 and means(out=p + 8) == -3 and means(lengths=p + 1) == -3
+
+
+def test_topk_whose_loops_would_wrap_is_refused():
+    """The loops over topk run in steps of 32: an int32 index passes 2^31 behind the last
+    of them and the kernel would write in front of the selection."""
+    from eraserdit_b200 import _native
+    fn = _native.load().erd_block_topk_attn
+    p = 1 << 20
+    for qb in (1, 128):
+        for topk in (0x7fff0001, 0x7fffffe1, 0x7fffffff):
+            fields = (p, p, p, 0, 0, p, p, p, *([64] * 12), 1 << 20, 0, 1, 2, 1, 5, 70, 64, topk, qb, 64, 0.125)
+            assert fn(_native.pack("erd_block_topk_attn", *fields), None, None) == -6
