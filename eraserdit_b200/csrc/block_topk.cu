@@ -39,6 +39,10 @@ constexpr int kDim = 64;       // head_dim
 constexpr int kTile = 128;     // queries of a tile and keys of a step
 constexpr int kHalf = 64;      // keys that are loaded (and chosen) together at least
 
+// Most queries, keys and chosen blocks: the kernels' int indices step past these
+// by up to 512 (a pooling warp's requests).
+constexpr int kMaxCount = 0x7fff0000;
+
 // ------------------------------------------------------------ small helpers
 template <typename T>
 __device__ __forceinline__ float2 unpack2(uint32_t w);
@@ -1344,10 +1348,10 @@ extern "C" int erd_block_key_means(int dtype, const void* k, int64_t k_token_str
   if (!aligned16(k) || !aligned16(means) || !btk::strides_ok(st) ||
       (reinterpret_cast<uintptr_t>(key_lengths) & 3) != 0)
     return kErrMisaligned;
+  if (kv_len > btk::kMaxCount) return kErrTooLarge;
   if (int rc = check_device_sm100()) return rc;
   const btk::PoolParams p = {k, st, kv_heads, kv_len, key_block,
-                             static_cast<int>((kv_len + static_cast<long long>(key_block) - 1) / key_block),
-                             key_lengths, 1, means};
+                             (kv_len + key_block - 1) / key_block, key_lengths, 1, means};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dtype == ERD_BF16 ? btk::launch_pool<__nv_bfloat16>(&p, nullptr, batch, s)
                            : btk::launch_pool<__half>(&p, nullptr, batch, s);
@@ -1367,8 +1371,8 @@ extern "C" int erd_block_topk_attn(const erd_block_topk_args* args, int* status,
       !(a.softmax_scale > 0.f && a.softmax_scale <= 3.0e38f))
     return kErrBadShape;
   if (a.batch > 65535 || a.q_heads > 65535 ||
-      static_cast<long long>(a.batch) * a.q_heads > 65535 || a.kv_len > 0x7fff0000 ||
-      a.q_len > 0x7fff0000 || a.topk > 0x7fff0000)  // int indices step past these by 128 at most
+      static_cast<long long>(a.batch) * a.q_heads > 65535 || a.kv_len > btk::kMaxCount ||
+      a.q_len > btk::kMaxCount || a.topk > btk::kMaxCount)
     return kErrTooLarge;
   const btk::Sizes sz =
       btk::workspace_sizes(a.batch, a.q_heads, a.kv_heads, a.q_len, a.kv_len, a.query_block,

@@ -524,6 +524,7 @@ int erd_block_topk_attn(const erd_block_topk_args* args, int* status, void* stre
  * means [batch][kv_heads][ceil(kv_len / key_block)][64] (0 for a block without a
  * valid key).  A caller that keeps keys keeps these next to them and recomputes
  * only the blocks it appends to (a view of k from a block's first key on).
+ * kv_len is at most 0x7fff0000.
  */
 int erd_block_key_means(int dtype, const void* k, int64_t k_token_stride, int64_t k_head_stride,
                         int64_t k_batch_stride, int batch, int kv_heads, int kv_len, int key_block,

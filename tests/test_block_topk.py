@@ -73,3 +73,13 @@ def test_topk_whose_loops_would_wrap_is_refused():
         for topk in (0x7fff0001, 0x7fffffe1, 0x7fffffff):
             fields = (p, p, p, 0, 0, p, p, p, *([64] * 12), 1 << 20, 0, 1, 2, 1, 5, 70, 64, topk, qb, 64, 0.125)
             assert fn(_native.pack("erd_block_topk_attn", *fields), None, None) == -6
+
+
+def test_means_of_as_many_keys_as_would_wrap_are_refused():
+    """A block's end, first key + 64 (or 128), has to fit int32."""
+    from eraserdit_b200 import _native
+    fn = _native.load().erd_block_key_means
+    p = 1 << 20
+    for kb in (64, 128):
+        for kv_len in (0x7fff0001, 0x7fffffc1, 0x7fffffff):
+            assert fn(0, p, 64, 64, 64, 1, 1, kv_len, kb, None, p, None) == -6
