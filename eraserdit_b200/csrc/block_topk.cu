@@ -40,7 +40,7 @@ constexpr int kTile = 128;     // queries of a tile and keys of a step
 constexpr int kHalf = 64;      // keys that are loaded (and chosen) together at least
 
 // Most queries, keys and chosen blocks: the kernels' int indices step past these
-// by up to 512 (a pooling warp's requests).
+// by at most 128.
 constexpr int kMaxCount = 0x7fff0000;
 
 // ------------------------------------------------------------ small helpers
@@ -858,6 +858,10 @@ __global__ void __launch_bounds__(kTileThreads, 4)
 constexpr int kRowWarps = 8;
 constexpr int kRowKeys = 4;
 constexpr int kMaxSplits = 8;
+// Shared memory: arrays of fixed size (2376 bytes and their alignment), scores and choice.
+constexpr int kRowStatic = 4096;
+constexpr int kRowSmemMax = 220 * 1024;
+static_assert(kRowStatic + kRowSmemMax <= 227 * 1024, "shared memory of a CTA");
 
 struct RowParams {
   const void *q, *k, *v;
@@ -1300,9 +1304,12 @@ int run(const Call& c, cudaStream_t st) {
   const long long rows = static_cast<long long>(c.batch) * c.q_heads * c.q_len;
   const int most = c.topk < blocks ? c.topk : blocks;  // chosen blocks of a row
   const int smem = blocks * 8 + most * 4;
-  if (smem > 48 * 1024) {
+  // Above 48 KB, the kernel's own arrays among them, the size has to be allowed first.
+  // That is a property of the function, which calls of other threads set too: always
+  // the largest size, so that no call takes back what another one needs.
+  if (smem + kRowStatic > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(
-        row_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        row_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSmemMax);
     if (e != cudaSuccess) return static_cast<int>(e);
   }
   RowParams p = {c.q, c.k, c.v, c.q_st, c.k_st, c.v_st, c.o_st, c.out, c.lengths, pool,
@@ -1378,7 +1385,7 @@ extern "C" int erd_block_topk_attn(const erd_block_topk_args* args, int* status,
       btk::workspace_sizes(a.batch, a.q_heads, a.kv_heads, a.q_len, a.kv_len, a.query_block,
                            a.key_block, a.key_means != nullptr);
   const long long rows = static_cast<long long>(a.batch) * a.q_heads * sz.groups;
-  if (rows > (1LL << 27) || (a.query_block == 1 && sz.blocks * 12 > 220 * 1024) ||
+  if (rows > (1LL << 27) || (a.query_block == 1 && sz.blocks * 12 > btk::kRowSmemMax) ||
       (sz.groups + 63) / 64 > 65535)
     return kErrTooLarge;
   if (sz.total > 0 && a.workspace == nullptr) return kErrNullPointer;

@@ -350,3 +350,45 @@ def test_scores_that_are_not_finite(query_block, dtype):
     k[0, 150, 0, 5] = 0.0  # one finite score behind two blocks of -inf
     out, _ = _run(q, k, v, 3, query_block=query_block)
     assert torch.equal(out, v[:, 150:151].expand_as(out))
+
+
+def test_many_blocks_in_the_first_call_of_a_process():
+    """5816 and 6112 blocks with 64 chosen: scores and choice take just below 48 KB of
+    shared memory, which the kernel's own 2.4 KB lift above it."""
+    import subprocess
+    import sys
+    from tests.conftest import ROOT
+    code = ("import torch\n"
+            "from eraserdit_b200.block_topk import block_topk_attention\n"
+            "for n in (5816, 6112):\n"
+            "    k = torch.randn(1, n * 64, 1, 64, device='cuda').bfloat16()\n"
+            "    block_topk_attention(k[:, :1], k, k, 0.125, 64, query_block=1)\n"
+            "torch.cuda.synchronize()\n")
+    done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("blocks,topk", [(1536, 7), (1537, 64), (5815, 64), (5816, 64), (6112, 64), (6113, 64),
+                                         (18773, 64), (18773, 18773)])
+def test_single_queries_over_very_many_blocks(blocks, topk):
+    """The choice from shared memory instead of registers (above 1536 blocks), up to the
+    stated limit; one block more is refused."""
+    from eraserdit_b200.block_topk import block_topk_attention, pool_key_blocks
+    kv_len = blocks * 64 - 3
+    q, k, v = _inputs(1, 2, kv_len, 1, 1, torch.bfloat16, blocks)
+    pool = pool_key_blocks(k)
+    for given in (pool, None):
+        out, sel = _run(q, k, v, topk, query_block=1, key_pool=given)
+        _check(out, sel, q, k, v, topk, 1, 64)
+    # ties, so that the bits of the scores decide
+    k[:, 64:] = k[:, :64].repeat(1, blocks - 1, 1, 1)[:, :kv_len - 64]
+    _, sel = _run(q, k, v, topk, query_block=1)
+    full = torch.arange(topk, device="cuda", dtype=torch.int32)
+    if topk < blocks:  # every whole block scores alike; the last, shorter one may lead
+        assert bool(((sel == full) | ((full == topk - 1) & (sel == blocks - 1))).all())
+    else:
+        assert bool((sel == full).all())
+    if blocks == 18773:
+        more = torch.zeros(1, blocks * 64 + 1, 1, 64, device="cuda", dtype=torch.bfloat16)
+        with pytest.raises(RuntimeError):
+            block_topk_attention(q, more, more, SCALE, topk, query_block=1)
