@@ -133,6 +133,8 @@ def block_topk_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Te
         raise ValueError("out must have the query's shape, type and device")
     else:
         _native.refuse_overlap("out", out, (key, value, key_lengths, key_pool), query)
+    if not return_selection:  # no list is wider than the blocks there are
+        topk = min(topk, max(1, -(-kv_len // key_block)))
     selection = query.new_empty((batch, heads, groups, topk), dtype=torch.int32)
     if batch and q_len and kv_len:
         nbytes = 0

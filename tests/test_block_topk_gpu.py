@@ -392,3 +392,24 @@ def test_single_queries_over_very_many_blocks(blocks, topk):
         more = torch.zeros(1, blocks * 64 + 1, 1, 64, device="cuda", dtype=torch.bfloat16)
         with pytest.raises(RuntimeError):
             block_topk_attention(q, more, more, SCALE, topk, query_block=1)
+
+
+@pytest.mark.parametrize("query_block", [1, 128])
+def test_topk_far_above_the_blocks_costs_nothing(query_block):
+    """"All blocks" asked for by a large number: without the selection in the result no
+    list of that width is made."""
+    from eraserdit_b200.block_topk import MAX_TOPK, block_topk_attention
+    q, k, v = _inputs(2, 130, 700, 4, 2, torch.bfloat16, 15)
+    want = block_topk_attention(q, k, v, SCALE, 11, query_block=query_block)
+    for topk in (2 ** 20, MAX_TOPK):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        out = block_topk_attention(q, k, v, SCALE, topk, query_block=query_block)
+        assert torch.cuda.max_memory_allocated() - before < 1 << 21
+        assert torch.equal(out, want)
+    _, sel = block_topk_attention(q, k, v, SCALE, 5000, query_block=query_block, return_selection=True)
+    assert sel.shape[-1] == 5000 and bool((sel[..., 11:] == -1).all())
+    for topk in (MAX_TOPK + 1, 2 ** 31 - 1, 2 ** 40):
+        with pytest.raises(ValueError):
+            block_topk_attention(q, k, v, SCALE, topk, query_block=query_block)
