@@ -588,10 +588,11 @@ __device__ __forceinline__ void weigh(uint32_t tS, float c, float m, int n, uint
   sum = m_tile < CUDART_INF_F ? sum0 + sum1 : CUDART_NAN_F;
 }
 
-// First key of 64-key piece `i` of a tile's list.
+// First key of 64-key piece `i` of a tile's list.  (An ordinary read: the kernel that
+// writes the list may still run when this one starts.)
 __device__ __forceinline__ int piece_key(const TileParams& p, const int* list, int i) {
   const int shift = p.key_block >> 7;  // pieces of a block: 1 << shift
-  return __ldg(list + (i >> shift)) * p.key_block + (i & shift) * kHalf;
+  return list[i >> shift] * p.key_block + (i & shift) * kHalf;
 }
 
 // kind::f16 instruction descriptor with BF16 (format 1) or FP16 (format 0)

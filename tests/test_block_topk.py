@@ -83,3 +83,15 @@ def test_means_of_as_many_keys_as_would_wrap_are_refused():
     for kb in (64, 128):
         for kv_len in (0x7fff0001, 0x7fffffc1, 0x7fffffff):
             assert fn(0, p, 64, 64, 64, 1, 1, kv_len, kb, None, p, None) == -6
+
+
+def test_only_inputs_are_read_as_constant():
+    """Kernels of one call start before the one in front has ended, so what that one
+    writes (means, sums, scores, choice) is not constant while they run: of all
+    pointers only the lengths, complete before the call, are read with __ldg."""
+    import re
+    from tests.conftest import ROOT
+    text = (ROOT / "eraserdit_b200" / "csrc" / "block_topk.cu").read_text()
+    reads = re.findall(r"__ldg\(([^;]*)", text)
+    assert reads and all(r.startswith("lengths + b)") for r in reads)
+    assert "__restrict__" not in text  # which would let the compiler choose such reads
