@@ -168,8 +168,10 @@ def _head_norm(what: str, x: torch.Tensor, norm: Any) -> tuple[torch.Tensor | No
     if not isinstance(norm, torch.nn.RMSNorm) and getattr(norm, "bias", None) is not None:
         raise ValueError(f"{what}_norm must have no bias")
     eps = getattr(norm, "eps", None)
-    if eps is None:  # torch.nn.RMSNorm's default
-        eps = torch.finfo(x.dtype).eps
+    if eps is None:
+        if not isinstance(norm, torch.nn.RMSNorm):
+            raise ValueError(f"{what}_norm needs an eps")
+        eps = torch.finfo(torch.float32).eps  # its default, for 16-bit inputs too
     eps = float(eps)
     if not eps >= 0:
         raise ValueError(f"{what}_norm needs eps >= 0")
@@ -194,7 +196,7 @@ def apply_fused_qk_head_rmsnorm_rotary(query: torch.Tensor, key: torch.Tensor | 
 
     ``query_norm`` / ``key_norm``: objects with ``eps`` and a ``weight`` [D] (of
     the inputs' type or FP32; None for 1) without ``bias``, such as
-    ``torch.nn.RMSNorm(D)``.  ``rotary``: a :class:`RotaryPositions`, or None for
+    ``torch.nn.RMSNorm(D)``, whose default ``eps=None`` is FP32's epsilon.  ``rotary``: a :class:`RotaryPositions`, or None for
     the norm alone; ``positions`` as in ``rotary.apply_rotary``.  Norm and
     rotation are computed in FP32 and rounded once (``apply_fused_qk_rmsnorm_rope``,
     which normalises across all heads, rounds after each step as its reference

@@ -393,3 +393,37 @@ def test_overlapping_destinations_are_refused():
                dict(query_out=heads(4, 6), key_out=heads(5, 7))):
         with pytest.raises(ValueError):
             apply_rotary(heads(0, 2), heads(2, 4), rotary, 0, **kw)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rms", [1e-4, 0.05, 1.0])
+def test_a_norm_with_torchs_default_eps(dtype, rms):
+    """torch.nn.RMSNorm(D) without eps: FP32's epsilon for every type, as torch computes it."""
+    from eraserdit_b200.operator_fusion import apply_fused_qk_head_rmsnorm_rotary
+    eps = torch.finfo(torch.float32).eps
+    norm = torch.nn.RMSNorm(64, device="cuda", dtype=dtype).requires_grad_(False)
+    norm.weight.copy_(_randn((64,), torch.float32, 25))
+    q, k = (rms * _randn((2, 6, 3, 64), torch.float32, s).to(dtype) for s in (26, 27))
+    qo, ko = apply_fused_qk_head_rmsnorm_rotary(q, k, norm, norm, None)
+    for x, y in ((q, qo), (k, ko)):
+        _close(y, _want(x, weight=norm.weight, eps=eps))
+        # torch's own result: one more rounding where it rounds before the weight
+        torchs = torch.nn.functional.rms_norm(x, (64,), norm.weight).double()
+        assert bool(((y.double() - torchs).abs() <= 2 * torch.finfo(dtype).eps * torchs.abs()
+                     + 4 * NORM * torchs.abs() + 1e-30).all())
+
+
+def test_norms_without_an_eps_are_refused():
+    """Nothing stands in for an epsilon that goes by another name, or for no norm."""
+    from types import SimpleNamespace
+    from eraserdit_b200.operator_fusion import apply_fused_qk_head_rmsnorm_rotary
+    x = torch.zeros(2, 6, 4, 64, device="cuda", dtype=torch.bfloat16)
+    w = torch.ones(64, device="cuda", dtype=torch.bfloat16)
+    good = SimpleNamespace(weight=w, eps=1e-6)
+    apply_fused_qk_head_rmsnorm_rotary(x, x, good, good, None)
+    for bad in (None, SimpleNamespace(weight=w), SimpleNamespace(weight=w, eps=None),
+                SimpleNamespace(weight=w, variance_epsilon=1e-6)):
+        with pytest.raises(ValueError):
+            apply_fused_qk_head_rmsnorm_rotary(x, x, bad, good, None)
+        with pytest.raises(ValueError):
+            apply_fused_qk_head_rmsnorm_rotary(x, x, good, bad, None)
