@@ -161,12 +161,21 @@ def apply_fused_qk_rmsnorm_rope(query: torch.Tensor, key: torch.Tensor, query_no
     return q_out, k_out
 
 
+# Norms that subtract a mean (without bias they look like RMS norms otherwise).
+_OTHER_NORMS = (torch.nn.LayerNorm, torch.nn.GroupNorm, torch.nn.modules.batchnorm._NormBase)
+
+
 def _head_norm(what: str, x: torch.Tensor, norm: Any) -> tuple[torch.Tensor | None, float]:
     """Weight and eps of a norm over one head of ``x``."""
     weight = getattr(norm, "weight", None)
+    if isinstance(norm, torch.nn.RMSNorm):
+        if weight is None and norm.normalized_shape != x.shape[-1:]:
+            raise ValueError(f"{what}_norm must be over one head's width")
     # (asking torch.nn.RMSNorm for what it never has takes 2 us)
-    if not isinstance(norm, torch.nn.RMSNorm) and getattr(norm, "bias", None) is not None:
+    elif getattr(norm, "bias", None) is not None:
         raise ValueError(f"{what}_norm must have no bias")
+    elif isinstance(norm, _OTHER_NORMS):
+        raise ValueError(f"{what}_norm must be an RMS norm")
     eps = getattr(norm, "eps", None)
     if eps is None:
         if not isinstance(norm, torch.nn.RMSNorm):

@@ -427,3 +427,22 @@ def test_norms_without_an_eps_are_refused():
             apply_fused_qk_head_rmsnorm_rotary(x, x, bad, good, None)
         with pytest.raises(ValueError):
             apply_fused_qk_head_rmsnorm_rotary(x, x, good, bad, None)
+
+
+def test_what_is_no_rms_norm_of_one_head_is_refused():
+    """Norms that subtract a mean, or that go over more or fewer channels than a head has,
+    also where no weight's shape shows it."""
+    from eraserdit_b200.operator_fusion import apply_fused_qk_head_rmsnorm_rotary
+    x = torch.zeros(2, 6, 4, 64, device="cuda", dtype=torch.bfloat16)
+    kw = dict(device="cuda", dtype=torch.bfloat16)
+    good = torch.nn.RMSNorm(64, elementwise_affine=False, **kw)
+    apply_fused_qk_head_rmsnorm_rotary(x, x, good, good, None)
+    for bad in (torch.nn.LayerNorm(64, bias=False, **kw), torch.nn.LayerNorm(64, elementwise_affine=False, **kw),
+                torch.nn.GroupNorm(1, 64, affine=False, **kw), torch.nn.BatchNorm1d(64, affine=False, **kw),
+                torch.nn.RMSNorm(32, elementwise_affine=False, **kw),
+                torch.nn.RMSNorm((4, 64), elementwise_affine=False, **kw)):
+        for p in bad.parameters():
+            p.requires_grad_(False)
+        for pair in ((bad, good), (good, bad)):
+            with pytest.raises(ValueError):
+                apply_fused_qk_head_rmsnorm_rotary(x, x, *pair, None)
