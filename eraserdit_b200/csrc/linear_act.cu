@@ -205,7 +205,7 @@ constexpr float kErfcx6 = -0x1.35bb0ap-2f;
 constexpr float kErfcx7 = 0x1.1a2760p-4f;
 // gelu with the normal distribution function, x Phi(x): Phi(-|x|) =
 // erfc(|x| / sqrt(2)) / 2 keeps its digits where 1 + erf would cancel, and
-// costs 17 instructions and 2 MUFU where erfcf made the epilogue of a 2048-deep
+// costs 18 instructions and 2 MUFU where erfcf made the epilogue of a 2048-deep
 // product longer than its tile's products (2.37 against 1.58 ms).
 __device__ __forceinline__ float gelu_erf(float x) {
   const float t = __fdividef(1.0f, fmaf(kErfcxP, fabsf(x), 1.0f));
@@ -217,7 +217,7 @@ __device__ __forceinline__ float gelu_erf(float x) {
   q = fmaf(q, t, kErfcx1);
   q = fmaf(q, t, kErfcx0);
   const float below = 0.5f * q * t * ex2_approx(-0.72134752044448f * x * x);  // Phi(-|x|)
-  const float y = x * below;
+  const float y = fminf(x, 64.f) * below;  // at 64 `below` has long been 0; +inf * 0 is NaN
   return x > 0.f ? x - y : y;
 }
 

@@ -286,3 +286,33 @@ def test_overlapping_destinations_are_refused():
         linear_act(x[:1].expand(300, 128), w)
     with pytest.raises(ValueError):
         linear_act(x[:128], w, out=w)
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m", [1, 20, 3000])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_activations_of_infinities_and_nan(act, m, dtype):
+    """From an operand, from the bias and from a product that leaves FP32's range: what
+    the formula gives (+inf stays +inf under every activation)."""
+    from eraserdit_b200.linear import linear_act
+    values = torch.tensor([math.inf, -math.inf, math.nan, 1.0, -1.0, 0.0, 40.0, -40.0], device="cuda").to(dtype)
+    x = torch.zeros(m, 64, device="cuda", dtype=dtype)
+    w = torch.zeros(8, 64, device="cuda", dtype=dtype)
+    bias = values.clone()
+
+    def check(got, v):
+        want = _act(v.double(), act).expand(m, -1).to(dtype)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+        assert torch.equal(got.sign()[want.isinf()], want.sign()[want.isinf()])
+        finite = want.isfinite()
+        assert torch.allclose(got[finite].double(), want[finite].double(), rtol=0.01, atol=1e-6)
+
+    check(linear_act(x, w, bias, activation=act), bias)
+    x[:, 3] = 1
+    w[:, 3] = values
+    check(linear_act(x, w, activation=act), values)
+    if dtype == torch.bfloat16:
+        x[:, 3], w[:, 3] = 3e38, torch.tensor([3e38, -3e38, 1, 2, 3, 4, 5, 6], device="cuda").to(dtype)
+        got = linear_act(x, w, activation=act)
+        assert bool((got[:, 0] == math.inf).all())
+        assert bool((got[:, 1] == 0).all() if act == "relu" else (~got[:, 1].isfinite()).all())
