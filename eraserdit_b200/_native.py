@@ -239,11 +239,15 @@ def status_word(device: torch.device) -> torch.Tensor:
     """Per-device int32 word that kernels set when a bounded wait gives up."""
     index = device.index if device.index is not None else torch.cuda.current_device()
     word = _status.get(index)
-    if word is None:
-        word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
-        # zero before any stream's kernel looks at it
-        torch.cuda.current_stream(index).synchronize()
-        _status[index] = word
+    if word is not None:
+        return word
+    with _lock:  # a second word would leave the first caller's kernels a freed one
+        word = _status.get(index)
+        if word is None:
+            word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+            # zero before any stream's kernel looks at it
+            torch.cuda.current_stream(index).synchronize()
+            _status[index] = word
     return word
 
 
