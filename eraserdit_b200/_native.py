@@ -233,6 +233,25 @@ def refuse_gradients(what: str, *tensors) -> None:
 
 
 _status: dict[int, torch.Tensor] = {}
+# Words of calls that a CUDA graph recorded before their device had its own.
+_captured_status: dict[int, list[torch.Tensor]] = {}
+
+
+def _capturing(index: int) -> bool:
+    with torch.cuda.device(index):
+        return torch.cuda.is_current_stream_capturing()
+
+
+def _captured_word(index: int) -> torch.Tensor:
+    """A word for one recorded call, cleared by the graph itself before that call's
+    kernels: the device's word cannot be made now, as nothing may wait for its zero."""
+    device = torch.device("cuda", index)
+    word = torch.zeros(1, dtype=torch.int32, device=device)
+    with torch.cuda.stream(torch.cuda.Stream(device)):  # not recorded: 0 until the first replay
+        word.zero_()
+    with _lock:
+        _captured_status.setdefault(index, []).append(word)
+    return word
 
 
 def status_word(device: torch.device) -> torch.Tensor:
@@ -241,6 +260,8 @@ def status_word(device: torch.device) -> torch.Tensor:
     word = _status.get(index)
     if word is not None:
         return word
+    if _capturing(index):
+        return _captured_word(index)
     with _lock:  # a second word would leave the first caller's kernels a freed one
         word = _status.get(index)
         if word is None:
@@ -252,23 +273,22 @@ def status_word(device: torch.device) -> torch.Tensor:
 
 
 def status_pointer(device: torch.device) -> int:
-    """Address of the device's status word.  It is made by the first call on a
-    device, which can therefore not be one that a CUDA graph records."""
-    index = device.index if device.index is not None else torch.cuda.current_device()
-    word = _status.get(index)
-    if word is None:
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("call the operator once on this device before capturing it")
-        word = status_word(device)
-    return word.data_ptr()
+    """Address of the device's status word."""
+    return status_word(device).data_ptr()
 
 
 def read_status(device: torch.device, reset: bool = True) -> int:
     """Synchronise and return the device status bits (0 = no kernel timed out)."""
-    word = status_word(device)
-    value = int(word.item())
-    if reset and value:
-        word.zero_()
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    words = [status_word(device), *_captured_status.get(index, ())]
+    if len(words) > 1:
+        torch.cuda.synchronize(index)  # graphs replay on any stream
+    value = 0
+    for word in words:
+        bits = int(word.item())
+        if reset and bits:
+            word.zero_()
+        value |= bits
     return value
 
 
