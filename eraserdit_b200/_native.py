@@ -18,6 +18,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIBRARY_PATH = Path(__file__).resolve().parent / "liberaserdit_b200.so"
 ABI_VERSION = 6
@@ -223,13 +224,19 @@ def refuse_overlap(what: str, out: torch.Tensor, inputs, in_place: torch.Tensor 
 
 
 def refuse_gradients(what: str, *tensors) -> None:
-    """The operators have no backward pass: an input that wants a gradient while
-    gradients are recorded is an error, not a silently detached result."""
+    """The operators have no backward pass and no forward derivative: an input that wants
+    a gradient while gradients are recorded, or that carries a tangent, is an error, not a
+    silently detached result."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise ValueError(f"{what} has no backward pass: call it under torch.no_grad() or "
                                  "with detached inputs")
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # within a dual level
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{what} has neither a backward pass nor a forward derivative: "
+                                 "call it with primal inputs")
 
 
 _status: dict[int, torch.Tensor] = {}

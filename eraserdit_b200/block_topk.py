@@ -121,8 +121,7 @@ def block_topk_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Te
     if not 0.0 < softmax_scale < float("inf"):
         raise ValueError("softmax_scale must be positive and finite")
     _check_lengths(key_lengths, key)
-    if torch.is_grad_enabled():
-        _native.refuse_gradients("block_topk_attention", query, key, value)
+    _native.refuse_gradients("block_topk_attention", query, key, value)
     if key_pool is not None:
         _check_means(key_pool, key, key_block)
     device, dtype = query.device, query.dtype
