@@ -224,9 +224,9 @@ def refuse_overlap(what: str, out: torch.Tensor, inputs, in_place: torch.Tensor 
 
 
 def refuse_gradients(what: str, *tensors) -> None:
-    """The operators have no backward pass and no forward derivative: an input that wants
-    a gradient while gradients are recorded, or that carries a tangent, is an error, not a
-    silently detached result."""
+    """The operators have no backward pass and no forward derivative: an input or a
+    destination that wants a gradient while gradients are recorded, or that carries a
+    tangent, is an error, not a silently detached result."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:

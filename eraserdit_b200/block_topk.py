@@ -71,7 +71,7 @@ def pool_key_blocks(key: torch.Tensor, key_block: int = 64, *,
     if key_block not in KEY_BLOCKS:
         raise ValueError(f"key_block must be one of {KEY_BLOCKS}")
     _check_lengths(key_lengths, key)
-    _native.refuse_gradients("pool_key_blocks", key)
+    _native.refuse_gradients("pool_key_blocks", key, out)
     batch, length, heads, _ = key.shape
     if out is None:
         out = torch.empty(batch, heads, -(-length // key_block), HEAD_DIM, device=key.device,
@@ -121,7 +121,7 @@ def block_topk_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Te
     if not 0.0 < softmax_scale < float("inf"):
         raise ValueError("softmax_scale must be positive and finite")
     _check_lengths(key_lengths, key)
-    _native.refuse_gradients("block_topk_attention", query, key, value)
+    _native.refuse_gradients("block_topk_attention", query, key, value, out)
     if key_pool is not None:
         _check_means(key_pool, key, key_block)
     device, dtype = query.device, query.dtype

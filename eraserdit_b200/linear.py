@@ -177,7 +177,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
                     ("out", out)):
         if t is not None and (t.dtype != dtype or t.device != device):
             raise ValueError(f"{what} must have x's type and device")
-    _native.refuse_gradients("linear_act", x, weight, bias, gate, residual)
+    _native.refuse_gradients("linear_act", x, weight, bias, gate, residual, out)
     if bias is not None and (bias.shape != (n,) or not bias.is_contiguous()):
         raise ValueError("bias must be a contiguous [n] tensor")
     if residual is not None and residual.shape != shape:

@@ -302,7 +302,7 @@ def head_rotary_call(what: str, query, key, rotary, positions, q_weight, k_weigh
     if key is not None:
         k_strides = _check_heads("key", key, query)
         kv_heads, k_ptr = key.shape[2], key.data_ptr()
-    _native.refuse_gradients(what, query, key, q_weight, k_weight)
+    _native.refuse_gradients(what, query, key, q_weight, k_weight, query_out, key_out)
     if rotary is not None:
         if not isinstance(rotary, RotaryPositions):
             raise ValueError("rotary must be a RotaryPositions")
