@@ -203,13 +203,19 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     ldr = 0 if residual is None else _row_stride("residual", residual)
     if ldx is None or ldy is None or ldr is None:
         # rows that no single stride walks, e.g. prefixes [B, L, k] of wider slots:
-        # one product per leading index
-        if x.dim() < 3 or (gate is not None and gate.dim() == 2 and gate.shape[0] != x.shape[0]):
+        # one product per leading index, each with its part of the gate
+        lead, groups = x.shape[0], 1 if gate is None or gate.dim() == 1 else gate.shape[0]
+        if x.dim() < 3:
             raise ValueError("x, residual and out must be viewable as [rows, last dim] with one "
                              "row stride")
-        for i in range(x.shape[0]):
-            linear_act(x[i], weight, bias, activation=activation,
-                       gate=gate[i] if gate is not None and gate.dim() == 2 else gate,
+        if groups % lead and lead % groups:
+            raise ValueError("a gate's group may not end within one leading index of rows "
+                             "without a common stride")
+        for i in range(lead):
+            part = gate
+            if groups > 1:
+                part = gate[i * groups // lead:max((i + 1) * groups // lead, i * groups // lead + 1)]
+            linear_act(x[i], weight, bias, activation=activation, gate=part,
                        residual=None if residual is None else residual[i], out=out[i])
         return out
     if ldx < k or ldw < k or ldy < n or (residual is not None and ldr < n):

@@ -316,3 +316,30 @@ def test_activations_of_infinities_and_nan(act, m, dtype):
         got = linear_act(x, w, activation=act)
         assert bool((got[:, 0] == math.inf).all())
         assert bool((got[:, 1] == 0).all() if act == "relu" else (~got[:, 1].isfinite()).all())
+
+
+@pytest.mark.parametrize("lead,groups", [(4, 1), (4, 2), (4, 4), (4, 8), (3, 6)])
+def test_gates_of_slots(lead, groups):
+    """Rows that no single stride walks (prefixes of wider slots), with every number of
+    gate groups that the rows divide into at a slot's end or within one."""
+    from eraserdit_b200.linear import linear_act
+    x, w, b, gate, res = _operands(lead * 30, 136, 128, torch.bfloat16, 31, groups=groups, residual=True)
+    wide = torch.randn(lead, 50, 128, device="cuda").bfloat16()
+    wide[:, :30] = x.view(lead, 30, 128)
+    got = linear_act(wide[:, :30], w, b, activation="silu", gate=gate, residual=res.view(lead, 30, 136))
+    assert got.shape == (lead, 30, 136)
+    _check(got, x, w, b, "silu", gate, res)
+    # two leading dimensions
+    if lead == 4:
+        deep = wide.view(2, 2, 50, 128)[:, :, :30]
+        again = linear_act(deep, w, b, activation="silu", gate=gate, residual=res.view(2, 2, 30, 136))
+        assert torch.equal(again.view(lead, 30, 136), got)
+
+
+def test_gate_groups_across_slots_are_refused():
+    from eraserdit_b200.linear import linear_act
+    wide = torch.zeros(3, 50, 128, device="cuda", dtype=torch.bfloat16)
+    w, gate = (torch.zeros(s, 128, device="cuda", dtype=torch.bfloat16) for s in (128, 2))
+    with pytest.raises(ValueError):
+        linear_act(wide[:, :30], w, gate=gate)  # 45 rows each: one and a half slots
+    linear_act(wide[:, :30].contiguous(), w, gate=gate)
