@@ -175,7 +175,7 @@ def pack(name: str, *fields) -> bytes:
     layout = STRUCTS[name]
     try:
         return layout.pack(layout.size, *fields)
-    except (struct.error, OverflowError) as error:  # a number beyond its field
+    except struct.error as error:  # a size beyond its field
         raise ValueError(f"{name}: {error}") from None
 
 
