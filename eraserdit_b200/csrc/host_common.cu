@@ -46,11 +46,22 @@ int encode_tensor_map(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t rank
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return kErrTensorMap;
   cuuint32_t elem_strides[5] = {1, 1, 1, 1, 1};
-  CUresult r = fn(map, dtype, rank, base, reinterpret_cast<const cuuint64_t*>(dims),
-                  reinterpret_cast<const cuuint64_t*>(strides_bytes),
-                  reinterpret_cast<const cuuint32_t*>(box), elem_strides,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return fn(map, dtype, rank, base, reinterpret_cast<const cuuint64_t*>(dims),
+              reinterpret_cast<const cuuint64_t*>(strides_bytes),
+              reinterpret_cast<const cuuint32_t*>(box), elem_strides,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
+    // A host thread whose first CUDA call this is: the driver wants the context that
+    // the runtime binds to a thread only with its first launch or device choice.
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess)
+      return kErrTensorMap;
+    r = encode();
+  }
   return r == CUDA_SUCCESS ? kErrOk : kErrTensorMap;
 }
 
