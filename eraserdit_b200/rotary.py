@@ -303,7 +303,7 @@ def head_rotary_call(what: str, query, key, rotary, positions, q_weight, k_weigh
         k_strides = _check_heads("key", key, query)
         kv_heads, k_ptr = key.shape[2], key.data_ptr()
     _native.refuse_gradients(what, query, key, q_weight, k_weight, query_out, key_out)
-    if rotary is not None:
+    if rotary is not None or not norm:
         if not isinstance(rotary, RotaryPositions):
             raise ValueError("rotary must be a RotaryPositions")
         if rotary.head_dim != dim:

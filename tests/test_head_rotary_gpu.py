@@ -446,3 +446,14 @@ def test_what_is_no_rms_norm_of_one_head_is_refused():
         for pair in ((bad, good), (good, bad)):
             with pytest.raises(ValueError):
                 apply_fused_qk_head_rmsnorm_rotary(x, x, *pair, None)
+
+
+def test_a_rotation_without_positions_is_refused():
+    """None stands for the norm alone, in the operator that has a norm."""
+    from eraserdit_b200.operator_fusion import apply_fused_qk_head_rmsnorm_rotary
+    from eraserdit_b200.rotary import apply_rotary
+    x = torch.zeros(2, 6, 4, 64, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        apply_rotary(x, x, None, 0)
+    norm = torch.nn.RMSNorm(64, device="cuda", dtype=torch.bfloat16).requires_grad_(False)
+    apply_fused_qk_head_rmsnorm_rotary(x, x, norm, norm, None)
