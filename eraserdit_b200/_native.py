@@ -223,6 +223,12 @@ def refuse_overlap(what: str, out: torch.Tensor, inputs, in_place: torch.Tensor 
             raise ValueError(f"{what} overlaps an input")
 
 
+def written(out: torch.Tensor) -> None:
+    """A caller's destination is written in place: autograd refuses what it saved of it."""
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+
+
 def refuse_gradients(what: str, *tensors) -> None:
     """The operators have no backward pass and no forward derivative: an input or a
     destination that wants a gradient while gradients are recorded, or that carries a

@@ -79,6 +79,7 @@ def pool_key_blocks(key: torch.Tensor, key_block: int = 64, *,
     else:
         _check_means(out, key, key_block)
         _native.refuse_overlap("out", out, (key, key_lengths))
+        _native.written(out)
     if out.numel():
         _native.call("erd_block_key_means", key.device, _native.DTYPE_CODES[key.dtype],
                      key.data_ptr(), *_strides("key", key), batch, heads, length, key_block,
@@ -132,6 +133,7 @@ def block_topk_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Te
         raise ValueError("out must have the query's shape, type and device")
     else:
         _native.refuse_overlap("out", out, (key, value, key_lengths, key_pool), query)
+        _native.written(out)
     if not return_selection:  # no list is wider than the blocks there are
         topk = min(topk, max(1, -(-kv_len // key_block)))
     selection = query.new_empty((batch, heads, groups, topk), dtype=torch.int32)

@@ -188,6 +188,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
         raise ValueError("out must be [..., n] and no expanded view")
     else:
         _native.refuse_overlap("out", out, (x, weight, bias, gate), residual)
+        _native.written(out)
     m = x.numel() // k
     gate_rows = 0
     if gate is not None:

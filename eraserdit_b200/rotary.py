@@ -322,12 +322,14 @@ def head_rotary_call(what: str, query, key, rotary, positions, q_weight, k_weigh
     else:
         q_out, qo_strides = query_out, _check_out("query_out", query_out, query)
         _native.refuse_overlap("query_out", q_out, (key, q_weight, k_weight), query)
+        _native.written(q_out)
     if key is not None:
         if key_out is None:
             k_out, ko_strides = _new_out(key)
         else:
             k_out, ko_strides = key_out, _check_out("key_out", key_out, key)
             _native.refuse_overlap("key_out", k_out, (query, q_out, q_weight, k_weight), key)
+            _native.written(k_out)
         ko_ptr = k_out.data_ptr()
     elif key_out is not None:
         raise ValueError("key_out needs a key")
