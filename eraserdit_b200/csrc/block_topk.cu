@@ -460,10 +460,13 @@ __global__ void __launch_bounds__(128)
 // written over the scores it came from.
 //
 // A CTA's steps are a chain (S ready -> softmax -> P V and the next Q K -> S
-// ready) of which the exponentials (8192 a step, 16 a clock and multiprocessor)
-// are 512 clocks at least.  Four chains keep that unit and the tensor cores
-// busy where two (with their buffers doubled instead) reached 65 % and 32 %:
-// 1.59 ms at 32640 tokens x 32 heads, 64 of 510 blocks.
+// ready).  Its exponentials take 384 clocks at least (8192 a step, of which MUFU
+// does three quarters at 16 a clock and multiprocessor).  Two chains, with their
+// buffers doubled, had MUFU at 65 % and the tensor cores at 32 % and took 1.59 ms
+// at 32640 tokens x 32 heads, 64 of 510 blocks; four take 1.24 ms with 61 % and
+// 40 %.  So no unit is full: with one score buffer a CTA's products and its softmax
+// never run together, and four CTAs do not cover each other's waits.  Where there
+// are fewer tiles than slots, one chain's length is the time: about 2 us a step.
 //
 // The chain also orders everything else.  When every row's P of step j has
 // arrived, S(j) had been ready, so Q K(j) and P V(j - 1) had completed: their

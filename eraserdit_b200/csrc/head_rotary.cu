@@ -199,7 +199,8 @@ __device__ __forceinline__ Two fma(Two a, Two b, Two c) {
 // coefficients are computed two values at a time (the rotation alone is not: a factor's
 // sign is free in the plain form, and eight registers fewer let 32 warps reside),
 // addresses advance by a constant, and weights and angles are read 16 bytes at a time:
-// 121 and 167 a group.
+// 121 and 167 a group.  The norm with 16-byte chunks is held at 80 registers, so that 24
+// warps reside; that spills one to three of them (4 to 12 bytes a thread).
 //
 // kAhead, the norm with eight groups or more a warp: it also asks L2 for the group
 // behind the next, which costs no registers: what 24 warps have requested at a time

@@ -183,7 +183,9 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
 }
 
 // x * sigmoid(z): the logistic function through 2^x and a reciprocal, both to
-// a few units in the last place of FP32 (a tanh instruction would keep 11 bits).
+// a few units in the last place of FP32 (a tanh instruction would keep 11 bits).  Below
+// z = -87.3 the quotient's divisor passes 2^126 and the result is 0, where the value is
+// under |x| 2^-126.
 __device__ __forceinline__ float times_sigmoid(float x, float z) {
   return __fdividef(x, 1.0f + ex2_approx(-1.4426950408889634f * z));
 }

@@ -419,7 +419,8 @@ int erd_attn_fwd_fp8_static_scratch(
  *   (y0, y1) -> (y0 c - y1 s, y0 s + y1 c) for each of the rotary_dim / 2 pairs,
  *   c = amplitude cos(2 pi t), s = amplitude sin(2 pi t) (s negated with
  *   `inverse`: the transposed rotation), t = position * turns[pair], evaluated
- *   and reduced in FP64; norm and rotation in FP32, one rounding.
+ *   and reduced to at most half a turn in FP64; sine, cosine, norm and rotation in
+ *   FP32, one rounding.
  * q [batch, tokens, q_heads, head_dim] and k [.., k_heads, ..] of `dtype`
  * (ERD_BF16, ERD_FP16, ERD_FP32) with a contiguous head (k may be NULL with
  * k_heads 0); q_out / k_out may be q / k themselves.  Pairs are channels

@@ -413,3 +413,22 @@ def test_topk_far_above_the_blocks_costs_nothing(query_block):
     for topk in (MAX_TOPK + 1, 2 ** 31 - 1, 2 ** 40):
         with pytest.raises(ValueError):
             block_topk_attention(q, k, v, SCALE, topk, query_block=query_block)
+
+
+def test_means_renewed_from_a_block_on_in_a_ragged_batch():
+    """An append to kept keys whose rest holds anything: the blocks from the first that
+    changed are renewed with what is left of each length there."""
+    from eraserdit_b200.block_topk import pool_key_blocks
+    keys = torch.full((3, 512, 2, 64), math.nan, device="cuda", dtype=torch.bfloat16)
+    old, new = [200, 70, 0], [330, 75, 64]
+    _, k, _ = _inputs(3, 1, 512, 2, 2, torch.bfloat16, 16)
+    for b, n in enumerate(old):
+        keys[b, :n] = k[b, :n]
+    pool = pool_key_blocks(keys, key_lengths=torch.tensor(old, dtype=torch.int32, device="cuda"))
+    for b, n in enumerate(new):
+        keys[b, :n] = k[b, :n]
+    lengths = torch.tensor(new, dtype=torch.int32, device="cuda")
+    i = min(n // 64 for n in old)
+    pool[:, :, i:] = pool_key_blocks(keys[:, i * 64:], key_lengths=lengths - i * 64)
+    assert torch.equal(pool, pool_key_blocks(keys, key_lengths=lengths))
+    assert bool(torch.isfinite(pool).all())
