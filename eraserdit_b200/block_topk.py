@@ -24,6 +24,7 @@ HEAD_DIM = 64
 QUERY_BLOCKS = (1, 128)
 KEY_BLOCKS = (64, 128)
 MAX_TOPK = 0x7fff0000
+MIN_SCALE, MAX_SCALE = 2.0 ** -149, 2.3e38  # FP32's least, and what log2(e) times is finite
 
 
 def _strides(what: str, t: torch.Tensor) -> tuple[int, int, int]:
@@ -119,8 +120,8 @@ def block_topk_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Te
         raise ValueError(f"query_block must be one of {QUERY_BLOCKS}, key_block of {KEY_BLOCKS}")
     if not isinstance(topk, int) or not 1 <= topk <= MAX_TOPK:
         raise ValueError(f"topk must be an int from 1 to {MAX_TOPK}")
-    if not 0.0 < softmax_scale < float("inf"):
-        raise ValueError("softmax_scale must be positive and finite")
+    if not MIN_SCALE <= softmax_scale <= MAX_SCALE:
+        raise ValueError("softmax_scale must be positive and finite (in FP32, in base 2)")
     _check_lengths(key_lengths, key)
     _native.refuse_gradients("block_topk_attention", query, key, value, out)
     if key_pool is not None:

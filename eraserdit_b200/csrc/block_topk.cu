@@ -42,6 +42,7 @@ constexpr int kHalf = 64;      // keys that are loaded (and chosen) together at 
 // Most queries, keys and chosen blocks: the kernels' int indices step past these
 // by at most 128.
 constexpr int kMaxCount = 0x7fff0000;
+constexpr float kMaxScale = 2.3e38f;  // times log2(e) it is finite
 
 // ------------------------------------------------------------ small helpers
 template <typename T>
@@ -1379,7 +1380,7 @@ extern "C" int erd_block_topk_attn(const erd_block_topk_args* args, int* status,
       a.q_heads <= 0 || a.kv_heads <= 0 || a.q_heads % a.kv_heads != 0 || a.q_len <= 0 ||
       a.kv_len <= 0 || a.topk <= 0 || (a.query_block != 1 && a.query_block != btk::kTile) ||
       (a.key_block != 64 && a.key_block != 128) ||
-      !(a.softmax_scale > 0.f && a.softmax_scale <= 3.0e38f))
+      !(a.softmax_scale > 0.f && a.softmax_scale <= btk::kMaxScale))
     return kErrBadShape;
   if (a.batch > 65535 || a.q_heads > 65535 ||
       static_cast<long long>(a.batch) * a.q_heads > 65535 || a.kv_len > btk::kMaxCount ||

@@ -489,7 +489,7 @@ int erd_linear_act(const erd_linear_act_args* args, int* status, void* stream);
  * highest-scoring blocks with a valid key (all, if there are fewer; ties: the
  * lowest index; NaN ranks last), and its queries attend the valid keys of those:
  * out = softmax(q . k * softmax_scale) v, 0 where there is none
- * (softmax_scale positive and finite: masked keys are -inf times it).
+ * (softmax_scale positive and at most 2.3e38: masked keys are -inf times it).
  * q / out [batch, q_len, q_heads, 64], k / v [batch, kv_len, kv_heads, 64] of
  * `dtype` (ERD_BF16 or ERD_FP16), element strides, 16-byte aligned; query head h
  * reads key head h / (q_heads / kv_heads).  key_lengths: device int32 [batch]

@@ -95,3 +95,15 @@ def test_only_inputs_are_read_as_constant():
     reads = re.findall(r"__ldg\(([^;]*)", text)
     assert reads and all(r.startswith("lengths + b)") for r in reads)
     assert "__restrict__" not in text  # which would let the compiler choose such reads
+
+
+def test_scales_whose_base_2_form_is_infinite_are_refused():
+    """The kernels multiply by scale / ln 2: above 2.35e38 that leaves FP32's range, and
+    scores of 0 times it are NaN."""
+    from eraserdit_b200 import _native
+    fn = _native.load().erd_block_topk_attn
+    p = 1 << 20
+    for qb in (1, 128):
+        for scale in (2.4e38, 3.0e38, 3.4e38):
+            fields = (p, p, p, 0, 0, p, p, p, *([64] * 12), 1 << 20, 0, 1, 2, 1, 5, 70, 64, 3, qb, 64, scale)
+            assert fn(_native.pack("erd_block_topk_attn", *fields), None, None) == -2

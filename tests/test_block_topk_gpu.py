@@ -432,3 +432,17 @@ def test_means_renewed_from_a_block_on_in_a_ragged_batch():
     pool[:, :, i:] = pool_key_blocks(keys[:, i * 64:], key_lengths=lengths - i * 64)
     assert torch.equal(pool, pool_key_blocks(keys, key_lengths=lengths))
     assert bool(torch.isfinite(pool).all())
+
+
+@pytest.mark.parametrize("query_block", [1, 128])
+def test_scales_at_the_ends_of_their_range(query_block):
+    from eraserdit_b200.block_topk import block_topk_attention
+    q, k, v = _inputs(1, 130, 200, 1, 1, torch.bfloat16, 17)
+    for scale in (1e39, 2.4e38, 1e-50):
+        with pytest.raises(ValueError):
+            block_topk_attention(q, k, v, scale, 2, query_block=query_block)
+    # scores that all but vanish, and scores of 0 under the greatest scale: the mean of v
+    want = torch.stack([v[0, :, 0].double().mean(0)] * 130)
+    for scale, queries in ((1e-44, q), (2e38, torch.zeros_like(q))):
+        out = block_topk_attention(queries, k, v, scale, 4, query_block=query_block)
+        assert float((out[0, :, 0].double() - want).abs().max()) < 2.0 ** -8
